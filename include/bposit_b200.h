@@ -282,6 +282,110 @@ int bp_bp32_to_f64(const uint32_t *codes, int M, int N, const int32_t *row_exp,
 int bp_bp32_to_f32(const uint32_t *codes, int M, int N, const int32_t *row_exp, const int32_t *col_exp,
                    const float *bias, float *out, void *stream);
 
+/* ---- paged key-value cache -------------------------------------------------
+ * Keys and values of a batch of sequences, held as b-posit codes in pages of
+ * page_size tokens: k and v are [layers, pages, kv_heads, page_size, head_dim]
+ * codes (fmt 8: uint8, fmt 16: uint16).  With fmt 8 every (token, kv head) row
+ * has one power-of-two exponent, k_exp and v_exp [layers, pages, kv_heads,
+ * page_size] int8, and an element's value is value(code) * 2^exp; with fmt 16
+ * both are NULL.  Entry i of sequence b is row i % page_size of page
+ * page_table[b * max_pages + i / page_size], for i < lengths[b]; all layers
+ * share the table and the lengths.  A sequence's capacity is max_pages *
+ * page_size.  positions (the entries' rotary positions) and scores (the
+ * attention weight that each entry has received) are optional, [layers, batch,
+ * kv_heads, capacity], indexed by the entry and not by the page.  All arrays
+ * are contiguous device memory; k, v, k_exp and v_exp are 16-byte aligned.
+ * Every kernel checks what it reads on the device: a length outside [0,
+ * capacity] counts as the nearer bound, and a page number outside [0, pages)
+ * is never followed (each call says what it gives instead).
+ * head_dim: 32, 64, 96 or 128.  page_size: a power of two from 16 to 1024.
+ * No reference counterpart (the reference has no model and no cache). */
+typedef struct bp_kv_cache {
+  int32_t fmt;         /* 8 or 16 */
+  int32_t layers;
+  int32_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t batch;
+  int32_t max_pages;   /* page table columns */
+  void *k, *v;
+  int8_t *k_exp, *v_exp;
+  const int32_t *page_table;
+  const int32_t *lengths;
+  int32_t *positions;  /* optional */
+  float *scores;       /* optional */
+} bp_kv_cache;
+
+/* dtype of activations (q, new keys and values, attention output). */
+#define BP_F32 0
+#define BP_BF16 1
+#define BP_F16 2
+
+/* Writes `tokens` new keys and values into one layer of the cache, rotating
+ * queries and keys by their positions on the way.
+ * k, v: [tokens, kv_heads, head_dim] of `dtype`, rows of a token contiguous,
+ * token stride k_stride / v_stride elements; q (optional): [tokens, heads,
+ * head_dim], token stride q_stride, rotated into q_out [tokens, heads,
+ * head_dim] (contiguous).  16-byte aligned pointers, strides of a multiple of
+ * 16 bytes.
+ * cos, sin: fp32 [rope_rows, head_dim / 2]; the rotation of pair (i, i +
+ * head_dim/2) at position p is (a c - b s, b c + a s) in float64 with c, s
+ * from row p, rounded once to fp32 (and then to q_out's dtype).  Both NULL:
+ * keys are stored as given, and q must be NULL.  A position outside [0,
+ * rope_rows) rotates with NaN.
+ * Token t goes to entry places[t] of sequence seqs[t]; with both NULL, to the
+ * last entry (lengths[t] - 1) of sequence t, and tokens must equal batch.  A
+ * sequence, entry or page outside the cache drops the write of that token (its
+ * q row is still rotated).  Two tokens of a call must not share an entry.
+ * positions[t] is token t's rotary position (NULL: its place); where the cache
+ * keeps positions and scores they are set to it and to 0.
+ * fmt 8: exponent floor(log2(largest finite |x| of the row)) - 3, at least
+ * -126 (0 for a row without one), codes = bp8 round-to-nearest (ties to the
+ * smaller magnitude) of x / 2^exponent; fmt 16: bp16 round-to-nearest-even.
+ * NaN -> NaR, which reads back as zero; +-inf -> +-maxpos. */
+int bp_kv_append(const bp_kv_cache *cache, int layer, int dtype, int tokens, const void *k, int64_t k_stride,
+                 const void *v, int64_t v_stride, const void *q, int heads, int64_t q_stride, const float *cos,
+                 const float *sin, int rope_rows, const int32_t *positions, const int32_t *seqs,
+                 const int32_t *places, void *q_out, void *stream);
+
+/* Attention of one new token per sequence over one layer of the cache:
+ *   out[b, h] = sum_i softmax_i(scale * q[b, h] . k[b, i, h / G]) v[b, i, h / G]
+ * over the entries i < lengths[b], G = heads / kv_heads.  q: [batch, heads,
+ * head_dim] of `dtype` with batch stride q_stride (16-byte aligned, stride a
+ * multiple of 16 bytes); out: [batch, heads, head_dim] of the same dtype,
+ * contiguous; lse (optional): fp32 [batch, heads], the natural logarithm of the
+ * softmax's denominator.  An empty sequence gives zeros (lse -inf); one with a
+ * page number outside the pool gives NaN.
+ * accumulate = 1 also adds the softmax weight of each entry, summed over the
+ * heads that share its kv head, to cache->scores (not for a sequence with a
+ * page number outside the pool).  Products are exact in fp32 or better, sums,
+ * softmax statistics and scores are fp32.  Entries at or past max_length are
+ * left out (0: capacity); it bounds the workspace.
+ * workspace: at least bp_paged_attention_workspace_size() bytes, 256-byte
+ * aligned; NULL takes it stream-ordered from the device's memory pool. */
+int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype, int heads, const void *q, int64_t q_stride,
+                       void *out, float *lse, float scale, int max_length, int accumulate, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* Workspace bytes bp_paged_attention needs. */
+size_t bp_paged_attention_workspace_size(const bp_kv_cache *cache, int heads, int max_length, int accumulate);
+
+/* Cuts every (layer, sequence, kv head) with more than `budget` entries down to
+ * the `budget` best of them, in place.  Entries rank by weights [layers, batch,
+ * kv_heads, capacity] (NULL: cache->scores), larger first, equal ones by lower
+ * place, NaN behind everything; entries whose position is below `sinks`, or
+ * within `recent` of the row's largest position, rank as +inf.  Kept entries at places
+ * >= budget move, in order, into the places < budget that were given up, with
+ * their keys, values, exponents, positions and scores; places >= budget keep
+ * their old contents.  keep (optional): int32 [layers, batch, kv_heads,
+ * budget], the place each entry came from, -1 past the length.  lengths is not
+ * written: the caller sets it to min(lengths, budget).  A row that cannot move
+ * an entry because a page number is outside the pool skips that entry's codes.
+ * The pages of a sequence must not be shared with another one. */
+int bp_kv_evict(const bp_kv_cache *cache, const float *weights, int budget, int recent, int sinks, int32_t *keep,
+                void *stream);
+
 #ifdef __cplusplus
 }
 #endif

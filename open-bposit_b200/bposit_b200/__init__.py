@@ -6,7 +6,7 @@ behind a C ABI, with drop-in mirrors of the reference's Python API:
 """
 from __future__ import annotations
 
-__all__ = ["bposit_fast", "bposit_quantize", "bposit_ref", "ops", "workloads", "dist"]
+__all__ = ["bposit_fast", "bposit_quantize", "bposit_ref", "ops", "workloads", "dist", "kv"]
 __version__ = "0.1.0"
 
 

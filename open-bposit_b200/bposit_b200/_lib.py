@@ -88,6 +88,11 @@ def lib() -> ctypes.CDLL:
             "bp_ipc_close": ([vp], i32),
             "bp_quire_gemm_noalloc": ([i32, vp, vp, i32, i32, i32, vp, vp, i32, vp, i64, vp, i32, vp], i32),
             "bp_bp32_to_f64": ([vp, i32, i32, vp, vp, vp, vp], i32),
+            "bp_kv_append": ([vp, i32, i32, i32, vp, i64, vp, i64, vp, i32, i64, vp, vp, i32, vp, vp, vp, vp,
+                              vp], i32),
+            "bp_paged_attention": ([vp, i32, i32, i32, vp, i64, vp, vp, ctypes.c_float, i32, i32, vp, sz, vp], i32),
+            "bp_paged_attention_workspace_size": ([vp, i32, i32, i32], sz),
+            "bp_kv_evict": ([vp, vp, i32, i32, i32, vp, vp], i32),
         }
         for name, (args, res) in sig.items():
             f = getattr(L, name)
@@ -105,7 +110,7 @@ EXPORTED = (
     "bp_quire_gemm", "bp_quire_gemm_f32",
     "bp_quire_gemm_workspace_size", "bp_quire_gemm_multi", "bp_enable_peer_access",
     "bp_ipc_alloc", "bp_ipc_free", "bp_ipc_open", "bp_ipc_close", "bp_quire_gemm_noalloc",
-    "bp_bp32_to_f64",
+    "bp_bp32_to_f64", "bp_kv_append", "bp_paged_attention", "bp_paged_attention_workspace_size", "bp_kv_evict",
 )
 
 

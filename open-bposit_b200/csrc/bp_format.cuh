@@ -180,6 +180,55 @@ BP_HD uint32_t bp8_apply(QEntry q, uint32_t M) {
   return (q.lo_sh & 0xFFu) + (M >> sh) + ((M & mask) > q.thr ? 1u : 0u);
 }
 
+// bp8 code of x / 2^e for fp32 bits u: the round-to-nearest rule of bp8_qentry
+// (ties to the smaller magnitude, nonzero stays nonzero, saturation, NaN ->
+// NaR) in closed form, on the exponent and mantissa so that no scaled value is
+// formed (it could leave fp32's range).  With |x| = 1.M * 2^E, E in [-16, 15]
+// keeps both exponent bits, codes are evenly spaced in the binade and the field
+// is base + (M rounded to its fraction bits, half down); outside, the last
+// codes are 2^-24, 2^-20, 2^-18, 2^-16 and 2^16, 2^18, 2^20, 2^24, told apart by
+// their midpoints.
+BP_HD uint32_t bp8_encode_exp(uint32_t u, int e) {
+  uint32_t a = u & 0x7FFFFFFFu;
+  if (a == 0u) return 0u;
+  if (a > 0x7F800000u) return 0x80u;
+  uint32_t m;
+  if (a == 0x7F800000u) {
+    m = 127u;
+  } else {
+    int E;
+    if (a < 0x00800000u) {             // subnormal: shift the leading bit up to bit 23
+      const int sh = clz32(a) - 8;
+      a <<= sh;
+      E = -126 - sh;
+    } else {
+      E = (int)(a >> 23) - 127;
+    }
+    E -= e;
+    const uint32_t M = a & 0x7FFFFFu;
+    if (E >= -16 && E < 16) {
+      const int k = E >> 2;
+      const int avail = k >= 0 ? 5 - k : 6 + k;             // bits after the regime, 2 .. 5
+      const int sh = 25 - avail;                            // 23 - fraction bits
+      const uint32_t R = k >= 0 ? (2u << (k + 1)) - 2u : 1u;
+      m = (R << avail) + ((uint32_t)(E & 3) << (avail - 2)) + ((M + (1u << (sh - 1)) - 1u) >> sh);
+    } else {
+      E = E < -32 ? -32 : (E > 32 ? 32 : E);                // past the last codes, and the key fits an int
+      const int key = E * (1 << 23) + (int)M;
+      m = E > 0 ? 124u + (key > 17 * (1 << 23) + 0x200000) + (key > 19 * (1 << 23) + 0x200000) +
+                      (key > 23 * (1 << 23) + 0x080000)
+                : 1u + (key > -21 * (1 << 23) + 0x080000) + (key > -19 * (1 << 23) + 0x200000) +
+                      (key > -17 * (1 << 23) + 0x200000);
+    }
+  }
+  return (u >> 31) ? 256u - m : m;
+}
+
+// floor(log2 |x|) of a finite nonzero fp32 magnitude's bits.
+BP_HD int f32_floor_log2(uint32_t a) {
+  return a < 0x00800000u ? -118 - clz32(a) : (int)(a >> 23) - 127;
+}
+
 // ---------------------------------------------------------------------------
 // fp32 -> bp16, the bit-string encoder _encode_unsigned(value, mode) of
 // reference/bposit_ref.py:382-486 on the exact value of x: regime, up to three
