@@ -1,139 +1,102 @@
 // bp_kv_attend.cu -- attention of one new token per sequence over the paged
-// b-posit key-value cache (bp_paged_attention).
+// b-posit key-value cache (bp_paged_attention): the entry
+// points, and the kernels that finish what k_kv_attend (bp_kv_attend.cuh) leaves in
+// parts.
 #include <math.h>
 
-#include "bp_kv.cuh"
+#include "bp_kv_attend.cuh"
 
 namespace bp {
 namespace {
 
-struct AttendParams {
-  KvView c;
-  int heads, group;          // query heads, query heads per kv head
-  int max_len;
-  const void *q;
-  int64_t qs;                // batch stride of q, elements
-  void *out;
-  float *lse;
-  float scale;               // of the scores, times log2(e)
-  float *raw;                // workspace: lse2 [batch, heads] when scores are accumulated
-};
-
-__device__ __forceinline__ float code_value(const KvView &c, const uint8_t *pool, int64_t at) {
-  return __uint_as_float(c.fmt == 8 ? posit_to_f32_bits<8, 2>(pool[at])
-                                    : bp16_to_f32_bits(reinterpret_cast<const uint16_t *>(pool)[at]));
-}
-
-// One block per (sequence, head); its warps take entries in turn, a warp's
-// lanes share an entry's dot product, and the warps' running maxima, sums and
-// outputs are joined at the end.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_attend_simple(AttendParams p) {
-  constexpr int E = D / 32;
-  const KvView &c = p.c;
-  const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = min(c.length(b), p.max_len), hk = h / p.group;
-  __shared__ float s_m[4], s_l[4], s_o[4][D];
-  float q[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    q[i] = to_f32(((const T *)p.q)[b * p.qs + h * D + lane * E + i]);
-    o[i] = 0.0f;
-  }
-  bool bad = false;
-  for (int i = warp; i < n; i += 4) {
-    const int page = c.page_of(b, i);
-    if (page < 0) {
-      bad = true;
-      continue;
-    }
-    const int64_t row = c.row(page, hk, i);
-    float s = 0.0f;
-#pragma unroll
-    for (int j = 0; j < E; ++j) s = fmaf(q[j], code_value(c, c.k, row * D + lane * E + j), s);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-    s *= p.scale;
-    if (c.k_exp) s *= exp2_int(c.k_exp[row]);
-    const float mn = fmaxf(m, s), a = exp2f(m - mn), w = exp2f(s - mn);
-    const float wv = c.v_exp ? w * exp2_int(c.v_exp[row]) : w;
-    m = mn;
-    l = fmaf(l, a, w);
-#pragma unroll
-    for (int j = 0; j < E; ++j) o[j] = fmaf(o[j], a, wv * code_value(c, c.v, row * D + lane * E + j));
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int j = 0; j < E; ++j) s_o[warp][lane * E + j] = o[j];
-  bad = __syncthreads_or(bad);
-  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float den = 0.0f, a[4];
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    a[w] = s_m[w] == -INFINITY && s_l[w] == 0.0f ? 0.0f : exp2f(s_m[w] - top);
-    den = fmaf(s_l[w], a[w], den);
-  }
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float x = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) x = fmaf(s_o[w][d], a[w], x);
-    x = n == 0 ? 0.0f : x / den;
-    if (bad) x = NAN;
-    ((T *)p.out)[((int64_t)b * p.heads + h) * D + d] = from_f32<T>(x);
-  }
-  if (threadIdx.x == 0) {
-    const float lse2 = bad ? NAN : (n == 0 ? -INFINITY : top + log2f(den));
-    if (p.lse) p.lse[b * p.heads + h] = lse2 * 0.6931471805599453f;
-    if (p.raw) p.raw[b * p.heads + h] = lse2;
-  }
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_scores_simple(AttendParams p) {
-  const KvView &c = p.c;
-  const int hk = blockIdx.x, b = blockIdx.y;
-  const int n = min(c.length(b), p.max_len);
-  if (n == 0 || isnan(p.raw[b * p.heads + hk * p.group])) return;
-  for (int i = threadIdx.x; i < n; i += 128) {
-    const int page = c.page_of(b, i);
-    if (page < 0) continue;
-    const int64_t row = c.row(page, hk, i);
-    const float ke = c.k_exp ? exp2_int(c.k_exp[row]) : 1.0f;
-    float w = 0.0f;
-    for (int g = 0; g < p.group; ++g) {
-      const T *q = (const T *)p.q + b * p.qs + (hk * p.group + g) * D;
-      float s = 0.0f;
-      for (int d = 0; d < D; ++d) s = fmaf(to_f32(q[d]), code_value(c, c.k, row * D + d), s);
-      w += exp2f(s * p.scale * ke - p.raw[b * p.heads + hk * p.group + g]);
-    }
-    c.scores[((int64_t)b * c.kv_heads + hk) * c.cap + i] += w;
-  }
-}
-
-template <typename T, int D>
-int launch_attend(const AttendParams &p, cudaStream_t s) {
-  k_attend_simple<T, D><<<dim3(p.heads, p.c.batch), 128, 0, s>>>(p);
-  int rc = check_launch("k_attend_simple");
-  if (rc != kOk || !p.raw) return rc;
-  k_scores_simple<T, D><<<dim3(p.c.kv_heads, p.c.batch), 128, 0, s>>>(p);
-  return check_launch("k_scores_simple");
-}
-
+// Joins the parts of a row that several CTAs of k_kv_attend worked on: block c
+// takes the row that starts in CTA c's range and goes on behind it.  Launched
+// early (programmatic dependent launch), so its latency hides behind the main
+// kernel; the parts of a row are few and in L2.
 template <typename T>
-int launch_attend_dim(const AttendParams &p, cudaStream_t s) {
-  switch (p.c.dim) {
-    case 32: return launch_attend<T, 32>(p, s);
-    case 64: return launch_attend<T, 64>(p, s);
-    case 96: return launch_attend<T, 96>(p, s);
-    default: return launch_attend<T, 128>(p, s);
+__global__ void __launch_bounds__(256) k_kv_join(AttendParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 open = p.cta_row[blockIdx.x];
+  if (open.x < 0) return;
+  const int D = p.c.dim, rec = kHeadsPerRow * D;
+  // the first part is the CTA's second record (a row that starts there), the others are first records
+  const float *first = p.cta_rec + ((int64_t)blockIdx.x * 2 + 1) * (rec + 16);
+  const int64_t step = 2 * (rec + 16);
+  for (int e = threadIdx.x; e < rec; e += 256) {
+    const int h = e / D;
+    float M = -INFINITY, L = 0.0f, O = 0.0f;
+    for (int k = 0; k < open.y; ++k) {
+      const float *r = first + k * step - (k ? rec + 16 : 0);
+      M = fmaxf(M, r[rec + h]);
+    }
+    for (int k = 0; k < open.y; ++k) {
+      const float *r = first + k * step - (k ? rec + 16 : 0);
+      const float a = ex2(r[rec + h] - M);
+      L = fmaf(r[rec + 8 + h], a, L);
+      O = fmaf(r[e], a, O);
+    }
+    write_out<T>(p, open.x, h, e - h * D, D, O / L);
+    if (e % D == 0) write_lse(p, open.x, h, M + log2f(L));
   }
 }
 
-size_t workspace_bytes_of(const KvView &c, int heads, int max_len, bool accumulate) {
-  return accumulate ? (size_t)c.batch * heads * 4 : 0;
+// scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2):
+// one thread per entry, so the sum has one order and needs no atomics.
+__global__ void __launch_bounds__(256) k_kv_scores(AttendParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int bk = blockIdx.y, b = bk / p.c.kv_heads;
+  const int n = min(p.c.length(b), p.max_len);
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float w = 0.0f;
+  for (int ch = 0; ch < p.chunks; ++ch) {
+    const int64_t row = (int64_t)bk * p.chunks + ch;
+    const float *raw = p.raw + (row * p.max_len + i) * p.gp;
+    const int heads = min(kHeadsPerRow, p.group - ch * kHeadsPerRow);
+    for (int h = 0; h < heads; h += 2) {
+      const float2 s = *reinterpret_cast<const float2 *>(raw + h);
+      w += ex2(s.x - p.lse2[row * kHeadsPerRow + h]);
+      if (h + 1 < heads) w += ex2(s.y - p.lse2[row * kHeadsPerRow + h + 1]);
+    }
+  }
+  // a sequence with a page outside the pool has NaN for all its sums and keeps its scores
+  if (!isnan(p.lse2[(int64_t)bk * p.chunks * kHeadsPerRow])) p.c.scores[(int64_t)bk * p.c.cap + i] += w;
+}
+
+template <typename K>
+int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t s, const char *what) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) return set_error(kECuda, "%s: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+// Workspace layout; every part starts on 256 bytes.
+struct Layout {
+  size_t warp_rec, cta_rec, cta_row, lse2, raw, bytes;
+};
+Layout layout_of(const KvView &c, int heads, int max_len, bool accumulate, int grid) {
+  const int group = heads / c.kv_heads, chunks = (group + kHeadsPerRow - 1) / kHeadsPerRow;
+  const int64_t rows = (int64_t)c.batch * c.kv_heads * chunks;
+  const size_t rec = (size_t)kHeadsPerRow * c.dim;
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  Layout l;
+  l.warp_rec = 0;
+  l.cta_rec = up((size_t)grid * kMaxWarps * rec * 4);
+  l.cta_row = l.cta_rec + up((size_t)grid * 2 * (rec + 16) * 4);
+  l.lse2 = l.cta_row + up((size_t)grid * sizeof(int4));
+  l.raw = l.lse2 + (accumulate ? up(rows * kHeadsPerRow * 4) : 0);
+  l.bytes = l.raw + (accumulate ? up((size_t)rows * max_len * raw_heads(group) * 4) : 0);
+  return l;
 }
 
 int attend_check(const bp_kv_cache *cache, int layer, int heads, int max_length, int accumulate, const char *what,
@@ -145,6 +108,9 @@ int attend_check(const bp_kv_cache *cache, int layer, int heads, int max_length,
   if (max_length < 0) return set_error(kEInval, "%s: negative max_length", what);
   if (accumulate && !cache->scores) return set_error(kEInval, "%s: the cache keeps no scores", what);
   *max_len = max_length && max_length < c->cap ? max_length : c->cap;
+  const int64_t rows = (int64_t)cache->batch * cache->kv_heads * ((heads / cache->kv_heads + 7) / 8);
+  if (rows * ((*max_len + 15) / 16) > 0x7FFFFFFF || (accumulate && cache->batch * (int64_t)cache->kv_heads > 65535))
+    return set_error(kERange, "%s: more work than the call can number", what);
   return kOk;
 }
 
@@ -156,11 +122,11 @@ using namespace bp;
 extern "C" size_t bp_paged_attention_workspace_size(const bp_kv_cache *cache, int heads, int max_length,
                                                     int accumulate) {
   KvView c;
-  int max_len;
+  int max_len = 0;
   clear_error();
   if (attend_check(cache, 0, heads, max_length, accumulate, "bp_paged_attention_workspace_size", &c, &max_len) != kOk)
     return 0;
-  return workspace_bytes_of(c, heads, max_len, accumulate != 0);
+  return layout_of(c, heads, max_len, accumulate != 0, sm_count()).bytes;
 }
 
 extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype, int heads, const void *q,
@@ -180,25 +146,40 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   if (!aligned16(q) || !aligned16(out) || q_stride % per)
     return set_error(kEAlign, "%s: pointers and strides must be multiples of 16 bytes", what);
   if (workspace && ((uintptr_t)workspace & 255u)) return set_error(kEAlign, "%s: workspace not 256-byte aligned", what);
-  const size_t need = workspace_bytes_of(p.c, heads, p.max_len, accumulate != 0);
-  if (workspace && workspace_bytes < need)
-    return set_error(kEWorkspace, "%s: workspace %zu bytes < %zu needed", what, workspace_bytes, need);
   rc = check_device();
+  const int grid = sm_count();
+  const Layout l = layout_of(p.c, heads, p.max_len, accumulate != 0, grid);
+  if (workspace && workspace_bytes < l.bytes)
+    return set_error(kEWorkspace, "%s: workspace %zu bytes < %zu needed", what, workspace_bytes, l.bytes);
+  if (rc != kOk) return rc;
+  rc = tc_error_word(&p.error);
   if (rc != kOk) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   void *ws = workspace;
-  if (!ws && need) {
-    cudaError_t e = cudaMallocAsync(&ws, need, s);
+  if (!ws) {
+    cudaError_t e = cudaMallocAsync(&ws, l.bytes, s);
     if (e != cudaSuccess) return set_error(kECuda, "%s: workspace allocation: %s", what, cudaGetErrorString(e));
   }
+  uint8_t *base = (uint8_t *)ws;
   p.heads = heads; p.group = heads / cache->kv_heads;
+  p.chunks = (p.group + kHeadsPerRow - 1) / kHeadsPerRow;
   p.q = q; p.qs = q_stride; p.out = out; p.lse = lse;
   p.scale = scale * 1.4426950408889634f;
-  p.raw = accumulate ? (float *)ws : nullptr;
-  if (dtype == BP_F32) rc = launch_attend_dim<float>(p, s);
-  else if (dtype == BP_BF16) rc = launch_attend_dim<__nv_bfloat16>(p, s);
-  else rc = launch_attend_dim<__half>(p, s);
-  if (!workspace && ws) {
+  p.warp_rec = (float *)(base + l.warp_rec);
+  p.cta_rec = (float *)(base + l.cta_rec);
+  p.cta_row = (int4 *)(base + l.cta_row);
+  p.lse2 = accumulate ? (float *)(base + l.lse2) : nullptr;
+  p.raw = accumulate ? (float *)(base + l.raw) : nullptr;
+  p.gp = raw_heads(p.group);
+  rc = p.c.fmt == 8 ? launch_kv_attend8(p, dtype, grid, s) : launch_kv_attend16(p, dtype, grid, s);
+  if (rc == kOk) {
+    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid), p, s, "k_kv_join");
+    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid), p, s, "k_kv_join");
+    else rc = launch_after(k_kv_join<__half>, dim3(grid), p, s, "k_kv_join");
+  }
+  if (rc == kOk && accumulate && p.max_len)
+    rc = launch_after(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), p, s, "k_kv_scores");
+  if (!workspace) {
     cudaError_t f = cudaFreeAsync(ws, s);
     if (rc == kOk && f != cudaSuccess) rc = set_error(kECuda, "%s: workspace free: %s", what, cudaGetErrorString(f));
   }
