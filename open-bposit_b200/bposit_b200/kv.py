@@ -88,8 +88,8 @@ class PagedKVCache:
         if not isinstance(table, torch.Tensor) or table.dim() != 2:
             raise ValueError("page_table must be a [batch, max_pages] int32 tensor")
         batch, per = table.shape
-        if batch > 4096:
-            raise ValueError(f"batch of at most 4096 sequences, got {batch}")
+        if batch > 2048:
+            raise ValueError(f"batch of at most 2048 sequences, got {batch}")
         row = tuple(k.shape[:-1])
         track = (layers, batch, heads, per * page)
         lens = (2, batch) if lengths.dim() == 2 else (batch,)

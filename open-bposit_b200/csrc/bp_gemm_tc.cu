@@ -2712,13 +2712,6 @@ int launch_gemm_tc(const GemmArgs &a, int4 *sta, int4 *stb, void *ws, size_t ws_
   return check_launch("tc_fixup");
 }
 
-// Device address of the kernel error word on the current device, for kernels
-// of other files that wait on barriers.
-int tc_error_word(int **out) {
-  const cudaError_t e = cudaGetSymbolAddress((void **)out, g_tc_error);
-  return e == cudaSuccess ? kOk : set_error(kECuda, "kernel error word: %s", cudaGetErrorString(e));
-}
-
 int tc_device_error(int *out) {
   int v = 0, zero = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_tc_error, sizeof v);

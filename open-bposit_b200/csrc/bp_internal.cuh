@@ -28,8 +28,6 @@ int sm_count();   // SMs of the current device
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
 
-int tc_error_word(int **out);   // device address of the kernel error word (bp_gemm_tc.cu)
-
 // ---- codec launchers (bp_codec.cu) ----
 int launch_decode(int fmt, const void *codes, size_t n, float *out, cudaStream_t s);
 int launch_quantize_bp8(const float *x, size_t n, bool nearest, uint8_t *codes, float *values,

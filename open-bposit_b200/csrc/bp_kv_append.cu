@@ -15,10 +15,12 @@ int kv_check(const bp_kv_cache *c, int layer, const char *what, KvView *view) {
     return set_error(kEInval, "%s: bad cache sizes", what);
   if (layer < 0 || layer >= c->layers)
     return set_error(kEInval, "%s: layer %d outside [0, %d)", what, layer, c->layers);
-  if (c->batch > 4096) return set_error(kERange, "%s: batch of at most 4096 sequences (got %d)", what, c->batch);
+  if (c->batch > 2048) return set_error(kERange, "%s: batch of at most 2048 sequences (got %d)", what, c->batch);
   if (c->kv_heads > 1024) return set_error(kERange, "%s: at most 1024 kv heads (got %d)", what, c->kv_heads);
   if ((int64_t)c->max_pages * c->page_size > (1 << 30))
     return set_error(kERange, "%s: capacity of at most 2^30 entries", what);
+  if ((int64_t)c->pages * c->kv_heads >= 0xFFFFFFF0LL / c->page_size)
+    return set_error(kERange, "%s: 2^32 or more rows in a layer of the pools", what);
   if (c->pages && (!c->k || !c->v)) return set_error(kEInval, "%s: null pool", what);
   if ((c->batch && !c->lengths) || (c->batch && c->max_pages && !c->page_table))
     return set_error(kEInval, "%s: null page table or lengths", what);

@@ -9,36 +9,48 @@
 namespace bp {
 namespace {
 
+constexpr int kJoinThreads = kHeadsPerRow * 32;
+constexpr int kJoinParts = 256;     // CTAs of one launch, at most
+
 // Joins the parts of a row that several CTAs of k_kv_attend worked on: block c
-// takes the row that starts in CTA c's range and goes on behind it.  Launched
+// takes the row that starts in CTA c's range and goes on behind it, a warp for
+// each head, blockIdx.y for each 32 columns of the output.  Launched
 // early (programmatic dependent launch), so its latency hides behind the main
 // kernel; the parts of a row are few and in L2.
 template <typename T>
-__global__ void __launch_bounds__(256) k_kv_join(AttendParams p) {
+__global__ void __launch_bounds__(kJoinThreads) k_kv_join(AttendParams p) {
+  __shared__ float weight[kHeadsPerRow][kJoinParts];   // 2^(m - M) of each part
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 open = p.cta_row[blockIdx.x];
+  const int2 open = p.cta_row[blockIdx.x];
   if (open.x < 0) return;
-  const int D = p.c.dim, rec = kHeadsPerRow * D;
+  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the first part is the CTA's second record (a row that starts there), the others are first records
-  const float *first = p.cta_rec + ((int64_t)blockIdx.x * 2 + 1) * (rec + 16);
+  const float *base = p.cta_rec + (int64_t)blockIdx.x * 2 * (rec + 16);
   const int64_t step = 2 * (rec + 16);
-  for (int e = threadIdx.x; e < rec; e += 256) {
-    const int h = e / D;
-    float M = -INFINITY, L = 0.0f, O = 0.0f;
-    for (int k = 0; k < open.y; ++k) {
-      const float *r = first + k * step - (k ? rec + 16 : 0);
-      M = fmaxf(M, r[rec + h]);
-    }
-    for (int k = 0; k < open.y; ++k) {
-      const float *r = first + k * step - (k ? rec + 16 : 0);
-      const float a = ex2(r[rec + h] - M);
-      L = fmaf(r[rec + 8 + h], a, L);
-      O = fmaf(r[e], a, O);
-    }
-    write_out<T>(p, open.x, h, e - h * D, D, O / L);
-    if (e % D == 0) write_lse(p, open.x, h, M + log2f(L));
+  const float *first = base + rec + 16;
+  auto part = [&](int k) { return k ? base + k * step : first; };
+  // one warp per head: the maximum and the sum over the parts
+  float M = -INFINITY, L = 0.0f;
+  for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[rec + warp]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+  for (int k = lane; k < parts; k += 32) {
+    const float a = ex2(part(k)[rec + warp] - M);
+    L = fmaf(part(k)[rec + 8 + warp], a, L);
+    weight[warp][k] = a;
   }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
+  __syncwarp();
+  const int64_t head = head_of(p, row_id(p, open.x), warp);
+  if (lane == 0 && blockIdx.y == 0) write_lse(p, open.x, warp, head, M + log2f(L));
+  if (head < 0) return;
+  const int d = blockIdx.y * 32 + lane;
+  float O = 0.0f;
+#pragma unroll 8
+  for (int k = 0; k < parts; ++k) O = fmaf(part(k)[warp * D + d], weight[warp][k], O);
+  ((T *)p.out)[head * D + d] = from_f32<T>(O / L);
 }
 
 // scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2):
@@ -80,6 +92,12 @@ int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t s, con
   return check_launch(what);
 }
 
+// CTAs of the main kernel: one per SM.
+int attend_grid() {
+  const int n = sm_count();
+  return n < kJoinParts ? n : kJoinParts;
+}
+
 // Workspace layout; every part starts on 256 bytes.
 struct Layout {
   size_t warp_rec, cta_rec, cta_row, lse2, raw, bytes;
@@ -93,7 +111,7 @@ Layout layout_of(const KvView &c, int heads, int max_len, bool accumulate, int g
   l.warp_rec = 0;
   l.cta_rec = up((size_t)grid * kMaxWarps * rec * 4);
   l.cta_row = l.cta_rec + up((size_t)grid * 2 * (rec + 16) * 4);
-  l.lse2 = l.cta_row + up((size_t)grid * sizeof(int4));
+  l.lse2 = l.cta_row + up((size_t)grid * sizeof(int2));
   l.raw = l.lse2 + (accumulate ? up(rows * kHeadsPerRow * 4) : 0);
   l.bytes = l.raw + (accumulate ? up((size_t)rows * max_len * raw_heads(group) * 4) : 0);
   return l;
@@ -126,7 +144,7 @@ extern "C" size_t bp_paged_attention_workspace_size(const bp_kv_cache *cache, in
   clear_error();
   if (attend_check(cache, 0, heads, max_length, accumulate, "bp_paged_attention_workspace_size", &c, &max_len) != kOk)
     return 0;
-  return layout_of(c, heads, max_len, accumulate != 0, sm_count()).bytes;
+  return layout_of(c, heads, max_len, accumulate != 0, attend_grid()).bytes;
 }
 
 extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype, int heads, const void *q,
@@ -147,12 +165,10 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
     return set_error(kEAlign, "%s: pointers and strides must be multiples of 16 bytes", what);
   if (workspace && ((uintptr_t)workspace & 255u)) return set_error(kEAlign, "%s: workspace not 256-byte aligned", what);
   rc = check_device();
-  const int grid = sm_count();
+  const int grid = attend_grid();
   const Layout l = layout_of(p.c, heads, p.max_len, accumulate != 0, grid);
   if (workspace && workspace_bytes < l.bytes)
     return set_error(kEWorkspace, "%s: workspace %zu bytes < %zu needed", what, workspace_bytes, l.bytes);
-  if (rc != kOk) return rc;
-  rc = tc_error_word(&p.error);
   if (rc != kOk) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   void *ws = workspace;
@@ -167,15 +183,15 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   p.scale = scale * 1.4426950408889634f;
   p.warp_rec = (float *)(base + l.warp_rec);
   p.cta_rec = (float *)(base + l.cta_rec);
-  p.cta_row = (int4 *)(base + l.cta_row);
+  p.cta_row = (int2 *)(base + l.cta_row);
   p.lse2 = accumulate ? (float *)(base + l.lse2) : nullptr;
   p.raw = accumulate ? (float *)(base + l.raw) : nullptr;
   p.gp = raw_heads(p.group);
   rc = p.c.fmt == 8 ? launch_kv_attend8(p, dtype, grid, s) : launch_kv_attend16(p, dtype, grid, s);
   if (rc == kOk) {
-    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid), p, s, "k_kv_join");
-    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid), p, s, "k_kv_join");
-    else rc = launch_after(k_kv_join<__half>, dim3(grid), p, s, "k_kv_join");
+    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid, p.c.dim / 32), p, s, "k_kv_join");
+    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid, p.c.dim / 32), p, s, "k_kv_join");
+    else rc = launch_after(k_kv_join<__half>, dim3(grid, p.c.dim / 32), p, s, "k_kv_join");
   }
   if (rc == kOk && accumulate && p.max_len)
     rc = launch_after(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), p, s, "k_kv_scores");

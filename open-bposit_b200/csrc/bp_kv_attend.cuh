@@ -11,31 +11,34 @@
 // in bp8) and every code has to be decoded, which at the memory's rate is about
 // 23 codes per clock and SM -- so decoding, not arithmetic on the decoded
 // values, is what the layout is built around:
-//  * Both products run on the tensor cores (mma.sync; tcgen05 would need the
-//    decoded operands written back to shared memory, 2 to 4 bytes per code,
-//    for an N of 8) with the cache as the wide operand: S^T = K q^T and
-//    O^T = V^T P^T.  The K dimension of an MMA and the order of its rows are
-//    free, so each thread's fragment is a contiguous piece of the rows in
-//    shared memory and is decoded in registers, without a transpose.
-//  * bp8 codes have at most 4 significant bits and a binade in [-24, 24]: exact
-//    in bf16.  A 256-entry table holds, per code and lane, the bf16 value in the
-//    low and in the high half of a word (64 KB: bank = lane, so no conflicts,
-//    and one byte permute makes the address).  bp16 codes have at most 11
-//    significant bits: exact in tf32; their fp32 bits are piecewise linear in
-//    the code (see decode16).
-//  * q and the softmax weights are fp32 and are split exactly into bf16 terms
-//    (8 bits each), or nearly so into two tf32 terms, so every product keeps
-//    fp32 accuracy; each tile's MMA sum is added to the running output by an
-//    fp32 fma (the tensor cores truncate their sums, which would drift over
-//    thousands of tiles).
+//  * Both products run on the tensor cores (mma.sync m16n8k8, tf32; tcgen05
+//    would need the decoded operands written back to shared memory, 4 bytes
+//    per code, for 8 rows of queries).  The cache is the B operand, whose K
+//    order and column order are free, so each thread's fragments are contiguous
+//    pieces of the rows in shared memory, decoded in registers without a
+//    transpose; and S^T's accumulators are P's A fragment as they are.
+//  * Codes are exact in tf32: bp8 values have at most 4 significant bits, bp16
+//    values at most 11.  bp8 goes through a table of fp32 values with a copy of
+//    every entry for each lane (64 KB: bank = lane, so no conflicts, and one byte
+//    permute makes the address); bp16 codes are decoded arithmetically
+//    (decode16).
+//  * The rows of the A operand are 8 query heads twice: the upper 11 bits of q
+//    (or of the softmax weight), and what is left of it, 11 bits more.  The two
+//    sums are added in fp32, so products keep fp32 accuracy.  Each tile's sum
+//    is added to the running output by an fp32 fma: the tensor cores truncate
+//    their sums, which would drift over thousands of tiles.
 //
-// Work split: rows are cut into tiles of TT entries; the tiles of all rows, in
+// Work split: rows are cut into units of 16 entries; the units of all rows, in
 // order, are dealt to the CTAs (one per SM) in equal contiguous ranges and
-// within a CTA to its warps, whatever the lengths are.  A warp fetches its
-// tiles by bulk copies (one per page and operand) into its own stage and needs
-// no other warp until its range ends.  A row that lies within one warp's range
-// is finished by that warp; parts of a row are joined first over the CTA's warps
-// in shared memory, then over CTAs by k_kv_join.
+// within a CTA to its warps, whatever the lengths are.  A warp takes its units
+// four at a time (a tile; single ones at the end of a row or of its range),
+// fetches tiles into its own stage (cp.async, 16 bytes a lane: a page table look-up per
+// page and no address work per row) and needs no other warp until its range
+// ends; the next tile's keys are fetched while this one's values are used, and
+// the other way round.  Rows lie in the stage with their 16-byte pieces permuted
+// (Swizzle) so that no fragment load has bank conflicts.  A row that lies within
+// one warp's range is finished by that warp; parts of a row are joined first
+// over the CTA's warps in shared memory, then over CTAs by k_kv_join.
 #pragma once
 #include <math.h>
 
@@ -43,8 +46,6 @@
 
 namespace bp {
 
-constexpr long long kKvWaitLimit = 4000000000LL;   // cycles (~2 s) before a wait gives up
-constexpr long long kKvDrainLimit = 200000000LL;   // cycles (~0.1 s) for copies in flight after that
 constexpr int kHeadsPerRow = 8;                     // query heads of one work row (N of the MMAs)
 
 struct AttendParams {
@@ -59,14 +60,15 @@ struct AttendParams {
   // workspace
   float *warp_rec;           // [CTA][warp][8 D]: parts that ended inside a warp's range
   float *cta_rec;            // [CTA][2][8 D + 16]: o, m, l of rows that cross CTAs
-  int4 *cta_row;             // [CTA]: {row that starts here and goes on or -1, CTAs that share it, -, -}
+  int2 *cta_row;             // [CTA]: {row that starts here and goes on behind it, or -1; CTAs that share it}
   float *lse2;               // [rows][8], base 2; null unless scores are accumulated
   float *raw;                // [rows][max_len][gp] scores, base 2; null unless accumulated
   int gp;                    // heads kept per entry in raw (even)
-  int *error;
 };
 
 constexpr int kMaxWarps = 16;
+constexpr int kTableAt = 65536;                     // shared address of the bp8 decode table
+constexpr int kSharedReserved = 1024;               // shared address where a block's own memory starts
 
 // Query heads kept per entry and work row in `raw`, even so that pairs are one access.
 inline int raw_heads(int group) { return group >= kHeadsPerRow ? kHeadsPerRow : (group + 1) & ~1; }
@@ -77,17 +79,32 @@ struct AttendCfg {
   static constexpr int BYTES = FMT / 8;
   static constexpr int ROWB = D * BYTES;
   static constexpr int TT = FMT == 8 ? (D <= 64 ? 64 : 32) : (D <= 32 ? 64 : 32);   // entries per tile
-  static constexpr int NW = FMT == 8 ? (D <= 64 ? 16 : 8) : (D <= 64 ? 12 : 8);
+#ifndef KV_NW
+#define KV_NW 12
+#endif
+  static constexpr int NW = D <= 64 ? KV_NW : 8;
   static constexpr int TILEB = TT * ROWB;
-  static constexpr int STAGE = 2 * TILEB + (FMT == 8 ? 2 * TT : 0);
-  static constexpr int LUT = FMT == 8 ? 65536 : 0;
+  // 2^exponent of a tile's keys and values as fp32, [t][n][2] in the order that thread t of a quad needs them, with
+  // a row stride that keeps the four rows in different banks
+  static constexpr int POWROW = TT / 4 + 4;
+  static constexpr int POWB = FMT == 8 ? 2 * 4 * POWROW * 4 : 0;
+  static constexpr int STAGE = 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;
   static constexpr int REC = kHeadsPerRow * D;                   // floats of one part's output
-  // table, stages, part statistics [NW][2][16], part rows [NW][2], barriers [NW][2], scan [NW + 1], tiles before
-  // each sequence [batch + 1]
-  static constexpr int META = LUT + NW * STAGE;
-  static constexpr int FIXED = META + NW * 2 * 64 + NW * 2 * 4 + NW * 2 * 8 + (NW + 2) * 4;
+  // Shared memory (bp8): the decode table at shared addresses 64 K .. 128 K, so that an entry's address is the
+  // bytes {lane, code, 1, 0}; FRONT stages below it, the others above.  (bp16: no table, all stages in front.)
+  static constexpr int FRONT = FMT == 8 ? (kTableAt - kSharedReserved) / STAGE : NW;
+  static constexpr int BACK = NW - (FRONT < NW ? FRONT : NW);
+  // offset of what follows the table, from shared address kSharedReserved
+  static constexpr int AFTER = FMT == 8 ? 2 * kTableAt - kSharedReserved : 0;
+  // part statistics [NW][2][16], part rows [NW][2], scan [NW + 2], tiles before each sequence [batch + 1]
+  static constexpr int META = AFTER + (FMT == 8 ? BACK : NW) * STAGE;
+  static constexpr int FIXED = META + NW * 2 * 64 + NW * 2 * 4 + (NW + 2) * 4;
   static size_t smem(int batch) { return FIXED + (size_t)(batch + 1) * 4; }
+  static __device__ __forceinline__ int stage_at(int warp) {
+    return warp < FRONT ? warp * STAGE : AFTER + (warp - FRONT) * STAGE;
+  }
   static_assert(REC * 4 <= STAGE, "a part's output fits the stage");
+  static_assert(TT % 32 == 0, "a lane converts TT / 32 exponents");
   static_assert(STAGE % 16 == 0, "stages stay 16-byte aligned");
 };
 
@@ -95,57 +112,75 @@ namespace {
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-__device__ __forceinline__ void bar_init(uint64_t *bar) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(bar)));
+// 16 bytes from global to shared memory, asynchronously; groups complete in order.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait of a whole warp; false (and the error word set) if it gave up.
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, int *error) {
-  if (__all_sync(~0u, bar_try(bar, parity))) return true;
-  const long long t0 = clock64();
-  while (true) {
-    if (__all_sync(~0u, bar_try(bar, parity))) return true;
-    if (__any_sync(~0u, clock64() - t0 > kKvWaitLimit)) {
-      if ((threadIdx.x & 31) == 0) atomicOr(error, 64);
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(dst)),
-      "l"(src), "r"(bytes), "r"(smem_addr(bar))
-      : "memory");
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All groups but the last one are complete, for the whole warp.
+__device__ __forceinline__ void copy_wait_but_one() {
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  __syncwarp();
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// Offset of 16-byte piece c of row r of a tile.  A fragment load takes the same
+// pieces of several rows at once: keys pieces of rows {0, 5}, {1, 4}, {2, 7} or
+// {3, 6} (two rows a quarter warp), values of rows 0-3 or 4-7 (four rows).  The
+// permutation puts those into different banks; rows of 96 and 192 bytes differ
+// enough by themselves.
+template <int ROWB>
+__device__ __forceinline__ int swizzle(int r, int c) {
+  int s = 0, lane = c;
+  if (ROWB == 32) {            // 4 rows in 128 bytes
+    lane = (r & 3) * 2 + c;
+    s = (r >> 2 & 1) * 4;
+    return (r >> 2) * 128 + (lane ^ s) * 16;
+  }
+  if (ROWB == 64) {            // 2 rows
+    lane = (r & 1) * 4 + c;
+    s = (r >> 1 & 1) * 2;
+    return (r >> 1) * 128 + (lane ^ s) * 16;
+  }
+  if (ROWB == 128) s = (r & 3) * 2 ^ (r & 1);
+  if (ROWB == 256) s = ((r & 1) | (r >> 1 & 1) * 4) ^ (c >> 3) * 2;
+  return r * ROWB + (c ^ s) * 16;
+}
+// N words at word `at` of row r; they lie within 16-byte pieces.
+template <int ROWB, int N>
+__device__ __forceinline__ void load_words(const uint8_t *tile, int r, int at, uint32_t (&x)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      *reinterpret_cast<uint4 *>(x + 4 * i) =
+          *reinterpret_cast<const uint4 *>(tile + swizzle<ROWB>(r, at / 4 + i));
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      *reinterpret_cast<uint2 *>(x + 2 * i) = *reinterpret_cast<const uint2 *>(
+          tile + swizzle<ROWB>(r, (at + 2 * i) / 4) + (at + 2 * i) % 4 * 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      x[i] = *reinterpret_cast<const uint32_t *>(tile + swizzle<ROWB>(r, (at + i) / 4) + (at + i) % 4 * 4);
+  }
+}
+
+// c += a b, and the same from a zero accumulator.
+__device__ __forceinline__ void mma_tf32_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+// Entry of the decode table by shared address.
+__device__ __forceinline__ uint32_t table_entry(uint32_t at) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("ld.shared.b32 %0, [%1];" : "=r"(y) : "r"(at));
   return y;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -159,45 +194,8 @@ __device__ __forceinline__ uint32_t to_tf32(float x) {
   return y;
 }
 
-// Terms that q and the weights are split into: fp32 exactly into three bf16
-// terms, or into two tf32 terms (relative error 2^-22); bf16 and fp16 queries
-// need one and two (one in tf32).  Weights for a 16-bit output take two terms
-// (2^-16 of each weight, far below the output's half step).
-template <int FMT, typename T>
-struct Terms {
-  static constexpr bool F32 = sizeof(T) == 4;
-  static constexpr bool BF16 = !F32 && __is_same(T, __nv_bfloat16);
-  static constexpr int Q = FMT == 8 ? (F32 ? 3 : (BF16 ? 1 : 2)) : (F32 ? 2 : 1);
-  static constexpr int P = FMT == 8 ? (F32 ? 3 : 2) : 2;
-};
-
-__device__ __forceinline__ uint32_t top_bits(uint32_t x) { return x & 0xFFFF0000u; }
-// (a's high half) | (b's high half) << 16
-__device__ __forceinline__ uint32_t pack_high(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
-
-// x and y as N packed pairs of bf16 terms, largest first: each term is the
-// rest's top 8 bits (truncated, so nothing overflows), the last of two or more
-// takes what is left (exact for three terms, rounded for fewer).
-template <int N>
-__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&out)[N]) {
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    if (n == N - 1 && N == 2) {
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(out[n]) : "f"(y), "f"(x));
-    } else {
-      out[n] = pack_high(__float_as_uint(x), __float_as_uint(y));
-      if (n < N - 1) {
-        x -= __uint_as_float(top_bits(__float_as_uint(x)));
-        y -= __uint_as_float(top_bits(__float_as_uint(y)));
-      }
-    }
-  }
-}
-template <int N>
-__device__ __forceinline__ void split_tf32(float x, uint32_t (&out)[N]) {
-  out[0] = __float_as_uint(x) & 0xFFFFE000u;
-  if (N == 2) out[N - 1] = to_tf32(x - __uint_as_float(out[0]));
-}
+// The upper 11 bits of x, and the rest of it as tf32.
+__device__ __forceinline__ uint32_t tf32_high(float x) { return __float_as_uint(x) & 0xFFFFE000u; }
 
 // fp32 bits of a bp16 code's value; `u` is 2^23 + 2^15 + the signed code as a
 // float.  Below 1 the value's exponent and fraction, read as one fixed-point
@@ -215,43 +213,52 @@ __device__ __forceinline__ uint32_t decode16(float u) {
   return v | (__float_as_uint(x) & 0x80000000u);
 }
 
-template <typename T>
-__device__ __forceinline__ void write_out(const AttendParams &p, int64_t row, int h, int d, int D, float x) {
-  const int ch = (int)(row % p.chunks);
-  const int64_t bk = row / p.chunks;
-  const int hk = (int)(bk % p.c.kv_heads), b = (int)(bk / p.c.kv_heads);
-  const int g = ch * kHeadsPerRow + h;
-  if (g < p.group) ((T *)p.out)[((int64_t)b * p.heads + hk * p.group + g) * D + d] = from_f32<T>(x);
+// A work row: 8 (or fewer) query heads of one kv head of one sequence.
+struct RowId {
+  int b, hk, ch;
+};
+__device__ __forceinline__ RowId row_id(const AttendParams &p, int row) {
+  const int bk = row / p.chunks, b = bk / p.c.kv_heads;
+  return {b, bk - b * p.c.kv_heads, row - bk * p.chunks};
 }
-__device__ __forceinline__ void write_lse(const AttendParams &p, int64_t row, int h, float lse2) {
-  if (p.lse2) p.lse2[row * kHeadsPerRow + h] = lse2;
-  if (!p.lse) return;
-  const int ch = (int)(row % p.chunks);
-  const int64_t bk = row / p.chunks;
-  const int g = ch * kHeadsPerRow + h;
-  if (g < p.group)
-    p.lse[bk / p.c.kv_heads * p.heads + bk % p.c.kv_heads * p.group + g] = lse2 * 0.6931471805599453f;
+// Query head h of the row as an index into [batch, heads]; -1 for a head that pads the row.
+__device__ __forceinline__ int64_t head_of(const AttendParams &p, const RowId &r, int h) {
+  const int g = r.ch * kHeadsPerRow + h;
+  return g < p.group ? (int64_t)r.b * p.heads + r.hk * p.group + g : -1;
+}
+__device__ __forceinline__ void write_lse(const AttendParams &p, int row, int h, int64_t head, float lse2) {
+  if (p.lse2) p.lse2[(int64_t)row * kHeadsPerRow + h] = lse2;
+  if (p.lse && head >= 0) p.lse[head] = lse2 * 0.6931471805599453f;
 }
 
-// CTAs that take part: at least kMinTiles tiles each, so that short batches are
+// The units 0 .. total - 1 over `parts`: the first total % parts of them have one more.
+struct Deal {
+  int each, more;
+  __device__ __forceinline__ Deal(int total, int parts) : each(total / parts), more(total - each * parts) {}
+  __device__ __forceinline__ int begin(int part) const { return part * each + min(part, more); }
+  __device__ __forceinline__ int part_of(int unit) const {
+    const int front = more * (each + 1);
+    return unit < front ? unit / (each + 1) : more + (unit - front) / each;
+  }
+};
+// CTAs that take part: at least kMinUnits units each, so that short batches are
 // not cut into parts that cost more to join than to read.
-constexpr int kMinTiles = 8;
-__device__ __forceinline__ int active_ctas(int tiles, int grid) {
-  const int n = (tiles + kMinTiles - 1) / kMinTiles;
-  return n < grid ? n : grid;
-}
+constexpr int kMinUnits = 32;
+__device__ __forceinline__ int active_ctas(int units, int grid) { return min((units + kMinUnits - 1) / kMinUnits, grid); }
 
 template <int FMT, int D, typename T>
 __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(AttendParams p) {
   using C = AttendCfg<FMT, D>;
-  using N = Terms<FMT, T>;
-  constexpr int TT = C::TT, NW = C::NW, MT = TT / 16, MD = D / 16, NT = NW * 32;
-  constexpr int QS = FMT == 8 ? D / 16 : D / 8;          // MMA steps along D
+  constexpr int TT = C::TT, NW = C::NW, NT = NW * 32;
+  constexpr int TU = TT / 16;           // units per tile
+  constexpr int DN = D / 8;             // 8-wide columns of O, and MMA steps along D
+  constexpr int KW = C::ROWB / 16;      // words of a key row that one thread holds
+  constexpr int VW = C::ROWB / 32;      // words of a value row that one thread holds
+  constexpr bool F32 = sizeof(T) == 4;
   extern __shared__ __align__(128) uint8_t smem[];
   float *const rec_ml = reinterpret_cast<float *>(smem + C::META);          // [NW][2][m 8, l 8]
   int *const rec_row = reinterpret_cast<int *>(rec_ml + NW * 32);           // [NW][2]
-  uint64_t *const bars = reinterpret_cast<uint64_t *>(rec_row + NW * 2);    // [NW][K, V]
-  int *const scan = reinterpret_cast<int *>(bars + NW * 2);
+  int *const scan = rec_row + NW * 2;
   int *const before = scan + NW + 2;                                        // [batch + 1]
   const KvView &c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -259,13 +266,13 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
   asm volatile("griddepcontrol.launch_dependents;");
 
   auto length = [&](int b) { return min(c.length(b), p.max_len); };
-  // tiles before each sequence
+  // units before each sequence
   {
     const int each = (c.batch + NT - 1) / NT;
     int mine = 0;
     for (int i = 0; i < each; ++i) {
       const int b = tid * each + i;
-      if (b < c.batch) mine += (length(b) + TT - 1) / TT * per_seq;
+      if (b < c.batch) mine += (length(b) + 15) / 16 * per_seq;
     }
     int incl = mine;
 #pragma unroll
@@ -274,11 +281,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
       if (lane >= d) incl += x;
     }
     if (lane == 31) scan[warp] = incl;
-    if (tid < NW * 2) {
-      rec_row[tid] = -1;
-      bar_init(&bars[tid]);
-    }
-    if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (tid < NW * 2) rec_row[tid] = -1;
     __syncthreads();
     int at = incl - mine;
     for (int w = 0; w < warp; ++w) at += scan[w];
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
       const int b = tid * each + i;
       if (b < c.batch) {
         before[b] = at;
-        at += (length(b) + TT - 1) / TT * per_seq;
+        at += (length(b) + 15) / 16 * per_seq;
       }
     }
     if (tid == NT - 1) before[c.batch] = at;
@@ -304,416 +307,404 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
   const int ctas = active_ctas(total, gridDim.x);
   const int cta = blockIdx.x;
   if (cta >= ctas) {
-    if (tid == 0) p.cta_row[cta] = make_int4(-1, 0, 0, 0);
+    if (tid == 0) p.cta_row[cta] = make_int2(-1, 0);
     return;
   }
-  const int lo = (int)((int64_t)total * cta / ctas), hi = (int)((int64_t)total * (cta + 1) / ctas);
-  const int wlo = lo + (int)((int64_t)(hi - lo) * warp / NW), whi = lo + (int)((int64_t)(hi - lo) * (warp + 1) / NW);
+  const Deal deal(total, ctas);
+  const int lo = deal.begin(cta), hi = deal.begin(cta + 1);
+  const Deal share(hi - lo, NW);
+  const int wlo = lo + share.begin(warp), whi = lo + share.begin(warp + 1);
 
-  uint8_t *const stage = smem + C::LUT + warp * C::STAGE;
+  uint8_t *const stage = smem + C::stage_at(warp);
   uint8_t *const sk = stage, *const sv = stage + C::TILEB;
   int8_t *const ske = reinterpret_cast<int8_t *>(stage + 2 * C::TILEB), *const sve = ske + TT;
-  uint64_t *const kbar = &bars[warp * 2], *const vbar = kbar + 1;
-
-  // ---- the tile that is fetched next: x = its number, and where it lies ----
-  int nx = wlo, nb = 0, nrow = 0, ntile = 0, nn = 0, npage = -1;
-  auto locate = [&]() {       // sequence of tile nx by bisection
-    int a = 0, z = c.batch;
-    while (z - a > 1) {
-      const int m = (a + z) >> 1;
-      if (before[m] <= nx) a = m;
-      else z = m;
+  float *const kpow = reinterpret_cast<float *>(stage + 2 * C::TILEB + 2 * TT), *const vpow = kpow + 4 * C::POWROW;
+  // ---- where tiles lie: units u .. u + count - 1 of a work row ----
+  struct Place {
+    int b, row, hk, ch, u, count, n;       // sequence, work row of it (hk * chunks + ch), units, entries of the row
+  };
+  auto units_of = [](int n) { return (n + 15) / 16; };
+  // the tile behind w, which must exist; `left`: units of this warp's range from there on
+  auto advance = [&](Place &w, int left) {
+    w.u += w.count;
+    if (w.u >= units_of(w.n)) {
+      w.u = 0;
+      ++w.row;
+      if (++w.ch == p.chunks) {
+        w.ch = 0;
+        ++w.hk;
+      }
+      if (w.row == per_seq) {
+        w.row = w.hk = 0;
+        do ++w.b;
+        while (before[w.b + 1] == before[w.b]);
+        w.n = length(w.b);
+      }
     }
-    nb = a;
-    nn = length(nb);
-    const int nt = (nn + TT - 1) / TT, r = nx - before[nb];
-    nrow = nt ? r / nt : 0;
-    ntile = nt ? r % nt : 0;
+    w.count = min(min(TU, units_of(w.n) - w.u), left);
   };
-  const int seg = min(TT, 1 << c.page_shift);            // entries per copy
-  auto pages = [&]() {        // this lane's page of the tile; its entries in it
-    const int i = ntile * TT + lane * seg;
-    npage = lane * seg < TT && i < nn ? c.page_of(nb, i) : -2;
+  // Pool row of the first entry of the tile's unit `lane` (its others follow): kLost when its page is outside the
+  // pool, kBehind when the tile has no such unit.
+  constexpr uint32_t kLost = ~0u, kBehind = ~0u - 1;
+  auto rows_of = [&](const Place &w) {
+    const int i = (w.u + lane) * 16;
+    if (lane >= w.count) return kBehind;
+    const int pg = c.page_of(w.b, i);
+    return pg < 0 ? kLost : (uint32_t)c.row(pg, w.hk, i);
   };
-  uint32_t fetched[2] = {0, 0};
-  auto fetch = [&](bool value) {
-    ++fetched[value];
-    const int i = ntile * TT + lane * seg;
-    const int cnt = npage == -2 ? 0 : min(seg, nn - i);
-    const bool ok = npage >= 0;
-    const uint32_t bytes = ok ? cnt * C::ROWB : 0, ebytes = FMT == 8 && ok ? (cnt + 15) & ~15 : 0;
-    const uint32_t all = __reduce_add_sync(~0u, bytes + ebytes);
-    uint64_t *bar = value ? vbar : kbar;
-    if (lane == 0) bar_expect(bar, all);
-    __syncwarp();
-    if (ok) {
-      const int64_t row = c.row(npage, nrow / p.chunks, i);
-      bulk_load((value ? sv : sk) + lane * seg * C::ROWB, (value ? c.v : c.k) + row * C::ROWB, bytes, bar);
-      if (FMT == 8) bulk_load((value ? sve : ske) + lane * seg, (value ? c.v_exp : c.k_exp) + row, ebytes, bar);
+  const uint32_t stage_s = smem_addr(stage);
+  constexpr int CPR = C::ROWB / 16;        // 16-byte pieces per row
+  constexpr int PJ = CPR / 2;              // pieces per lane of 16 rows
+  // piece `lane` of 16 rows; piece j * 32 + lane lies 512 j behind it, permuted alike (see below for 256-byte rows)
+  const uint32_t to = swizzle<C::ROWB>(lane / CPR, lane % CPR);
+  auto fetch = [&](const Place &w, uint32_t rows, bool value) {
+    const uint8_t *pool = (value ? c.v : c.k) + lane * 16;
+    const uint32_t dst = stage_s + (value ? C::TILEB : 0) + to;
+    const int valid = w.n - w.u * 16;
+#pragma unroll
+    for (int i = 0; i < TU; ++i) {
+      const uint32_t row = __shfl_sync(~0u, rows, i);
+      if (row >= kBehind) continue;        // (the same for all lanes)
+      const uint8_t *src = pool + (uint64_t)row * C::ROWB;
+#pragma unroll
+      for (int j = 0; j < PJ; ++j) {
+        const uint32_t d = dst + i * 16 * C::ROWB + j * 512;
+        if (i * 16 + (j * 32 + lane) / CPR < valid) copy16(CPR == 16 && (j & 1) ? d ^ 64 : d, src + j * 512);
+      }
     }
+    if (FMT == 8 && rows < kBehind)
+      copy16(stage_s + 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + rows);
+    copy_commit();
   };
 
+  Place cur{}, nxt{};
+  uint32_t rows_c = kBehind, rows_n = kBehind;
   if (wlo < whi) {
-    locate();
-    pages();
-    fetch(false);
-    fetch(true);
+    int a = 0, z = c.batch;                // sequence of the first unit, by bisection
+    while (z - a > 1) {
+      const int mid = (a + z) >> 1;
+      if (before[mid] <= wlo) a = mid;
+      else z = mid;
+    }
+    cur.b = a;
+    cur.n = length(a);
+    const int r = wlo - before[a], nu = units_of(cur.n);
+    cur.row = r / nu;
+    cur.u = r - cur.row * nu;
+    cur.hk = cur.row / p.chunks;
+    cur.ch = cur.row - cur.hk * p.chunks;
+    cur.count = min(min(TU, nu - cur.u), whi - wlo);
+    rows_c = rows_of(cur);
+    nxt = cur;
   }
   if (FMT == 8) {
-    // the decode table: word 64 code + lane (value in the low half) and + 32 (in the high half)
-    for (int i = tid; i < 512; i += NT) {
-      const int code = i & 255;
-      const uint32_t v = posit_to_f32_bits<8, 2>(code);
-      uint32_t *row = reinterpret_cast<uint32_t *>(smem) + code * 64;
-      const int half = (i >> 8) * 32;
-#pragma unroll 8
-      for (int j = 0; j < 32; ++j) row[half + ((j + i) & 31)] = half ? v : v >> 16;
+    // the decode table: word 64 code + lane
+    for (int i = tid; i < 256; i += NT) {
+      const uint32_t v = posit_to_f32_bits<8, 2>(i);
+      uint4 *row = reinterpret_cast<uint4 *>(smem + (kTableAt - kSharedReserved)) + i * 16;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) row[(j + i) & 7] = make_uint4(v, v, v, v);
     }
   }
+  fetch(cur, rows_c, false);
+  fetch(cur, rows_c, true);
   __syncthreads();
-  const uint32_t lane4 = lane * 4;
-  // bytes ka of a and kb of b as a pair of bf16 values
-  auto pair8 = [&](uint32_t a, int ka, uint32_t b, int kb) {
-    const uint32_t x = __byte_perm(a, lane4, 0x5504 | ka << 4), y = __byte_perm(b, lane4, 0x5504 | kb << 4);
-    return *reinterpret_cast<const uint32_t *>(smem + x) | *reinterpret_cast<const uint32_t *>(smem + 128 + y);
+  const uint32_t entry = lane * 4 | (kTableAt >> 16) << 8;
+  // fp32 bits of code k of a word
+  auto decode = [&](uint32_t w, int k) {
+    if (FMT == 8) return table_entry(__byte_perm(w, entry, 0x6504 | k << 4));
+    return decode16(__uint_as_float(__byte_perm(w ^ 0x80008000u, 0x4B00u, k ? 0x5432 : 0x5410)));
+  };
+  constexpr int CW = 4 / C::BYTES;      // codes per word
+
+  // The thread's place in the fragments: head g of A and of the accumulators; column g of S is entry `er` of its 8
+  // entries, and the accumulators' columns 2t and 2t + 1 (K of the second product: t and t + 4) are entries t and
+  // 4 + (t ^ 1) -- an order in which neighbouring quads read rows of different banks.
+  const int er = (g & 1) ? 4 + ((g >> 1) ^ 1) : g >> 1;
+  const int e0 = t, e1 = 4 + (t ^ 1);
+  uint32_t qf[DN][F32 ? 4 : 2];
+  float o[DN][2], m = -INFINITY, l = 0.0f;
+
+  bool lost = false;
+  int at_row = 0;                          // first unit of the current row that this warp has
+
+  // The three stages of a step over U units, from unit i0 of the stage on.
+  // S[head, entry] = q K^T
+  auto scores = [&](auto &s, int i0) {
+    constexpr int SN = sizeof(s) / sizeof(s[0]);
+#pragma unroll
+    for (int i = 0; i < SN; ++i) {
+      uint32_t kw[KW];
+      load_words<C::ROWB>(sk + (i0 * 16 + i * 8) * C::ROWB, er, t * KW, kw);
+      float c4[4];
+#pragma unroll
+      for (int w = 0; w < DN; ++w) {
+        const uint32_t b0 = decode(kw[2 * w / CW], 2 * w % CW), b1 = decode(kw[2 * w / CW], 2 * w % CW + 1);
+        const uint32_t a[4] = {qf[w][0], F32 ? qf[w][1] : 0u, qf[w][F32 ? 2 : 1], F32 ? qf[w][F32 ? 3 : 0] : 0u};
+        if (w == 0) mma_tf32_first(c4, a, b0, b1);
+        else mma_tf32(c4, a, b0, b1);
+      }
+      s[i][0] = F32 ? c4[0] + c4[2] : c4[0];
+      s[i][1] = F32 ? c4[1] + c4[3] : c4[1];
+    }
+  };
+  // S becomes e^(S - maximum), maximum and sum move on; returns the factor for what was summed before
+  auto weights = [&](auto &s, int i0, int valid) {
+    constexpr int SN = sizeof(s) / sizeof(s[0]);
+#pragma unroll
+    for (int i = 0; i < SN; i += 2) {
+      float4 f = make_float4(p.scale, p.scale, p.scale, p.scale);
+      if (FMT == 8) f = *reinterpret_cast<const float4 *>(kpow + t * C::POWROW + 4 * i0 + 2 * i);
+      s[i][0] *= f.x;
+      s[i][1] *= f.y;
+      s[i + 1][0] *= f.z;
+      s[i + 1][1] *= f.w;
+    }
+    if (SN == 2) {             // only a unit by itself can end behind the length
+#pragma unroll
+      for (int i = 0; i < SN; ++i) {
+        if (i * 8 + e0 >= valid) s[i][0] = -INFINITY;
+        if (i * 8 + e1 >= valid) s[i][1] = -INFINITY;
+      }
+    }
+    if (p.raw && g < p.gp) {
+      float *raw = p.raw + (((int64_t)cur.b * per_seq + cur.row) * p.max_len + (cur.u + i0) * 16) * p.gp + g;
+#pragma unroll
+      for (int i = 0; i < SN; ++i) {
+        if (SN > 2 || i * 8 + e0 < valid) raw[(i * 8 + e0) * p.gp] = s[i][0];
+        if (SN > 2 || i * 8 + e1 < valid) raw[(i * 8 + e1) * p.gp] = s[i][1];
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < SN; i += 2) mx = fmaxf(mx, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i + 1][0], s[i + 1][1])));
+    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+    mx = fmaxf(m, mx);
+    const float at = mx == -INFINITY ? 0.0f : mx;       // nothing but -inf so far: weigh it with 0
+    const float alpha = ex2(m - at);
+    m = mx;
+    float sum[4] = {l * alpha, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < SN; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s[i][j] = ex2(s[i][j] - at);
+        sum[(2 * i + j) & 3] += s[i][j];
+      }
+    l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    return alpha;
+  };
+  // O[head, d] = alpha O + P V
+  auto values = [&](const auto &s, int i0, float alpha) {
+    constexpr int SN = sizeof(s) / sizeof(s[0]);
+    float acc[DN][4];
+#pragma unroll
+    for (int i = 0; i < SN; ++i) {
+      float w0 = s[i][0], w1 = s[i][1];
+      if (FMT == 8) {      // (entries behind the length have weight 0 and any exponent: 0 times a finite power)
+        const float2 f = *reinterpret_cast<const float2 *>(vpow + t * C::POWROW + 4 * i0 + 2 * i);
+        w0 *= f.x;
+        w1 *= f.y;
+      }
+      const uint32_t a[4] = {tf32_high(w0), tf32_high(w0 - __uint_as_float(tf32_high(w0))), tf32_high(w1),
+                             tf32_high(w1 - __uint_as_float(tf32_high(w1)))};
+      uint32_t v0[VW], v1[VW];
+      const uint8_t *r = sv + (i0 * 16 + i * 8) * C::ROWB;
+      load_words<C::ROWB>(r, e0, g * VW, v0);
+      load_words<C::ROWB>(r, e1, g * VW, v1);
+#pragma unroll
+      for (int d = 0; d < DN; ++d) {
+        const uint32_t b0 = decode(v0[d / CW], d % CW), b1 = decode(v1[d / CW], d % CW);
+        if (i == 0) mma_tf32_first(acc[d], a, b0, b1);
+        else mma_tf32(acc[d], a, b0, b1);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DN; ++d) {
+      o[d][0] = fmaf(o[d][0], alpha, acc[d][0] + acc[d][2]);
+      o[d][1] = fmaf(o[d][1], alpha, acc[d][1] + acc[d][3]);
+    }
+  };
+  // each exponent of the tile is turned into a power of two once, and read back by the four threads that need it
+  auto powers = [&](const int8_t *exps, float *pow, float scale) {
+    if constexpr (FMT == 8) {
+#pragma unroll
+      for (int i = 0; i < TT / 32; ++i) {
+        const int e = i * 32 + lane, y = e & 7;
+        pow[(y < 4 ? y : (y - 4) ^ 1) * C::POWROW + (e >> 3) * 2 + (y >> 2)] = exp2_int(exps[e]) * scale;
+      }
+      __syncwarp();
+    }
   };
 
-  uint32_t qf[QS][N::Q][2];
-  float o[MD][4], m[2], l[2];
-  bool dead = false;
-  // entry of an S tile's row g (and, + 8, of row g + 8): see the header on the free order
-  const int er = (g & 1) ? 4 + ((g >> 1) ^ 1) : g >> 1;
-
-  for (int x = wlo; x < whi; ++x) {
-    const int b = nb, row = nrow, tile = ntile, n = nn, nt = (n + TT - 1) / TT;
-    const int64_t grow = (int64_t)b * per_seq + row;
-    const int valid = min(TT, n - tile * TT);
-    const uint32_t parity = (x - wlo) & 1;
-    const bool lost = __any_sync(~0u, npage == -1);
-    if (x == wlo || tile == 0) {       // a new row: its queries, and an empty state
-      const int hk = row / p.chunks, h = (row % p.chunks) * kHeadsPerRow + g;
-      const T *q = (const T *)p.q + b * p.qs + (int64_t)(hk * p.group + h) * D + t * (D / 4);
+  for (int x = wlo; x < whi;) {
+    lost |= __any_sync(~0u, rows_c == kLost);
+    if (x == wlo || cur.u == 0) {          // a new row: its queries, and an empty state
+      const int h = cur.ch * kHeadsPerRow + g;
+      const T *q = (const T *)p.q + cur.b * p.qs + (int64_t)(cur.hk * p.group + h) * D + t * (D / 4);
+      constexpr int QV = D / 4 * sizeof(T) / 16;
+      uint4 raw[QV];
 #pragma unroll
-      for (int s = 0; s < QS; ++s) {
-        constexpr int per = FMT == 8 ? 4 : 2;
-        float f[per];
+      for (int i = 0; i < QV; ++i) raw[i] = h < p.group ? reinterpret_cast<const uint4 *>(q)[i] : make_uint4(0, 0, 0, 0);
+      T f[D / 4];
+      memcpy(f, raw, sizeof f);
 #pragma unroll
-        for (int j = 0; j < per; ++j) f[j] = h < p.group ? to_f32(q[s * per + j]) : 0.0f;
-        if (FMT == 8) {
-          uint32_t u[N::Q], w[N::Q];
-          split_bf16<N::Q>(f[0], f[1], u);
-          split_bf16<N::Q>(f[per - 2], f[per - 1], w);
-#pragma unroll
-          for (int i = 0; i < N::Q; ++i) {
-            qf[s][i][0] = u[i];
-            qf[s][i][1] = w[i];
-          }
-        } else {
-          uint32_t u[N::Q], w[N::Q];
-          split_tf32<N::Q>(f[0], u);
-          split_tf32<N::Q>(f[1], w);
-#pragma unroll
-          for (int i = 0; i < N::Q; ++i) {
-            qf[s][i][0] = u[i];
-            qf[s][i][1] = w[i];
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < MD; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.0f;
-    }
-    // ---- scores: S^T[entry, head] ----
-    if (!dead) dead = !bar_wait(kbar, parity, p.error);
-    float s[MT][4];
-    float kscale[MT][2];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
-      const int e = i * 16 + er;
-      kscale[i][0] = FMT == 8 ? exp2_int(ske[e]) * p.scale : p.scale;
-      kscale[i][1] = FMT == 8 ? exp2_int(ske[e + 8]) * p.scale : p.scale;
-      if (FMT == 8) {
-        uint32_t a0[D / 16], a1[D / 16];
-        const uint8_t *r0 = sk + e * C::ROWB + t * (D / 4), *r1 = r0 + 8 * C::ROWB;
-        if constexpr (D % 64 == 0) {
-#pragma unroll
-          for (int w = 0; w < D / 64; ++w) {
-            *reinterpret_cast<uint4 *>(a0 + 4 * w) = reinterpret_cast<const uint4 *>(r0)[w];
-            *reinterpret_cast<uint4 *>(a1 + 4 * w) = reinterpret_cast<const uint4 *>(r1)[w];
-          }
-        } else {
-#pragma unroll
-          for (int w = 0; w < D / 32; ++w) {
-            *reinterpret_cast<uint2 *>(a0 + 2 * w) = reinterpret_cast<const uint2 *>(r0)[w];
-            *reinterpret_cast<uint2 *>(a1 + 2 * w) = reinterpret_cast<const uint2 *>(r1)[w];
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < QS; ++w) {
-          const uint32_t a[4] = {pair8(a0[w], 0, a0[w], 1), pair8(a1[w], 0, a1[w], 1), pair8(a0[w], 2, a0[w], 3),
-                                 pair8(a1[w], 2, a1[w], 3)};
-#pragma unroll
-          for (int j = N::Q - 1; j >= 0; --j) mma_bf16(s[i], a, qf[w][j][0], qf[w][j][1]);
-        }
-      } else {
-        const uint8_t *r0 = sk + e * C::ROWB + t * (D / 2), *r1 = r0 + 8 * C::ROWB;
-#pragma unroll
-        for (int w = 0; w < D / 32; ++w) {      // 8 codes of each row
-          const uint4 x0 = reinterpret_cast<const uint4 *>(r0)[w], x1 = reinterpret_cast<const uint4 *>(r1)[w];
-          const uint32_t y0[4] = {x0.x, x0.y, x0.z, x0.w}, y1[4] = {x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t u0 = y0[k] ^ 0x80008000u, u1 = y1[k] ^ 0x80008000u;
-            const uint32_t a[4] = {decode16(__uint_as_float(__byte_perm(u0, 0x4B00u, 0x5410))),
-                                   decode16(__uint_as_float(__byte_perm(u1, 0x4B00u, 0x5410))),
-                                   decode16(__uint_as_float(__byte_perm(u0, 0x4B00u, 0x5432))),
-                                   decode16(__uint_as_float(__byte_perm(u1, 0x4B00u, 0x5432)))};
-#pragma unroll
-            for (int j = N::Q - 1; j >= 0; --j) mma_tf32(s[i], a, qf[w * 4 + k][j][0], qf[w * 4 + k][j][1]);
-          }
-        }
-      }
-    }
-    __syncwarp();
-    // ---- the next tile's keys ----
-    const bool more = x + 1 < whi;
-    if (more) {
-      ++nx;
-      ++ntile;
-      if (ntile == nt) {
-        ntile = 0;
-        if (++nrow == per_seq) {
-          nrow = 0;
-          do ++nb;
-          while (before[nb + 1] == before[nb]);
-          nn = length(nb);
-        }
-      }
-      pages();
-      if (!dead) fetch(false);
-    }
-    // ---- weights ----
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = i * 16 + er + (j >> 1) * 8;
-        s[i][j] = e < valid ? s[i][j] * kscale[i][j >> 1] : -INFINITY;
-        mx[j & 1] = fmaxf(mx[j & 1], s[i][j]);
-      }
-    if (p.raw) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int s = 0; s < DN; ++s)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int e = i * 16 + er + j * 8;
-          if (e < valid && 2 * t < p.gp)
-            *reinterpret_cast<float2 *>(p.raw + ((grow * p.max_len + tile * TT + e) * p.gp + 2 * t)) =
-                make_float2(s[i][2 * j], s[i][2 * j + 1]);
-        }
-    }
-    float alpha[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(~0u, mx[j], d));
-      const float mn = fmaxf(m[j], mx[j]);
-      // nothing but -inf so far: weigh it with 0
-      const float at = mn == -INFINITY ? 0.0f : mn;
-      alpha[j] = ex2(m[j] - at);
-      l[j] *= alpha[j];
-      m[j] = mn;
-      mx[j] = at;
-    }
-    if (!dead) dead = !bar_wait(vbar, parity, p.error);
-    if (lost || dead) l[0] = l[1] = NAN;
-    // ---- O^T += V^T P^T ----
-    float acc[MD][4];
-#pragma unroll
-    for (int i = 0; i < MD; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      float w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = ex2(s[i][j] - mx[j & 1]);
-        l[j & 1] += w[j];
-      }
-      if (FMT == 8) {
-        const int e = i * 16 + er;
-        const float v0 = exp2_int(sve[e]), v1 = exp2_int(sve[e + 8]);
-        // (entries behind the length have weight 0 and any exponent: 0 times a finite power)
-        uint32_t u0[N::P], u1[N::P];
-        split_bf16<N::P>(w[0] * v0, w[1] * v0, u0);
-        split_bf16<N::P>(w[2] * v1, w[3] * v1, u1);
-#pragma unroll
-        for (int j = 0; j < N::P; ++j) {
-          u0[j] = transpose8x8(u0[j]);
-          u1[j] = transpose8x8(u1[j]);
-        }
-        // this thread's entries of the 16: t, 4 + (t ^ 1), 8 + t, 12 + (t ^ 1)
-        uint32_t a[4][D / 32];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint8_t *r = sv + (i * 16 + k * 4 + ((k & 1) ? t ^ 1 : t)) * C::ROWB + g * (D / 8);
-          if constexpr (D == 128) *reinterpret_cast<uint4 *>(a[k]) = *reinterpret_cast<const uint4 *>(r);
-          else if constexpr (D == 64) *reinterpret_cast<uint2 *>(a[k]) = *reinterpret_cast<const uint2 *>(r);
-          else
-#pragma unroll
-            for (int y = 0; y < D / 32; ++y) a[k][y] = reinterpret_cast<const uint32_t *>(r)[y];
-        }
-#pragma unroll
-        for (int d = 0; d < MD; ++d) {
-          const int y = d >> 1, k = (d & 1) * 2;
-          const uint32_t v[4] = {pair8(a[0][y], k, a[1][y], k), pair8(a[0][y], k + 1, a[1][y], k + 1),
-                                 pair8(a[2][y], k, a[3][y], k), pair8(a[2][y], k + 1, a[3][y], k + 1)};
-#pragma unroll
-          for (int j = N::P - 1; j >= 0; --j) mma_bf16(acc[d], v, u0[j], u1[j]);
-        }
-      } else {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {        // rows 0-7 and 8-15: one MMA step of 8 entries each
-          const uint32_t lo16 = transpose8x8(__byte_perm(__float_as_uint(w[2 * half]), __float_as_uint(w[2 * half + 1]), 0x5410));
-          const uint32_t hi16 = transpose8x8(pack_high(__float_as_uint(w[2 * half]), __float_as_uint(w[2 * half + 1])));
-          uint32_t u0[N::P], u1[N::P];
-          split_tf32<N::P>(__uint_as_float(__byte_perm(lo16, hi16, 0x5410)), u0);
-          split_tf32<N::P>(__uint_as_float(__byte_perm(lo16, hi16, 0x7632)), u1);
-          uint32_t a[2][D / 16];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint8_t *r = sv + (i * 16 + half * 8 + (k ? 4 + (t ^ 1) : t)) * C::ROWB + g * (D / 4);
-            if constexpr (D % 64 == 0) {
-#pragma unroll
-              for (int y = 0; y < D / 64; ++y)
-                *reinterpret_cast<uint4 *>(a[k] + 4 * y) = reinterpret_cast<const uint4 *>(r)[y];
-            } else {
-#pragma unroll
-              for (int y = 0; y < D / 32; ++y)
-                *reinterpret_cast<uint2 *>(a[k] + 2 * y) = reinterpret_cast<const uint2 *>(r)[y];
-            }
-          }
-#pragma unroll
-          for (int d = 0; d < MD; ++d) {
-            const uint32_t x0 = a[0][d] ^ 0x80008000u, x1 = a[1][d] ^ 0x80008000u;
-            const uint32_t v[4] = {decode16(__uint_as_float(__byte_perm(x0, 0x4B00u, 0x5410))),
-                                   decode16(__uint_as_float(__byte_perm(x0, 0x4B00u, 0x5432))),
-                                   decode16(__uint_as_float(__byte_perm(x1, 0x4B00u, 0x5410))),
-                                   decode16(__uint_as_float(__byte_perm(x1, 0x4B00u, 0x5432)))};
-#pragma unroll
-            for (int j = N::P - 1; j >= 0; --j) mma_tf32(acc[d], v, u0[j], u1[j]);
+          const float y = to_f32(f[2 * s + j]);
+          if (F32) {
+            qf[s][2 * j] = tf32_high(y);
+            qf[s][2 * j + 1] = to_tf32(y - __uint_as_float(tf32_high(y)));
+          } else {
+            qf[s][j] = __float_as_uint(y);     // bf16 and fp16 are tf32 values
           }
         }
+#pragma unroll
+      for (int i = 0; i < DN; ++i) o[i][0] = o[i][1] = 0.0f;
+      m = -INFINITY;
+      l = 0.0f;
+      at_row = cur.u;
+      lost = __any_sync(~0u, rows_c == kLost);
+    }
+    // the next tile's pages are looked up while this one's keys are worked on
+    const int next = x + cur.count;
+    const bool more = next < whi;
+    if (more) {
+      advance(nxt, whi - next);
+      rows_n = rows_of(nxt);
+    }
+    const int valid = cur.n - cur.u * 16;
+    if (cur.count == TU && valid >= TT) {
+      float s[TT / 8][2];
+      copy_wait_but_one();
+      scores(s, 0);
+      powers(ske, kpow, p.scale);
+      __syncwarp();
+      if (more) fetch(nxt, rows_n, false);
+      else copy_commit();
+      const float alpha = weights(s, 0, TT);
+      copy_wait_but_one();
+      powers(sve, vpow, 1.0f);
+      values(s, 0, alpha);
+      __syncwarp();
+      if (more) fetch(nxt, rows_n, true);
+      else copy_commit();
+    } else {
+      copy_wait_but_one();
+      copy_commit();
+      copy_wait_but_one();
+      powers(ske, kpow, p.scale);
+      powers(sve, vpow, 1.0f);
+#pragma unroll 1
+      for (int i = 0; i < cur.count; ++i) {
+        float s[2][2];
+        scores(s, i);
+        values(s, i, weights(s, i, valid - i * 16));
+      }
+      __syncwarp();
+      if (more) {
+        fetch(nxt, rows_n, false);
+        fetch(nxt, rows_n, true);
       }
     }
-#pragma unroll
-    for (int d = 0; d < MD; ++d)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[d][j] = fmaf(o[d][j], alpha[j & 1], acc[d][j]);
-    __syncwarp();
-    if (more && !dead) fetch(true);
 
     // ---- the end of a row, or of this warp's range ----
-    if (tile + 1 == nt || !more) {
+    const bool ended = cur.u + cur.count == units_of(cur.n);
+    if (ended || !more) {
+      l += __shfl_xor_sync(~0u, l, 1);
+      l += __shfl_xor_sync(~0u, l, 2);
+      if (lost) l = NAN;
+      const int row = cur.b * per_seq + cur.row;
+      // this thread holds head g, columns t D/4 .. (t + 1) D/4
+      if (at_row == 0 && ended) {
+        const int64_t head = head_of(p, RowId{cur.b, cur.hk, cur.ch}, g);
+        if (head >= 0) {
+          const float inv = 1.0f / l;
+          T f[D / 4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(~0u, l[j], d);
-      const bool begun = x - tile >= wlo, ended = tile + 1 == nt;
-      if (begun && ended) {
+            for (int d = 0; d < DN; ++d) f[j * DN + d] = from_f32<T>(o[d][j] * inv);
+          uint4 raw[sizeof f / 16];
+          memcpy(raw, f, sizeof f);
+          uint4 *out = reinterpret_cast<uint4 *>((T *)p.out + head * D + t * (D / 4));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int h = 2 * t + j, ch = row % p.chunks, gh = ch * kHeadsPerRow + h;
-          if (gh < p.group) {
-            T *out = (T *)p.out + ((int64_t)b * p.heads + (row / p.chunks) * p.group + gh) * D + g * (D / 8);
-            const float inv = 1.0f / l[j];
-#pragma unroll
-            for (int d = 0; d < MD; ++d) {
-              out[2 * d] = from_f32<T>(o[d][j] * inv);
-              out[2 * d + 1] = from_f32<T>(o[d][2 + j] * inv);
-            }
-          }
-          if (g == 0) write_lse(p, grow, h, m[j] + log2f(l[j]));
+          for (int i = 0; i < (int)(sizeof f / 16); ++i) out[i] = raw[i];
         }
+        if (t == 0) write_lse(p, row, g, head, m + log2f(l));
       } else {
         // a part: inside the range it goes to the workspace (the stage holds the next tile), at its end to the stage
         const int slot = more ? 0 : 1;
-        float *rec = more ? p.warp_rec + ((int64_t)cta * NW + warp) * C::REC : reinterpret_cast<float *>(stage);
+        float4 *rec = reinterpret_cast<float4 *>(
+            (more ? p.warp_rec + ((int64_t)cta * NW + warp) * C::REC : reinterpret_cast<float *>(stage)) + g * D +
+            t * (D / 4));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float *r = rec + (2 * t + j) * D + g * (D / 8);
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int d = 0; d < MD; ++d) {
-            r[2 * d] = o[d][j];
-            r[2 * d + 1] = o[d][2 + j];
-          }
-          if (g == 0) {
-            rec_ml[(warp * 2 + slot) * 16 + 2 * t + j] = m[j];
-            rec_ml[(warp * 2 + slot) * 16 + 8 + 2 * t + j] = l[j];
-          }
+          for (int d = 0; d < DN; d += 4)
+            rec[(j * DN + d) / 4] = make_float4(o[d][j], o[d + 1][j], o[d + 2][j], o[d + 3][j]);
+        if (t == 0) {
+          rec_ml[(warp * 2 + slot) * 16 + g] = m;
+          rec_ml[(warp * 2 + slot) * 16 + 8 + g] = l;
         }
-        if (lane == 0) rec_row[warp * 2 + slot] = (int)grow;
+        if (lane == 0) rec_row[warp * 2 + slot] = row;
       }
     }
-  }
-  if (dead) {      // the copies in flight may still land: wait for them, with a limit
-    const long long t0 = clock64();
-    while (clock64() - t0 < kKvDrainLimit)
-      if (bar_try(kbar, (fetched[0] - 1) & 1) && bar_try(vbar, (fetched[1] - 1) & 1)) break;
+    x = next;
+    cur = nxt;
+    rows_c = rows_n;
   }
   __syncthreads();
 
-  // ---- join the parts of this CTA's rows ----
-  int4 open = make_int4(-1, 0, 0, 0);
-  for (int i = 0; i < NW * 2;) {
-    const int row = rec_row[i];
-    if (row < 0) {
-      ++i;
-      continue;
-    }
-    int z = i + 1;
-    while (z < NW * 2 && (rec_row[z] == row || rec_row[z] < 0)) ++z;
-    const int b = row / per_seq, nt = (before[b + 1] - before[b]) / per_seq;
-    const int x0 = before[b] + (row - b * per_seq) * nt, x1 = x0 + nt;
+  // ---- join the parts of this CTA's rows: a warp takes 32 columns of a head, a lane one part's statistics ----
+  static_assert(NW * 2 <= 32, "a part per lane");
+  int2 open = make_int2(-1, 0);
+  const int mine = lane < NW * 2 ? rec_row[lane] : -1;
+  const float *rec = (lane & 1) ? reinterpret_cast<const float *>(smem + C::stage_at(lane >> 1))
+                                : p.warp_rec + ((int64_t)cta * NW + (lane >> 1)) * C::REC;
+  for (uint32_t left = __ballot_sync(~0u, mine >= 0); left;) {
+    const int row = __shfl_sync(~0u, mine, __ffs(left) - 1);
+    const bool in = mine == row;
+    const uint32_t parts = __ballot_sync(~0u, in);
+    left &= ~parts;
+    const RowId id = row_id(p, row);
+    const int nu = units_of(length(id.b));
+    const int x0 = before[id.b] + (row - id.b * per_seq) * nu, x1 = x0 + nu;
     const bool whole = x0 >= lo && x1 <= hi;
-    float *out = p.cta_rec + ((int64_t)cta * 2 + (x0 >= lo)) * (C::REC + 16);
-    for (int e = tid; e < C::REC; e += NT) {
+    float *out = p.cta_rec + (cta * 2 + (x0 >= lo)) * (C::REC + 16);
+#pragma unroll 1
+    for (int e = warp * 32; e < C::REC; e += NT) {
       const int h = e / D;
-      float M = -INFINITY, L = 0.0f, O = 0.0f;
-      for (int k = i; k < z; ++k)
-        if (rec_row[k] == row) M = fmaxf(M, rec_ml[k * 16 + h]);
-      for (int k = i; k < z; ++k)
-        if (rec_row[k] == row) {
-          const float a = ex2(rec_ml[k * 16 + h] - M);
-          const float *rec = (k & 1) ? reinterpret_cast<const float *>(smem + C::LUT + (k >> 1) * C::STAGE)
-                                     : p.warp_rec + ((int64_t)cta * NW + (k >> 1)) * C::REC;
-          L = fmaf(rec_ml[k * 16 + 8 + h], a, L);
-          O = fmaf(rec[e], a, O);
-        }
+      const float mp = in ? rec_ml[lane * 16 + h] : -INFINITY;
+      float M = mp;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+      const float a = in ? ex2(mp - M) : 0.0f;
+      float L = in ? rec_ml[lane * 16 + 8 + h] * a : 0.0f, O = 0.0f;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
+#pragma unroll 1
+      for (uint32_t rest = parts; rest; rest &= rest - 1) {
+        const int k = __ffs(rest) - 1;
+        const float *r = reinterpret_cast<const float *>(__shfl_sync(~0u, (unsigned long long)rec, k));
+        O = fmaf(r[e + lane], __shfl_sync(~0u, a, k), O);
+      }
       if (whole) {
-        write_out<T>(p, row, h, e - h * D, D, O / L);
-        if (e % D == 0) write_lse(p, row, h, M + log2f(L));
+        const int64_t head = head_of(p, id, h);
+        if (head >= 0) ((T *)p.out)[head * D + (e + lane) % D] = from_f32<T>(O / L);
+        if (e % D == 0 && lane == 0) write_lse(p, row, h, head, M + log2f(L));
       } else {
-        out[e] = O;
-        if (e % D == 0) {
+        out[e + lane] = O;
+        if (e % D == 0 && lane == 0) {
           out[C::REC + h] = M;
           out[C::REC + 8 + h] = L;
         }
       }
     }
-    if (x0 >= lo && x1 > hi) {
-      // the CTA that holds tile x1 - 1 is the last one of this row
-      const int last = (int)(((int64_t)x1 * ctas - 1) / total);
-      open = make_int4(row, last - cta + 1, 0, 0);
-    }
-    i = z;
+    // (the CTA that holds the row's last unit is the last one with a part)
+    if (x0 >= lo && x1 > hi) open = make_int2(row, deal.part_of(x1 - 1) - cta + 1);
   }
   if (tid == 0) p.cta_row[cta] = open;
 }
@@ -728,7 +719,13 @@ template <int FMT, int D, typename T>
 int launch_kv_attend_one(const AttendParams &p, int grid, cudaStream_t s) {
   using C = AttendCfg<FMT, D>;
   const size_t bytes = C::smem(p.c.batch);
-  static_assert(C::FIXED + 4 * 4097 <= 232448, "shared memory per CTA");
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return set_error(kENoDev, "k_kv_attend: no device");
+  static_assert(C::FIXED + 4 * 2049 <= 232448, "shared memory per CTA");
+  int reserved = 0;
+  if (FMT == 8 && (cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, device) != cudaSuccess ||
+                   reserved != kSharedReserved))
+    return set_error(kENoDev, "k_kv_attend: shared memory starts at %d, not %d", reserved, kSharedReserved);
   cudaError_t e = cudaFuncSetAttribute(k_kv_attend<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return set_error(kECuda, "k_kv_attend: %s", cudaGetErrorString(e));
   k_kv_attend<FMT, D, T><<<grid, C::NW * 32, bytes, s>>>(p);
