@@ -401,22 +401,22 @@ def bp32_to_f64(codes: torch.Tensor, row_exp=None, col_exp=None) -> torch.Tensor
 _ACT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _act(t, name: str, shape, cache, dtype=None) -> torch.Tensor:
+def _act(t, name: str, rows, heads, cache, dtype=None) -> torch.Tensor:
     """`t` as [rows, heads, head_dim] activations that the cache's kernels can
     read: heads contiguous, rows 16 bytes apart or more (copied if not)."""
     if not isinstance(t, torch.Tensor) or t.device != cache.device:
         raise ValueError(f"{name} must be a CUDA tensor on {cache.device}")
     if t.dtype not in _ACT or (dtype is not None and t.dtype != dtype):
         raise ValueError(f"{name} must be {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
-    if t.dim() != 3 or t.shape[2] != cache.head_dim or (shape[0] is not None and t.shape[0] != shape[0]) or \
-            (shape[1] is not None and t.shape[1] != shape[1]):
-        want = [shape[0] if shape[0] is not None else "rows", shape[1] if shape[1] is not None else "heads",
-                cache.head_dim]
-        raise ValueError(f"{name} must be {want}, got {list(t.shape)}")
+    D = cache.head_dim
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != D or (rows is not None and shape[0] != rows) or \
+            (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be {['rows' if rows is None else rows, 'heads' if heads is None else heads, D]}, "
+                         f"got {list(shape)}")
     s0, s1, s2 = t.stride()
-    per = 16 // t.element_size()
-    if s2 != 1 or (s1 != t.shape[2] and t.shape[1] > 1) or s0 % per or s0 < t.shape[1] * t.shape[2] or \
-            t.data_ptr() & 15:
+    if s2 != 1 or (s1 != D and shape[1] > 1) or s0 & (3 if t.dtype == torch.float32 else 7) or \
+            s0 < shape[1] * D or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -430,16 +430,26 @@ def _ints(t, name: str, n: int, cache):
     return t.data_ptr()
 
 
+def _like(out, q: torch.Tensor, name: str) -> torch.Tensor:
+    """`out`, or a new contiguous tensor of q's shape and type."""
+    if out is None:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if not isinstance(out, torch.Tensor) or out.dtype != q.dtype or out.shape != q.shape or \
+            out.device != q.device or not out.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor like q")
+    return out
+
+
 def _call(fn, device, *args):
     """fn(*args, stream) on `device`'s current stream, with `device` current."""
     i = device.index
     if torch.cuda.current_device() != i:
         with torch.cuda.device(i):
-            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-        if rc:
-            _lib.check(rc)
+    if rc:
+        _lib.check(rc)
 
 
 def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=None, positions=None, seqs=None,
@@ -447,46 +457,41 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=Non
     """Write new keys and values k, v [tokens, kv_heads, head_dim] (float32,
     bfloat16 or float16; views of a fused projection are read in place) into one
     layer of a kv.PagedKVCache.  Token t goes to entry places[t] of sequence
-    seqs[t] (int32; a pair outside the cache, such as -1, drops the token), or,
-    without them, to the last entry of sequence t.  With cos, sin [rows,
-    head_dim/2] (float32) keys, and queries q [tokens, heads, head_dim], are
-    rotated by the tables' rows positions[t] (int32; default: the place) on the
-    way, in float64, rounded once; returns the rotated queries (or None).
+    seqs[t] (int32; a pair outside the cache, such as -1, drops the token; two
+    tokens must not share an entry), or, without them, to the last entry of
+    sequence t.  With cos, sin [rows, head_dim/2] (float32) keys, and queries q
+    [tokens, heads, head_dim], are rotated by the tables' rows positions[t]
+    (int32; default: the place; NaN outside the tables) on the way, in float64,
+    rounded once; returns the rotated queries (or None).
     A bp8 cache stores each row as round-to-nearest bp8 codes of x / 2^e, e =
     floor(log2 max|x|) - 3; a bp16 cache as round-to-nearest-even bp16 codes."""
-    k = _act(k, "k", (None, cache.kv_heads), cache)
+    k = _act(k, "k", None, cache.kv_heads, cache)
+    dt = k.dtype
     n = k.shape[0]
-    v = _act(v, "v", (n, cache.kv_heads), cache, k.dtype)
-    heads = qs = 0
-    rows = 0
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin come together")
-    if cos is not None:
-        half = cache.head_dim // 2
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            if not isinstance(t, torch.Tensor) or t.device != cache.device or t.dtype != torch.float32 or \
-                    t.dim() != 2 or t.shape[1] != half or t.shape[0] != cos.shape[0] or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous float32 CUDA tensor [rows, {half}]")
-        rows = cos.shape[0]
+    v = _act(v, "v", n, cache.kv_heads, cache, dt)
+    rows = heads = qs = 0
+    cp = sp = qp = op = None
+    if cos is not None or sin is not None:
+        if cos is None or sin is None:
+            raise ValueError("cos and sin come together")
+        shape = (cos.shape[0], cache.head_dim // 2)
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.shape != shape or t.device != cache.device or not t.is_contiguous():
+                raise ValueError(f"cos and sin must be contiguous float32 CUDA tensors [rows, {shape[1]}]")
+        rows, cp, sp = shape[0], cos.data_ptr(), sin.data_ptr()
     if q is not None:
         if cos is None:
             raise ValueError("queries are only rotated: give cos and sin")
-        q = _act(q, "q", (n, None), cache, k.dtype)
-        heads, qs = q.shape[1], q.stride(0)
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif q_out.dtype != q.dtype or q_out.shape != q.shape or q_out.device != q.device or \
-                not q_out.is_contiguous():
-            raise ValueError("q_out must be a contiguous tensor like q")
-    if places is None and seqs is None and n != cache.batch:
-        raise ValueError(f"{n} tokens for {cache.batch} sequences: give seqs and places")
+        q = _act(q, "q", n, None, cache, dt)
+        q_out = _like(q_out, q, "q_out")
+        heads, qs, qp, op = q.shape[1], q.stride(0), q.data_ptr(), q_out.data_ptr()
     if (places is None) != (seqs is None):
         raise ValueError("seqs and places come together")
-    _call(_lib.lib().bp_kv_append, cache.device, cache._ref, layer, _ACT[k.dtype], n, k.data_ptr(), k.stride(0),
-          v.data_ptr(), v.stride(0), None if q is None else q.data_ptr(), heads, qs,
-          None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), rows,
-          _ints(positions, "positions", n, cache), _ints(seqs, "seqs", n, cache), _ints(places, "places", n, cache),
-          None if q is None else q_out.data_ptr())
+    if places is None and n != cache.batch:
+        raise ValueError(f"{n} tokens for {cache.batch} sequences: give seqs and places")
+    _call(_lib.lib().bp_kv_append, cache.device, cache._ref, layer, _ACT[dt], n, k.data_ptr(), k.stride(0),
+          v.data_ptr(), v.stride(0), qp, heads, qs, cp, sp, rows, _ints(positions, "positions", n, cache),
+          _ints(seqs, "seqs", n, cache), _ints(places, "places", n, cache), op)
     return None if q is None else q_out
 
 
@@ -501,24 +506,23 @@ def paged_attention(cache, q: torch.Tensor, layer: int = 0, scale: float | None 
     scale: default head_dim ** -0.5.  accumulate: add the weight that each entry
     receives, summed over the query heads of its kv head, to cache.scores.
     max_length: entries at or past it are left out (default: the capacity); a
-    bound of the lengths keeps the workspace of `accumulate` small."""
-    q = _act(q, "q", (cache.batch, None), cache)
-    heads, dev = q.shape[1], cache.device
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.device != q.device or not out.is_contiguous():
-        raise ValueError("out must be a contiguous tensor like q")
+    bound of the lengths keeps the workspace of `accumulate` small.  The order of
+    the sums follows from the lengths of the whole batch: the same call gives
+    the same bits, another batch may round differently."""
+    q = _act(q, "q", cache.batch, None, cache)
+    heads, dev, dt = q.shape[1], cache.device, q.dtype
+    out = _like(out, q, "out")
     lse = torch.empty((cache.batch, heads), dtype=torch.float32, device=dev) if return_lse else None
-    if scale is None:
-        scale = cache.head_dim ** -0.5
-    if max_length is not None and max_length < 1:
+    if max_length is None:
+        max_length = 0
+    elif max_length < 1:
         raise ValueError("max_length must be positive")
     L = _lib.lib()
-    need = L.bp_paged_attention_workspace_size(cache._ref, heads, max_length or 0, int(accumulate))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(L.bp_paged_attention, dev, cache._ref, layer, _ACT[q.dtype], heads, q.data_ptr(), q.stride(0),
-          out.data_ptr(), None if lse is None else lse.data_ptr(), scale, max_length or 0, int(accumulate),
-          None if ws is None else ws.data_ptr(), need)
+    need = L.bp_paged_attention_workspace_size(cache._ref, heads, max_length, accumulate)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(L.bp_paged_attention, dev, cache._ref, layer, _ACT[dt], heads, q.data_ptr(), q.stride(0), out.data_ptr(),
+          None if lse is None else lse.data_ptr(), cache.head_dim ** -0.5 if scale is None else scale, max_length,
+          accumulate, ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 

@@ -9,48 +9,69 @@
 namespace bp {
 namespace {
 
-constexpr int kJoinThreads = kHeadsPerRow * 32;
-constexpr int kJoinParts = 256;     // CTAs of one launch, at most
+constexpr int kJoinParts = 256;     // CTAs of one launch, at most: a part per thread
 
-// Joins the parts of a row that several CTAs of k_kv_attend worked on: block c
-// takes the row that starts in CTA c's range and goes on behind it, a warp for
-// each head, blockIdx.y for each 32 columns of the output.  Launched
-// early (programmatic dependent launch), so its latency hides behind the main
-// kernel; the parts of a row are few and in L2.
+// Joins the parts of a row that several CTAs of k_kv_attend worked on: block
+// (c, h) takes head h of the row that starts in CTA c's range and goes on behind
+// it.  Every part's maximum and sum is one thread's, its output one of 8 warps',
+// so that three rounds of loads (the row, the statistics, the outputs) are all
+// that is waited for, whatever the number of parts.  Launched early
+// (programmatic dependent launch), its start hides behind the main kernel.
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) k_kv_join(AttendParams p) {
-  __shared__ float weight[kHeadsPerRow][kJoinParts];   // 2^(m - M) of each part
+__global__ void __launch_bounds__(kJoinParts) k_kv_join(AttendParams p) {
+  __shared__ float weight[kJoinParts], sums[8][128], ml[2][8];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 open = p.cta_row[blockIdx.x];
   if (open.x < 0) return;
-  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y, h = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t head = head_of(p, row_id(p, open.x), h);
+  if (head < 0) {
+    if (tid == 0) write_lse(p, open.x, h, head, 0.0f);
+    return;
+  }
   // the first part is the CTA's second record (a row that starts there), the others are first records
   const float *base = p.cta_rec + (int64_t)blockIdx.x * 2 * (rec + 16);
   const int64_t step = 2 * (rec + 16);
-  const float *first = base + rec + 16;
-  auto part = [&](int k) { return k ? base + k * step : first; };
-  // one warp per head: the maximum and the sum over the parts
-  float M = -INFINITY, L = 0.0f;
-  for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[rec + warp]);
+  auto part = [&](int k) { return k ? base + k * step : base + rec + 16; };
+  const bool in = tid < parts;
+  const float m = in ? part(tid)[rec + h] : -INFINITY, l = in ? part(tid)[rec + 8 + h] : 0.0f;
+  float M = m;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
-  for (int k = lane; k < parts; k += 32) {
-    const float a = ex2(part(k)[rec + warp] - M);
-    L = fmaf(part(k)[rec + 8 + warp], a, L);
-    weight[warp][k] = a;
-  }
+  if (lane == 0) ml[0][warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) M = fmaxf(M, ml[0][w]);
+  const float a = in ? ex2(m - M) : 0.0f;
+  weight[tid] = a;
+  float L = l * a;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
-  __syncwarp();
-  const int64_t head = head_of(p, row_id(p, open.x), warp);
-  if (lane == 0 && blockIdx.y == 0) write_lse(p, open.x, warp, head, M + log2f(L));
-  if (head < 0) return;
-  const int d = blockIdx.y * 32 + lane;
-  float O = 0.0f;
-#pragma unroll 8
-  for (int k = 0; k < parts; ++k) O = fmaf(part(k)[warp * D + d], weight[warp][k], O);
-  ((T *)p.out)[head * D + d] = from_f32<T>(O / L);
+  if (lane == 0) ml[1][warp] = L;
+  __syncthreads();
+  L = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) L += ml[1][w];
+  float O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int k = warp; k < parts; k += 8) {
+    const float *r = part(k) + h * D + lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i * 32 < D) O[i] = fmaf(r[i * 32], weight[k], O[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sums[warp][i * 32 + lane] = O[i];
+  __syncthreads();
+  if (tid < D) {
+    float o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) o += sums[w][tid];
+    ((T *)p.out)[head * D + tid] = from_f32<T>(o / L);
+  }
+  if (tid == 0) write_lse(p, open.x, h, head, M + log2f(L));
 }
 
 // scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2):
@@ -188,10 +209,12 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   p.raw = accumulate ? (float *)(base + l.raw) : nullptr;
   p.gp = raw_heads(p.group);
   rc = p.c.fmt == 8 ? launch_kv_attend8(p, dtype, grid, s) : launch_kv_attend16(p, dtype, grid, s);
-  if (rc == kOk) {
-    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid, p.c.dim / 32), p, s, "k_kv_join");
-    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid, p.c.dim / 32), p, s, "k_kv_join");
-    else rc = launch_after(k_kv_join<__half>, dim3(grid, p.c.dim / 32), p, s, "k_kv_join");
+  // (a batch of at most kMinUnits units is one CTA's, and no row of it is in parts)
+  const int64_t units = (int64_t)cache->batch * cache->kv_heads * p.chunks * ((p.max_len + 15) / 16);
+  if (rc == kOk && units > kMinUnits) {
+    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join");
+    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join");
+    else rc = launch_after(k_kv_join<__half>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join");
   }
   if (rc == kOk && accumulate && p.max_len)
     rc = launch_after(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), p, s, "k_kv_scores");

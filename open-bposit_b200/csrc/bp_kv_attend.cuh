@@ -67,6 +67,7 @@ struct AttendParams {
 };
 
 constexpr int kMaxWarps = 16;
+constexpr int kMaxBatch = 2048;
 constexpr int kTableAt = 65536;                     // shared address of the bp8 decode table
 constexpr int kSharedReserved = 1024;               // shared address where a block's own memory starts
 
@@ -74,7 +75,7 @@ constexpr int kSharedReserved = 1024;               // shared address where a bl
 inline int raw_heads(int group) { return group >= kHeadsPerRow ? kHeadsPerRow : (group + 1) & ~1; }
 
 // Tile and launch shape of one instance.
-template <int FMT, int D>
+template <int FMT, int D, typename T>
 struct AttendCfg {
   static constexpr int BYTES = FMT / 8;
   static constexpr int ROWB = D * BYTES;
@@ -88,7 +89,10 @@ struct AttendCfg {
   // a row stride that keeps the four rows in different banks
   static constexpr int POWROW = TT / 4 + 4;
   static constexpr int POWB = FMT == 8 ? 2 * 4 * POWROW * 4 : 0;
-  static constexpr int STAGE = 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;
+  // keys, values, their exponents, the powers, and the queries of the next row (read once, when it starts)
+  static constexpr int QAT = 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;
+  static constexpr int QROW = D * (int)sizeof(T) + 16;           // padded: the 8 heads' pieces in different banks
+  static constexpr int STAGE = QAT + kHeadsPerRow * QROW;
   static constexpr int REC = kHeadsPerRow * D;                   // floats of one part's output
   // Shared memory (bp8): the decode table at shared addresses 64 K .. 128 K, so that an entry's address is the
   // bytes {lane, code, 1, 0}; FRONT stages below it, the others above.  (bp16: no table, all stages in front.)
@@ -96,10 +100,11 @@ struct AttendCfg {
   static constexpr int BACK = NW - (FRONT < NW ? FRONT : NW);
   // offset of what follows the table, from shared address kSharedReserved
   static constexpr int AFTER = FMT == 8 ? 2 * kTableAt - kSharedReserved : 0;
-  // part statistics [NW][2][16], part rows [NW][2], scan [NW + 2], tiles before each sequence [batch + 1]
+  // part statistics [NW][2][16], part rows [NW][2], scan [NW + 2], units before each sequence [batch + 1], lengths
+  // [batch]
   static constexpr int META = AFTER + (FMT == 8 ? BACK : NW) * STAGE;
   static constexpr int FIXED = META + NW * 2 * 64 + NW * 2 * 4 + (NW + 2) * 4;
-  static size_t smem(int batch) { return FIXED + (size_t)(batch + 1) * 4; }
+  static size_t smem(int batch) { return FIXED + (size_t)(2 * batch + 1) * 4; }
   static __device__ __forceinline__ int stage_at(int warp) {
     return warp < FRONT ? warp * STAGE : AFTER + (warp - FRONT) * STAGE;
   }
@@ -247,8 +252,8 @@ constexpr int kMinUnits = 32;
 __device__ __forceinline__ int active_ctas(int units, int grid) { return min((units + kMinUnits - 1) / kMinUnits, grid); }
 
 template <int FMT, int D, typename T>
-__global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(AttendParams p) {
-  using C = AttendCfg<FMT, D>;
+__global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(AttendParams p) {
+  using C = AttendCfg<FMT, D, T>;
   constexpr int TT = C::TT, NW = C::NW, NT = NW * 32;
   constexpr int TU = TT / 16;           // units per tile
   constexpr int DN = D / 8;             // 8-wide columns of O, and MMA steps along D
@@ -260,19 +265,32 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
   int *const rec_row = reinterpret_cast<int *>(rec_ml + NW * 32);           // [NW][2]
   int *const scan = rec_row + NW * 2;
   int *const before = scan + NW + 2;                                        // [batch + 1]
+  int *const lens = before + p.c.batch + 1;                                 // [batch]
   const KvView &c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_seq = c.kv_heads * p.chunks;             // work rows of one sequence
   asm volatile("griddepcontrol.launch_dependents;");
 
   auto length = [&](int b) { return min(c.length(b), p.max_len); };
+  if (FMT == 8) {          // the decode table: word 64 code + lane
+    for (int i = tid; i < 256; i += NT) {
+      const uint32_t v = posit_to_f32_bits<8, 2>(i);
+      uint4 *row = reinterpret_cast<uint4 *>(smem + (kTableAt - kSharedReserved)) + i * 16;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) row[(j + i) & 7] = make_uint4(v, v, v, v);
+    }
+  }
   // units before each sequence
   {
     const int each = (c.batch + NT - 1) / NT;
     int mine = 0;
     for (int i = 0; i < each; ++i) {
       const int b = tid * each + i;
-      if (b < c.batch) mine += (length(b) + 15) / 16 * per_seq;
+      if (b < c.batch) {
+        const int n = length(b);
+        lens[b] = n;
+        mine += (n + 15) / 16 * per_seq;
+      }
     }
     int incl = mine;
 #pragma unroll
@@ -289,7 +307,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
       const int b = tid * each + i;
       if (b < c.batch) {
         before[b] = at;
-        at += (length(b) + 15) / 16 * per_seq;
+        at += (lens[b] + 15) / 16 * per_seq;
       }
     }
     if (tid == NT - 1) before[c.batch] = at;
@@ -338,47 +356,66 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
         w.row = w.hk = 0;
         do ++w.b;
         while (before[w.b + 1] == before[w.b]);
-        w.n = length(w.b);
+        w.n = lens[w.b];
       }
     }
     w.count = min(min(TU, units_of(w.n) - w.u), left);
   };
-  // Pool row of the first entry of the tile's unit `lane` (its others follow): kLost when its page is outside the
-  // pool, kBehind when the tile has no such unit.
-  constexpr uint32_t kLost = ~0u, kBehind = ~0u - 1;
-  auto rows_of = [&](const Place &w) {
-    const int i = (w.u + lane) * 16;
-    if (lane >= w.count) return kBehind;
-    const int pg = c.page_of(w.b, i);
-    return pg < 0 ? kLost : (uint32_t)c.row(pg, w.hk, i);
+  // Page of the tile's unit `lane` (-1: the tile has no such unit).
+  auto page_of = [&](const Place &w) {
+    return lane < w.count ? c.table[(int64_t)w.b * c.max_pages + ((w.u + lane) * 16 >> c.page_shift)] : -1;
   };
   const uint32_t stage_s = smem_addr(stage);
   constexpr int CPR = C::ROWB / 16;        // 16-byte pieces per row
   constexpr int PJ = CPR / 2;              // pieces per lane of 16 rows
   // piece `lane` of 16 rows; piece j * 32 + lane lies 512 j behind it, permuted alike (see below for 256-byte rows)
   const uint32_t to = swizzle<C::ROWB>(lane / CPR, lane % CPR);
-  auto fetch = [&](const Place &w, uint32_t rows, bool value) {
+  // (looking a page up and using it are apart, so that the copies and not the look-up wait for it)
+  auto fetch = [&](const Place &w, int page, bool value, bool first) {
     const uint8_t *pool = (value ? c.v : c.k) + lane * 16;
     const uint32_t dst = stage_s + (value ? C::TILEB : 0) + to;
     const int valid = w.n - w.u * 16;
+    constexpr uint32_t kNone = ~0u;        // pools have fewer rows
+    const uint32_t rows = (unsigned)page < (unsigned)c.pages ? (uint32_t)c.row(page, w.hk, (w.u + lane) * 16) : kNone;
+    uint32_t row[TU];
 #pragma unroll
-    for (int i = 0; i < TU; ++i) {
-      const uint32_t row = __shfl_sync(~0u, rows, i);
-      if (row >= kBehind) continue;        // (the same for all lanes)
-      const uint8_t *src = pool + (uint64_t)row * C::ROWB;
+    for (int i = 0; i < TU; ++i) row[i] = __shfl_sync(~0u, rows, i);
+    if (valid >= TT && __all_sync(~0u, lane >= TU || rows != kNone)) {
 #pragma unroll
-      for (int j = 0; j < PJ; ++j) {
-        const uint32_t d = dst + i * 16 * C::ROWB + j * 512;
-        if (i * 16 + (j * 32 + lane) / CPR < valid) copy16(CPR == 16 && (j & 1) ? d ^ 64 : d, src + j * 512);
+      for (int i = 0; i < TU; ++i) {
+        const uint8_t *src = pool + (uint64_t)row[i] * C::ROWB;
+#pragma unroll
+        for (int j = 0; j < PJ; ++j) {
+          const uint32_t d = dst + i * 16 * C::ROWB + j * 512;
+          copy16(CPR == 16 && (j & 1) ? d ^ 64 : d, src + j * 512);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < w.count; ++i) {
+        const uint32_t r = __shfl_sync(~0u, rows, i);
+        const uint8_t *src = pool + (uint64_t)r * C::ROWB;
+#pragma unroll
+        for (int j = 0; j < PJ; ++j) {
+          const uint32_t d = dst + i * 16 * C::ROWB + j * 512;
+          if (r != kNone && i * 16 + (j * 32 + lane) / CPR < valid) copy16(CPR == 16 && (j & 1) ? d ^ 64 : d, src + j * 512);
+        }
       }
     }
-    if (FMT == 8 && rows < kBehind)
+    if (!value && (w.u == 0 || first)) {   // a new row for this warp: its queries, 4 lanes a head
+      const int h = w.ch * kHeadsPerRow + g;
+      const uint8_t *q = reinterpret_cast<const uint8_t *>((const T *)p.q + w.b * p.qs + (int64_t)(w.hk * p.group + h) * D);
+#pragma unroll
+      for (int i = 0; i < D * (int)sizeof(T) / 64; ++i)
+        if (h < p.group) copy16(stage_s + C::QAT + g * C::QROW + (i * 4 + t) * 16, q + (i * 4 + t) * 16);
+    }
+    if (FMT == 8 && rows != kNone)
       copy16(stage_s + 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + rows);
     copy_commit();
   };
 
   Place cur{}, nxt{};
-  uint32_t rows_c = kBehind, rows_n = kBehind;
+  int page_c = -1, page_n = -1;
   if (wlo < whi) {
     int a = 0, z = c.batch;                // sequence of the first unit, by bisection
     while (z - a > 1) {
@@ -387,27 +424,18 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
       else z = mid;
     }
     cur.b = a;
-    cur.n = length(a);
+    cur.n = lens[a];
     const int r = wlo - before[a], nu = units_of(cur.n);
     cur.row = r / nu;
     cur.u = r - cur.row * nu;
     cur.hk = cur.row / p.chunks;
     cur.ch = cur.row - cur.hk * p.chunks;
     cur.count = min(min(TU, nu - cur.u), whi - wlo);
-    rows_c = rows_of(cur);
+    page_c = page_of(cur);
     nxt = cur;
   }
-  if (FMT == 8) {
-    // the decode table: word 64 code + lane
-    for (int i = tid; i < 256; i += NT) {
-      const uint32_t v = posit_to_f32_bits<8, 2>(i);
-      uint4 *row = reinterpret_cast<uint4 *>(smem + (kTableAt - kSharedReserved)) + i * 16;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) row[(j + i) & 7] = make_uint4(v, v, v, v);
-    }
-  }
-  fetch(cur, rows_c, false);
-  fetch(cur, rows_c, true);
+  fetch(cur, page_c, false, true);
+  fetch(cur, page_c, true, false);
   __syncthreads();
   const uint32_t entry = lane * 4 | (kTableAt >> 16) << 8;
   // fp32 bits of code k of a word
@@ -432,20 +460,29 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
   // S[head, entry] = q K^T
   auto scores = [&](auto &s, int i0) {
     constexpr int SN = sizeof(s) / sizeof(s[0]);
+    // four columns at a time: an MMA waits for the one before it in its sum
+    constexpr int G = SN < 4 ? SN : 4;
 #pragma unroll
-    for (int i = 0; i < SN; ++i) {
-      uint32_t kw[KW];
-      load_words<C::ROWB>(sk + (i0 * 16 + i * 8) * C::ROWB, er, t * KW, kw);
-      float c4[4];
+    for (int i = 0; i < SN; i += G) {
+      uint32_t kw[G][KW];
+      float c4[G][4];
+#pragma unroll
+      for (int k = 0; k < G; ++k) load_words<C::ROWB>(sk + (i0 * 16 + (i + k) * 8) * C::ROWB, er, t * KW, kw[k]);
 #pragma unroll
       for (int w = 0; w < DN; ++w) {
-        const uint32_t b0 = decode(kw[2 * w / CW], 2 * w % CW), b1 = decode(kw[2 * w / CW], 2 * w % CW + 1);
         const uint32_t a[4] = {qf[w][0], F32 ? qf[w][1] : 0u, qf[w][F32 ? 2 : 1], F32 ? qf[w][F32 ? 3 : 0] : 0u};
-        if (w == 0) mma_tf32_first(c4, a, b0, b1);
-        else mma_tf32(c4, a, b0, b1);
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          const uint32_t b0 = decode(kw[k][2 * w / CW], 2 * w % CW), b1 = decode(kw[k][2 * w / CW], 2 * w % CW + 1);
+          if (w == 0) mma_tf32_first(c4[k], a, b0, b1);
+          else mma_tf32(c4[k], a, b0, b1);
+        }
       }
-      s[i][0] = F32 ? c4[0] + c4[2] : c4[0];
-      s[i][1] = F32 ? c4[1] + c4[3] : c4[1];
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        s[i + k][0] = F32 ? c4[k][0] + c4[k][2] : c4[k][0];
+        s[i + k][1] = F32 ? c4[k][1] + c4[k][3] : c4[k][1];
+      }
     }
   };
   // S becomes e^(S - maximum), maximum and sum move on; returns the factor for what was summed before
@@ -539,14 +576,22 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
   };
 
   for (int x = wlo; x < whi;) {
-    lost |= __any_sync(~0u, rows_c == kLost);
+    lost |= __any_sync(~0u, lane < cur.count && (unsigned)page_c >= (unsigned)c.pages);
+    // the next tile's pages are looked up while this one's keys are worked on
+    const int next = x + cur.count;
+    const bool more = next < whi;
+    if (more) {
+      advance(nxt, whi - next);
+      page_n = page_of(nxt);
+    }
+    copy_wait_but_one();
     if (x == wlo || cur.u == 0) {          // a new row: its queries, and an empty state
-      const int h = cur.ch * kHeadsPerRow + g;
-      const T *q = (const T *)p.q + cur.b * p.qs + (int64_t)(cur.hk * p.group + h) * D + t * (D / 4);
+      const uint4 *q = reinterpret_cast<const uint4 *>(stage + C::QAT + g * C::QROW + t * (D / 4) * (int)sizeof(T));
       constexpr int QV = D / 4 * sizeof(T) / 16;
+      const bool real = cur.ch * kHeadsPerRow + g < p.group;
       uint4 raw[QV];
 #pragma unroll
-      for (int i = 0; i < QV; ++i) raw[i] = h < p.group ? reinterpret_cast<const uint4 *>(q)[i] : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < QV; ++i) raw[i] = real ? q[i] : make_uint4(0, 0, 0, 0);
       T f[D / 4];
       memcpy(f, raw, sizeof f);
 #pragma unroll
@@ -566,33 +611,24 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
       m = -INFINITY;
       l = 0.0f;
       at_row = cur.u;
-      lost = __any_sync(~0u, rows_c == kLost);
-    }
-    // the next tile's pages are looked up while this one's keys are worked on
-    const int next = x + cur.count;
-    const bool more = next < whi;
-    if (more) {
-      advance(nxt, whi - next);
-      rows_n = rows_of(nxt);
+      lost = __any_sync(~0u, lane < cur.count && (unsigned)page_c >= (unsigned)c.pages);
     }
     const int valid = cur.n - cur.u * 16;
     if (cur.count == TU && valid >= TT) {
       float s[TT / 8][2];
-      copy_wait_but_one();
       scores(s, 0);
       powers(ske, kpow, p.scale);
       __syncwarp();
-      if (more) fetch(nxt, rows_n, false);
+      if (more) fetch(nxt, page_n, false, false);
       else copy_commit();
       const float alpha = weights(s, 0, TT);
       copy_wait_but_one();
       powers(sve, vpow, 1.0f);
       values(s, 0, alpha);
       __syncwarp();
-      if (more) fetch(nxt, rows_n, true);
+      if (more) fetch(nxt, page_n, true, false);
       else copy_commit();
     } else {
-      copy_wait_but_one();
       copy_commit();
       copy_wait_but_one();
       powers(ske, kpow, p.scale);
@@ -605,8 +641,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
       }
       __syncwarp();
       if (more) {
-        fetch(nxt, rows_n, false);
-        fetch(nxt, rows_n, true);
+        fetch(nxt, page_n, false, false);
+        fetch(nxt, page_n, true, false);
       }
     }
 
@@ -654,57 +690,68 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D>::NW * 32, 1) k_kv_attend(Att
     }
     x = next;
     cur = nxt;
-    rows_c = rows_n;
+    page_c = page_n;
   }
   __syncthreads();
 
-  // ---- join the parts of this CTA's rows: a warp takes 32 columns of a head, a lane one part's statistics ----
-  static_assert(NW * 2 <= 32, "a part per lane");
+  // ---- join the parts of this CTA's rows: a warp takes a head, a lane one part's statistics and D / 32 columns ----
+  // (a row has at most one part in the workspace, its last one here: it ended inside a warp's range)
+  static_assert(NW * 2 <= 32 && NW >= kHeadsPerRow, "a part per lane, a head per warp");
   int2 open = make_int2(-1, 0);
   const int mine = lane < NW * 2 ? rec_row[lane] : -1;
-  const float *rec = (lane & 1) ? reinterpret_cast<const float *>(smem + C::stage_at(lane >> 1))
-                                : p.warp_rec + ((int64_t)cta * NW + (lane >> 1)) * C::REC;
   for (uint32_t left = __ballot_sync(~0u, mine >= 0); left;) {
-    const int row = __shfl_sync(~0u, mine, __ffs(left) - 1);
+    const int row = __shfl_sync(~0u, mine, __ffs(left) - 1), h = warp;
     const bool in = mine == row;
     const uint32_t parts = __ballot_sync(~0u, in);
     left &= ~parts;
     const RowId id = row_id(p, row);
-    const int nu = units_of(length(id.b));
+    const int nu = units_of(lens[id.b]);
     const int x0 = before[id.b] + (row - id.b * per_seq) * nu, x1 = x0 + nu;
-    const bool whole = x0 >= lo && x1 <= hi;
-    float *out = p.cta_rec + (cta * 2 + (x0 >= lo)) * (C::REC + 16);
-#pragma unroll 1
-    for (int e = warp * 32; e < C::REC; e += NT) {
-      const int h = e / D;
-      const float mp = in ? rec_ml[lane * 16 + h] : -INFINITY;
-      float M = mp;
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
-      const float a = in ? ex2(mp - M) : 0.0f;
-      float L = in ? rec_ml[lane * 16 + 8 + h] * a : 0.0f, O = 0.0f;
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
-#pragma unroll 1
-      for (uint32_t rest = parts; rest; rest &= rest - 1) {
-        const int k = __ffs(rest) - 1;
-        const float *r = reinterpret_cast<const float *>(__shfl_sync(~0u, (unsigned long long)rec, k));
-        O = fmaf(r[e + lane], __shfl_sync(~0u, a, k), O);
-      }
-      if (whole) {
-        const int64_t head = head_of(p, id, h);
-        if (head >= 0) ((T *)p.out)[head * D + (e + lane) % D] = from_f32<T>(O / L);
-        if (e % D == 0 && lane == 0) write_lse(p, row, h, head, M + log2f(L));
-      } else {
-        out[e + lane] = O;
-        if (e % D == 0 && lane == 0) {
-          out[C::REC + h] = M;
-          out[C::REC + 8 + h] = L;
-        }
-      }
-    }
     // (the CTA that holds the row's last unit is the last one with a part)
     if (x0 >= lo && x1 > hi) open = make_int2(row, deal.part_of(x1 - 1) - cta + 1);
+    if (h >= kHeadsPerRow) continue;
+    const float mp = in ? rec_ml[lane * 16 + h] : -INFINITY;
+    float M = mp;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+    const float a = in ? ex2(mp - M) : 0.0f;
+    float L = in ? rec_ml[lane * 16 + 8 + h] * a : 0.0f, O[D / 32];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) O[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = __shfl_sync(~0u, a, 2 * w + 1);
+      if (parts >> (2 * w + 1) & 1) {
+        const float *r = reinterpret_cast<const float *>(smem + C::stage_at(w)) + h * D + lane;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) O[i] = fmaf(r[i * 32], f, O[i]);
+      }
+    }
+    if (const uint32_t last = parts & 0x55555555u) {
+      const int k = __ffs(last) - 1;
+      const float f = __shfl_sync(~0u, a, k);
+      const float *r = p.warp_rec + ((int64_t)cta * NW + (k >> 1)) * C::REC + h * D + lane;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) O[i] = fmaf(r[i * 32], f, O[i]);
+    }
+    if (x0 >= lo && x1 <= hi) {
+      const int64_t head = head_of(p, id, h);
+      if (head >= 0) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) ((T *)p.out)[head * D + i * 32 + lane] = from_f32<T>(O[i] / L);
+      }
+      if (lane == 0) write_lse(p, row, h, head, M + log2f(L));
+    } else {
+      float *out = p.cta_rec + (cta * 2 + (x0 >= lo)) * (C::REC + 16);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) out[h * D + i * 32 + lane] = O[i];
+      if (lane == 0) {
+        out[C::REC + h] = M;
+        out[C::REC + 8 + h] = L;
+      }
+    }
   }
   if (tid == 0) p.cta_row[cta] = open;
 }
@@ -717,11 +764,11 @@ int launch_kv_attend16(const AttendParams &p, int dtype, int grid, cudaStream_t 
 
 template <int FMT, int D, typename T>
 int launch_kv_attend_one(const AttendParams &p, int grid, cudaStream_t s) {
-  using C = AttendCfg<FMT, D>;
+  using C = AttendCfg<FMT, D, T>;
   const size_t bytes = C::smem(p.c.batch);
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return set_error(kENoDev, "k_kv_attend: no device");
-  static_assert(C::FIXED + 4 * 2049 <= 232448, "shared memory per CTA");
+  static_assert(C::FIXED + 4 * (2 * kMaxBatch + 1) <= 232448, "shared memory per CTA");
   int reserved = 0;
   if (FMT == 8 && (cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, device) != cudaSuccess ||
                    reserved != kSharedReserved))
