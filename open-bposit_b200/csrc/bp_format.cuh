@@ -273,6 +273,23 @@ BP_HD uint32_t bp16_encode_bits(uint32_t u, bool rtne) {
   return (sign << 15) | field;
 }
 
+// bp16_encode_bits(u, true) in closed form where the regime leaves all three
+// exponent bits: the field is base + (M rounded to nearest even at the dropped
+// bits), and a carry moves on to the next binade's field by itself.  Outside
+// (|x| beyond 2^+-88, subnormals, zero, inf, NaN) the bit-string form.
+BP_HD uint32_t bp16_encode_rtne(uint32_t u) {
+  const int E = (int)(u >> 23 & 0xFFu) - 127;
+  if (E < -88 || E > 87) return bp16_encode_bits(u, true);
+  const int k = E >> 3;
+  const int sh = k >= 0 ? 13 + k : 12 - k;                  // dropped mantissa bits: 23 - (12 - regime bits)
+  const uint32_t R = k >= 0 ? (2u << (k + 1)) - 2u : 1u;
+  const uint32_t base = (R << 3 | (uint32_t)(E & 7)) << (23 - sh);
+  const uint32_t M = u & 0x7FFFFFu;
+  const uint32_t odd = (base + (M >> sh)) & 1u;
+  const uint32_t field = base + ((M + (1u << (sh - 1)) - 1u + odd) >> sh);
+  return (u >> 31) ? 0x10000u - field : field;
+}
+
 // The same encoder as a per-binade table, for the streaming kernels.  Inside
 // one fp32 binade b (biased exponent) the regime and exponent bits are fixed,
 // so the 15-bit field is base(b) + (M >> sh(b)) with M the 23-bit mantissa,

@@ -1,5 +1,7 @@
 // bp_kv_append.cu -- writes new tokens into the paged key-value cache
 // (bp_kv_append) and holds the argument checks that the cache's calls share.
+#include <math.h>
+
 #include "bp_kv.cuh"
 
 namespace bp {
@@ -58,6 +60,8 @@ struct AppendParams {
   void *q_out;
 };
 
+constexpr int kAppendThreads = 128;
+
 // Four consecutive activations as fp32.
 __device__ __forceinline__ void load4(const float *p, float *x) {
   const float4 f = *reinterpret_cast<const float4 *>(p);
@@ -84,108 +88,127 @@ __device__ __forceinline__ void store4(T *p, const float *x) {
   *reinterpret_cast<uint2 *>(p) = w;
 }
 
-// One group of GW lanes handles one row (a head of q, k or v) of one token; a
-// lane holds four pairs (i, i + D/2), so that loads and stores are 16 bytes
-// (fp32) and a row's maximum is a shuffle within the group.  The rotation is
-// in float64: both products are exact there, so the result is the exact sum
-// rounded to float64 and then to fp32 whatever the order of evaluation.
+// A warp works on one token: groups of GW lanes take its rows (a head of k, v or
+// q) in turn, a lane four pairs (i, i + D/2) of a row, so that loads and stores
+// are 16 bytes (fp32) and a row's maximum is a shuffle within the group.  The
+// rotation is in float64: both products are exact there, so the result is the
+// exact sum rounded to float64 and then to fp32 whatever the order of
+// evaluation; the table's row is converted once per token.  The next row is
+// loaded while one is worked on.  gridDim.y warps share a token when there are
+// few tokens.
 template <typename T, int D, int FMT>
-__global__ void __launch_bounds__(128) k_kv_append(AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
   constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW;
   const KvView &c = p.c;
   const int rows = 2 * c.kv_heads + (p.q ? p.heads : 0);
-  const int chunks = (rows + RPW - 1) / RPW;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, sub = lane & (GW - 1);
-  if (w >= (int64_t)p.tokens * chunks) return;
-  const int t = (int)(w / chunks);
-  const int r = (int)(w % chunks) * RPW + lane / GW;
-  const bool on = r < rows && sub < GL;
-  const int part = r < c.kv_heads ? 0 : (r < 2 * c.kv_heads ? 1 : 2);
-  const int h = part == 2 ? r - 2 * c.kv_heads : (part == 1 ? r - c.kv_heads : r);
+  if (t >= p.tokens) return;
+  const int step = gridDim.y * RPW, first = blockIdx.y * RPW + lane / GW;
 
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-  if (on) {
-    const T *src = part == 0 ? (const T *)p.k + t * p.ks : (part == 1 ? (const T *)p.v + t * p.vs
-                                                                      : (const T *)p.q + t * p.qs);
-    src += h * D + sub * 4;
+  auto load = [&](int r, float *x) {     // row r of the token: k, v, then q heads
+    const T *src = r < c.kv_heads       ? (const T *)p.k + t * p.ks + r * D
+                   : r < 2 * c.kv_heads ? (const T *)p.v + t * p.vs + (r - c.kv_heads) * D
+                                        : (const T *)p.q + t * p.qs + (r - 2 * c.kv_heads) * D;
+    src += sub * 4;
     load4(src, x);
     load4(src + D / 2, x + 4);
-  }
-  int b = -1, place = -1;
+  };
+  float x[8], y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
+  if (first < rows && sub < GL) load(first, x);
+  int b = t, place;
   if (p.places) {
     b = p.seqs[t];
     place = p.places[t];
   } else {
-    b = t;
     place = c.length(t) - 1;
   }
   const int at = p.positions ? p.positions[t] : place;
-  if (on && part != 1 && p.cos) {
+  double cc[4], ss[4];
+  if (p.cos) {
     const bool known = (unsigned)at < (unsigned)p.rope_rows;
-    float cs[4], sn[4];
-    if (known) {
+    float cs[4] = {NAN, NAN, NAN, NAN}, sn[4] = {NAN, NAN, NAN, NAN};
+    if (known && sub < GL) {
       load4(p.cos + (int64_t)at * (D / 2) + sub * 4, cs);
       load4(p.sin + (int64_t)at * (D / 2) + sub * 4, sn);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const double cc = known ? (double)cs[i] : __longlong_as_double(0x7FF8000000000000LL);
-      const double ss = known ? (double)sn[i] : cc;
-      const double a = x[i], d = x[4 + i];
-      x[i] = (float)__dsub_rn(__dmul_rn(a, cc), __dmul_rn(d, ss));
-      x[4 + i] = (float)__dadd_rn(__dmul_rn(d, cc), __dmul_rn(a, ss));
+      cc[i] = cs[i];
+      ss[i] = sn[i];
     }
   }
-  if (on && part == 2) {
-    T *dst = (T *)p.q_out + ((int64_t)t * p.heads + h) * D + sub * 4;
-    store4(dst, x);
-    store4(dst + D / 2, x + 4);
-  }
-  int e = 0;
-  if (FMT == 8) {
-    uint32_t top = 0;
+  int page = -1;
+  if ((unsigned)b < (unsigned)c.batch && (unsigned)place < (unsigned)c.cap) page = c.page_of(b, place);
+
+  // (whole warps stay in the loop for the shuffles: a group without a row of its own has `on` false)
+  for (int r = first; r - lane / GW < rows; r += step) {
+    const bool on = r < rows && sub < GL;
+    if (r + step < rows && sub < GL) load(r + step, y);
+    const int part = r < c.kv_heads ? 0 : (r < 2 * c.kv_heads ? 1 : 2);
+    if (part != 1 && p.cos) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t a = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-      top = a < 0x7F800000u && a > top ? a : top;
+      for (int i = 0; i < 4; ++i) {
+        const double u = x[i], w = x[4 + i];
+        x[i] = (float)__fma_rn(u, cc[i], -__dmul_rn(w, ss[i]));
+        x[4 + i] = (float)__fma_rn(w, cc[i], __dmul_rn(u, ss[i]));
+      }
+    }
+    if (part == 2) {
+      if (on) {
+        T *dst = (T *)p.q_out + ((int64_t)t * p.heads + r - 2 * c.kv_heads) * D + sub * 4;
+        store4(dst, x);
+        store4(dst + D / 2, x + 4);
+      }
+    }
+    if (__any_sync(~0u, part != 2)) {
+      int e = 0;
+      if (FMT == 8) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t a = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+          top = a < 0x7F800000u && a > top ? a : top;
+        }
+#pragma unroll
+        for (int d = GW / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+        e = top ? max(f32_floor_log2(top) - 3, -126) : 0;
+      }
+      if (on && part != 2 && page >= 0) {
+        const int h = part == 0 ? r : r - c.kv_heads;
+        const int64_t row = c.row(page, h, place);
+        uint8_t *pool = part == 0 ? c.k : c.v;
+        if (FMT == 8) {
+          uint32_t lo = 0, hi = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            lo |= bp8_encode_exp(__float_as_uint(x[i]), e) << (8 * i);
+            hi |= bp8_encode_exp(__float_as_uint(x[4 + i]), e) << (8 * i);
+          }
+          *reinterpret_cast<uint32_t *>(pool + row * D + sub * 4) = lo;
+          *reinterpret_cast<uint32_t *>(pool + row * D + D / 2 + sub * 4) = hi;
+          if (sub == 0) (part == 0 ? c.k_exp : c.v_exp)[row] = (int8_t)e;
+        } else {
+          uint32_t o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            o[i] = bp16_encode_rtne(__float_as_uint(x[2 * i])) |
+                   (bp16_encode_rtne(__float_as_uint(x[2 * i + 1])) << 16);
+          uint16_t *dst = (uint16_t *)pool + row * D + sub * 4;
+          *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0], o[1]);
+          *reinterpret_cast<uint2 *>(dst + D / 2) = make_uint2(o[2], o[3]);
+        }
+        if (part == 0 && sub == 0) {
+          const int64_t i = ((int64_t)b * c.kv_heads + h) * c.cap + place;
+          if (c.positions) c.positions[i] = at;
+          if (c.scores) c.scores[i] = 0.0f;
+        }
+      }
     }
 #pragma unroll
-    for (int d = GW / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
-    e = top ? max(f32_floor_log2(top) - 3, -126) : 0;
-  }
-  if (!on || part == 2) return;
-  if ((unsigned)b >= (unsigned)c.batch || (unsigned)place >= (unsigned)c.cap) return;
-  const int page = c.page_of(b, place);
-  if (page < 0) return;
-  const int64_t row = c.row(page, h, place);
-  uint8_t *pool = part == 0 ? c.k : c.v;
-  if (FMT == 8) {
-    uint32_t lo = 0, hi = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lo |= bp8_encode_exp(__float_as_uint(x[i]), e) << (8 * i);
-      hi |= bp8_encode_exp(__float_as_uint(x[4 + i]), e) << (8 * i);
-    }
-    *reinterpret_cast<uint32_t *>(pool + row * D + sub * 4) = lo;
-    *reinterpret_cast<uint32_t *>(pool + row * D + D / 2 + sub * 4) = hi;
-    if (sub == 0) (part == 0 ? c.k_exp : c.v_exp)[row] = (int8_t)e;
-  } else {
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      o[i] = bp16_encode_bits(__float_as_uint(x[2 * i]), true) |
-             (bp16_encode_bits(__float_as_uint(x[2 * i + 1]), true) << 16);
-    uint16_t *dst = (uint16_t *)pool + row * D + sub * 4;
-    *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0], o[1]);
-    *reinterpret_cast<uint2 *>(dst + D / 2) = make_uint2(o[2], o[3]);
-  }
-  if (part == 0 && sub == 0) {
-    const int64_t i = ((int64_t)b * c.kv_heads + h) * c.cap + place;
-    if (c.positions) c.positions[i] = at;
-    if (c.scores) c.scores[i] = 0.0f;
+    for (int i = 0; i < 8; ++i) x[i] = y[i];
   }
 }
 
@@ -193,11 +216,14 @@ template <typename T, int D>
 int launch_append(const AppendParams &p, cudaStream_t s) {
   constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW;
   const int rows = 2 * p.c.kv_heads + (p.q ? p.heads : 0);
-  const int64_t warps = (int64_t)p.tokens * ((rows + RPW - 1) / RPW);
-  const int64_t blocks = (warps + 3) / 4;
-  if (blocks > 0x7FFFFFFF) return set_error(kERange, "bp_kv_append: too many tokens");
-  if (p.c.fmt == 8) k_kv_append<T, D, 8><<<(unsigned)blocks, 128, 0, s>>>(p);
-  else k_kv_append<T, D, 16><<<(unsigned)blocks, 128, 0, s>>>(p);
+  const unsigned blocks = (p.tokens + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+  // one warp a token once that fills the GPU (16 warps an SM); below, as many as the token has rows for
+  const int most = (rows + RPW - 1) / RPW;
+  int share = (int)(((int64_t)sm_count() * 16 + p.tokens - 1) / p.tokens);
+  share = share < most ? share : most;
+  const dim3 grid(blocks, share);
+  if (p.c.fmt == 8) k_kv_append<T, D, 8><<<grid, kAppendThreads, 0, s>>>(p);
+  else k_kv_append<T, D, 16><<<grid, kAppendThreads, 0, s>>>(p);
   return check_launch("k_kv_append");
 }
 

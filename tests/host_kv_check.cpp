@@ -9,3 +9,6 @@ extern "C" void kv_encode_bp8(const uint32_t *u, size_t n, int e, uint8_t *out) 
 extern "C" void kv_floor_log2(const uint32_t *a, size_t n, int *out) {
   for (size_t i = 0; i < n; ++i) out[i] = bp::f32_floor_log2(a[i]);
 }
+extern "C" void kv_encode_bp16(const uint32_t *u, size_t n, uint32_t *out) {
+  for (size_t i = 0; i < n; ++i) out[i] = bp::bp16_encode_rtne(u[i]);
+}
