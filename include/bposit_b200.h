@@ -330,10 +330,11 @@ typedef struct bp_kv_cache {
  * head_dim] (contiguous).  16-byte aligned pointers, strides of a multiple of
  * 16 bytes.
  * cos, sin: fp32 [rope_rows, head_dim / 2]; the rotation of pair (i, i +
- * head_dim/2) at position p is (a c - b s, b c + a s) in float64 with c, s
- * from row p, rounded once to fp32 (and then to q_out's dtype).  Both NULL:
- * keys are stored as given, and q must be NULL.  A position outside [0,
- * rope_rows) rotates with NaN.
+ * head_dim/2) at position p is (a c - b s, b c + a s) with c, s from row p: for
+ * keys in float64, rounded once to fp32; for queries in fp32 (one rounded
+ * product and an fma), then rounded to q_out's dtype.  Both NULL: keys are
+ * stored as given, and q must be NULL.  A position outside [0, rope_rows)
+ * rotates with NaN.
  * Token t goes to entry places[t] of sequence seqs[t]; with both NULL, to the
  * last entry (lengths[t] - 1) of sequence t, and tokens must equal batch.  A
  * sequence, entry or page outside the cache drops the write of that token (its

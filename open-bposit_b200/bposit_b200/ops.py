@@ -461,8 +461,8 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=Non
     tokens must not share an entry), or, without them, to the last entry of
     sequence t.  With cos, sin [rows, head_dim/2] (float32) keys, and queries q
     [tokens, heads, head_dim], are rotated by the tables' rows positions[t]
-    (int32; default: the place; NaN outside the tables) on the way, in float64,
-    rounded once; returns the rotated queries (or None).
+    (int32; default: the place; NaN outside the tables) on the way, keys in float64
+    and rounded once, queries in fp32; returns the rotated queries (or None).
     A bp8 cache stores each row as round-to-nearest bp8 codes of x / 2^e, e =
     floor(log2 max|x|) - 3; a bp16 cache as round-to-nearest-even bp16 codes."""
     k = _act(k, "k", None, cache.kv_heads, cache)

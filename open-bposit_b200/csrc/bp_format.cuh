@@ -273,21 +273,46 @@ BP_HD uint32_t bp16_encode_bits(uint32_t u, bool rtne) {
   return (sign << 15) | field;
 }
 
-// bp16_encode_bits(u, true) in closed form where the regime leaves all three
-// exponent bits: the field is base + (M rounded to nearest even at the dropped
-// bits), and a carry moves on to the next binade's field by itself.  Outside
-// (|x| beyond 2^+-88, subnormals, zero, inf, NaN) the bit-string form.
-BP_HD uint32_t bp16_encode_rtne(uint32_t u) {
-  const int E = (int)(u >> 23 & 0xFFu) - 127;
-  if (E < -88 || E > 87) return bp16_encode_bits(u, true);
-  const int k = E >> 3;
-  const int sh = k >= 0 ? 13 + k : 12 - k;                  // dropped mantissa bits: 23 - (12 - regime bits)
-  const uint32_t R = k >= 0 ? (2u << (k + 1)) - 2u : 1u;
-  const uint32_t base = (R << 3 | (uint32_t)(E & 7)) << (23 - sh);
-  const uint32_t M = u & 0x7FFFFFu;
-  const uint32_t odd = (base + (M >> sh)) & 1u;
-  const uint32_t field = base + ((M + (1u << (sh - 1)) - 1u + odd) >> sh);
-  return (u >> 31) ? 0x10000u - field : field;
+// Round-to-nearest encoders without tables or cases, for values whose regime
+// leaves all exponent bits.  Decoding such a code below 1 reads the exponent and
+// fraction of its magnitude m, as an fp32 number, as a fixed-point logarithm that
+// moves 2^es times as fast as the value's (see decode16 in bp_kv_attend.cuh);
+// so, backwards, `a`, the distance of the value's fp32 bits from those of 1.0,
+// divided by 2^es and taken from the bits of the magnitude of 1.0 are the bits
+// of m with its dropped bits as a fraction, and rounding that number to an
+// integer rounds the code.  What the division drops is or-ed into the last bit.
+// Above 1 the code is 2^(NB-1) - m.
+//
+// bp16, to nearest even: bits V of |x|, 2^-88 <= |x| < 2^88 (bp16_in_range).
+BP_HD bool bp16_in_range(uint32_t V) { return V - (39u << 23) < (176u << 23); }
+BP_HD bool bp8_in_range(uint32_t V) { return V - (111u << 23) < (32u << 23); }
+BP_HD float add_magic(uint32_t bits) {   // rounds to an integer, nearest even
+  float f;
+  memcpy(&f, &bits, 4);
+#ifdef __CUDA_ARCH__
+  return __fadd_rn(f, 8388608.0f);
+#else
+  volatile float g = f + 8388608.0f;
+  return g;
+#endif
+}
+BP_HD uint32_t bp16_encode_near(uint32_t V) {
+  const int32_t d = (int32_t)(V - 0x3F800000u), n = d < 0 ? d : -d;
+  const float f = add_magic((uint32_t)((141 << 23) + (n >> 3)) | ((n & 7) != 0));
+  uint32_t m;
+  memcpy(&m, &f, 4);
+  m -= 0x4B000000u;
+  return d > 0 ? 0x8000u - m : m;
+}
+// bp8, to the nearest value, ties to the smaller one: bits V of |x|, 2^-16 <= |x|
+// < 2^16 (bp8_in_range).  Half a bit less than V is never a tie.
+BP_HD uint32_t bp8_encode_near(uint32_t V) {
+  const int32_t d = (int32_t)(2u * V - 1u - 0x7F000000u), n = d < 0 ? d : -d;
+  const float f = add_magic((uint32_t)((133 << 23) + (n >> 3)) | 1u);
+  uint32_t m;
+  memcpy(&m, &f, 4);
+  m -= 0x4B000000u;
+  return d > 0 ? 0x80u - m : m;
 }
 
 // The same encoder as a per-binade table, for the streaming kernels.  Inside

@@ -53,6 +53,7 @@ namespace {
 struct AppendParams {
   KvView c;
   int tokens, heads, rope_rows;
+  int q_warps;               // warps of one token that take queries; the others take keys and values
   const void *k, *v, *q;
   int64_t ks, vs, qs;        // token strides, elements
   const float *cos, *sin;
@@ -88,36 +89,68 @@ __device__ __forceinline__ void store4(T *p, const float *x) {
   *reinterpret_cast<uint2 *>(p) = w;
 }
 
-// A warp works on one token: groups of GW lanes take its rows (a head of k, v or
-// q) in turn, a lane four pairs (i, i + D/2) of a row, so that loads and stores
-// are 16 bytes (fp32) and a row's maximum is a shuffle within the group.  The
-// rotation is in float64: both products are exact there, so the result is the
-// exact sum rounded to float64 and then to fp32 whatever the order of
-// evaluation; the table's row is converted once per token.  The next row is
-// loaded while one is worked on.  gridDim.y warps share a token when there are
-// few tokens.
-template <typename T, int D, int FMT>
+// A warp works on rows of one token, either keys and values or queries (a row is
+// a head): a group of GW lanes takes a row, a lane four pairs (i, i + D/2) of it,
+// so that loads and stores are 16 bytes (fp32) and a row's maximum is a shuffle
+// within the group.  Keys are rotated in float64: both products are exact there,
+// so the result is the exact sum rounded to float64 and then to fp32 whatever
+// the order of evaluation, and the codes that are stored do not depend on it.
+// Queries are rotated in fp32 (a product and an fma): converting all their values
+// to float64 and back took the conversion unit longer than the memory needs for
+// them.  With many tokens a group takes U rows of queries at a time, all loaded
+// before the first is worked on.
+// Codes of eight values of a row (bp8: of x / 2^e), four to a word or two.
+__device__ __noinline__ void encode_any(const float *x, int e, int fmt, uint32_t *o) {
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(x[i]);
+    if (fmt == 8) o[i >> 2] |= bp8_encode_exp(u, e) << 8 * (i & 3);
+    else o[i >> 1] |= bp16_encode_bits(u, true) << 16 * (i & 1);
+  }
+}
+template <int FMT>
+__device__ __forceinline__ void encode8(const float (&x)[8], int e, uint32_t (&o)[FMT / 4]) {
+  bool easy = true;
+  uint32_t m[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+    const uint32_t V = FMT == 8 ? a - ((uint32_t)e << 23) : a;
+    // (a bound on `a` too: subtracting e from an exponent of zero could wrap into the range)
+    easy = easy && (FMT == 8 ? bp8_in_range(V) && a - 0x00800000u < 0x7F000000u : bp16_in_range(V));
+    m[i] = FMT == 8 ? bp8_encode_near(V) : bp16_encode_near(V);
+    m[i] = __float_as_uint(x[i]) >> 31 ? 0u - m[i] : m[i];
+  }
+  if (FMT == 8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      o[i] = __byte_perm(__byte_perm(m[4 * i], m[4 * i + 1], 0x0040), __byte_perm(m[4 * i + 2], m[4 * i + 3], 0x0040), 0x5410);
+  } else {
+#pragma unroll
+    for (int i = 0; i < FMT / 4; ++i) o[i] = __byte_perm(m[(2 * i) & 7], m[(2 * i + 1) & 7], 0x5410);
+  }
+  if (!easy) {             // zeros, very small values, infinities, NaN
+    float y[8];
+    uint32_t w[FMT / 4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+#pragma unroll
+    for (int i = 0; i < FMT / 4; ++i) w[i] = 0;
+    encode_any(y, e, FMT, w);
+#pragma unroll
+    for (int i = 0; i < FMT / 4; ++i) o[i] = w[i];
+  }
+}
+
+template <typename T, int D, int FMT, int U>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
   constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW;
   const KvView &c = p.c;
-  const int rows = 2 * c.kv_heads + (p.q ? p.heads : 0);
   const int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, sub = lane & (GW - 1);
+  const int lane = threadIdx.x & 31, sub = lane & (GW - 1), grp = lane / GW;
   if (t >= p.tokens) return;
-  const int step = gridDim.y * RPW, first = blockIdx.y * RPW + lane / GW;
-
-  auto load = [&](int r, float *x) {     // row r of the token: k, v, then q heads
-    const T *src = r < c.kv_heads       ? (const T *)p.k + t * p.ks + r * D
-                   : r < 2 * c.kv_heads ? (const T *)p.v + t * p.vs + (r - c.kv_heads) * D
-                                        : (const T *)p.q + t * p.qs + (r - 2 * c.kv_heads) * D;
-    src += sub * 4;
-    load4(src, x);
-    load4(src + D / 2, x + 4);
-  };
-  float x[8], y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
-  if (first < rows && sub < GL) load(first, x);
+  const bool on = sub < GL, queries = (int)blockIdx.y < p.q_warps;
+  const int chunk = queries ? blockIdx.y : blockIdx.y - p.q_warps;
+  const int kv_rows = 2 * c.kv_heads;
   int b = t, place;
   if (p.places) {
     b = p.seqs[t];
@@ -126,115 +159,126 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
     place = c.length(t) - 1;
   }
   const int at = p.positions ? p.positions[t] : place;
-  double cc[4], ss[4];
-  if (p.cos) {
+
+  float x[U][8];
+  const T *src;
+  const int r0 = chunk * (queries ? RPW * U : RPW) + grp;
+  if (queries) {
+    src = (const T *)p.q + t * p.qs + r0 * D + sub * 4;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (on && r0 + i * RPW < p.heads) {
+        load4(src + i * RPW * D, x[i]);
+        load4(src + i * RPW * D + D / 2, x[i] + 4);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[0][i] = 0.0f;
+    src = r0 < c.kv_heads ? (const T *)p.k + t * p.ks + r0 * D : (const T *)p.v + t * p.vs + (r0 - c.kv_heads) * D;
+    if (on && r0 < kv_rows) {
+      load4(src + sub * 4, x[0]);
+      load4(src + sub * 4 + D / 2, x[0] + 4);
+    }
+  }
+  const bool key = r0 < c.kv_heads;
+  float cs[4], sn[4];
+  if (p.cos && (queries || key)) {
     const bool known = (unsigned)at < (unsigned)p.rope_rows;
-    float cs[4] = {NAN, NAN, NAN, NAN}, sn[4] = {NAN, NAN, NAN, NAN};
-    if (known && sub < GL) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cs[i] = sn[i] = NAN;
+    if (known && on) {
       load4(p.cos + (int64_t)at * (D / 2) + sub * 4, cs);
       load4(p.sin + (int64_t)at * (D / 2) + sub * 4, sn);
     }
+  }
+
+  if (queries) {
+    T *dst = (T *)p.q_out + ((int64_t)t * p.heads + r0) * D + sub * 4;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (on && r0 + i * RPW < p.heads) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          y[j] = __fmaf_rn(x[i][j], cs[j], -__fmul_rn(x[i][4 + j], sn[j]));
+          y[4 + j] = __fmaf_rn(x[i][4 + j], cs[j], __fmul_rn(x[i][j], sn[j]));
+        }
+        store4(dst + i * RPW * D, y);
+        store4(dst + i * RPW * D + D / 2, y + 4);
+      }
+    return;
+  }
+  if (key && p.cos) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      cc[i] = cs[i];
-      ss[i] = sn[i];
+      const double u = x[0][i], w = x[0][4 + i], cc = cs[i], ss = sn[i];
+      x[0][i] = (float)__fma_rn(u, cc, -__dmul_rn(w, ss));
+      x[0][4 + i] = (float)__fma_rn(w, cc, __dmul_rn(u, ss));
     }
   }
-  int page = -1;
-  if ((unsigned)b < (unsigned)c.batch && (unsigned)place < (unsigned)c.cap) page = c.page_of(b, place);
-
-  // (whole warps stay in the loop for the shuffles: a group without a row of its own has `on` false)
-  for (int r = first; r - lane / GW < rows; r += step) {
-    const bool on = r < rows && sub < GL;
-    if (r + step < rows && sub < GL) load(r + step, y);
-    const int part = r < c.kv_heads ? 0 : (r < 2 * c.kv_heads ? 1 : 2);
-    if (part != 1 && p.cos) {
+  int e = 0;
+  if (FMT == 8) {
+    uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double u = x[i], w = x[4 + i];
-        x[i] = (float)__fma_rn(u, cc[i], -__dmul_rn(w, ss[i]));
-        x[4 + i] = (float)__fma_rn(w, cc[i], __dmul_rn(u, ss[i]));
-      }
-    }
-    if (part == 2) {
-      if (on) {
-        T *dst = (T *)p.q_out + ((int64_t)t * p.heads + r - 2 * c.kv_heads) * D + sub * 4;
-        store4(dst, x);
-        store4(dst + D / 2, x + 4);
-      }
-    }
-    if (__any_sync(~0u, part != 2)) {
-      int e = 0;
-      if (FMT == 8) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t a = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-          top = a < 0x7F800000u && a > top ? a : top;
-        }
-#pragma unroll
-        for (int d = GW / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
-        e = top ? max(f32_floor_log2(top) - 3, -126) : 0;
-      }
-      if (on && part != 2 && page >= 0) {
-        const int h = part == 0 ? r : r - c.kv_heads;
-        const int64_t row = c.row(page, h, place);
-        uint8_t *pool = part == 0 ? c.k : c.v;
-        if (FMT == 8) {
-          uint32_t lo = 0, hi = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            lo |= bp8_encode_exp(__float_as_uint(x[i]), e) << (8 * i);
-            hi |= bp8_encode_exp(__float_as_uint(x[4 + i]), e) << (8 * i);
-          }
-          *reinterpret_cast<uint32_t *>(pool + row * D + sub * 4) = lo;
-          *reinterpret_cast<uint32_t *>(pool + row * D + D / 2 + sub * 4) = hi;
-          if (sub == 0) (part == 0 ? c.k_exp : c.v_exp)[row] = (int8_t)e;
-        } else {
-          uint32_t o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[i] = bp16_encode_rtne(__float_as_uint(x[2 * i])) |
-                   (bp16_encode_rtne(__float_as_uint(x[2 * i + 1])) << 16);
-          uint16_t *dst = (uint16_t *)pool + row * D + sub * 4;
-          *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0], o[1]);
-          *reinterpret_cast<uint2 *>(dst + D / 2) = make_uint2(o[2], o[3]);
-        }
-        if (part == 0 && sub == 0) {
-          const int64_t i = ((int64_t)b * c.kv_heads + h) * c.cap + place;
-          if (c.positions) c.positions[i] = at;
-          if (c.scores) c.scores[i] = 0.0f;
-        }
-      }
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = __float_as_uint(x[0][i]) & 0x7FFFFFFFu;
+      top = a < 0x7F800000u && a > top ? a : top;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i];
+    for (int d = GW / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+    e = top ? max(f32_floor_log2(top) - 3, -126) : 0;
+  }
+  if (!on || r0 >= kv_rows || (unsigned)b >= (unsigned)c.batch || (unsigned)place >= (unsigned)c.cap) return;
+  const int page = c.page_of(b, place);
+  if (page < 0) return;
+  const int h = key ? r0 : r0 - c.kv_heads;
+  const int64_t row = c.row(page, h, place);
+  uint8_t *pool = (key ? c.k : c.v) + row * (D * FMT / 8);
+  uint32_t o[FMT / 4];
+  encode8<FMT>(x[0], e, o);
+  if (FMT == 8) {
+    reinterpret_cast<uint32_t *>(pool)[sub] = o[0];
+    reinterpret_cast<uint32_t *>(pool)[D / 8 + sub] = o[1];
+    if (sub == 0) (key ? c.k_exp : c.v_exp)[row] = (int8_t)e;
+  } else {
+    reinterpret_cast<uint2 *>(pool)[sub] = make_uint2(o[0], o[1]);
+    reinterpret_cast<uint2 *>(pool)[D / 8 + sub] = make_uint2(o[FMT / 4 - 2], o[FMT / 4 - 1]);
+  }
+  if (key && sub == 0) {
+    const int64_t i = ((int64_t)b * c.kv_heads + h) * c.cap + place;
+    if (c.positions) c.positions[i] = at;
+    if (c.scores) c.scores[i] = 0.0f;
   }
 }
 
-template <typename T, int D>
-int launch_append(const AppendParams &p, cudaStream_t s) {
-  constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW;
-  const int rows = 2 * p.c.kv_heads + (p.q ? p.heads : 0);
+template <typename T, int D, int FMT>
+int launch_append(AppendParams p, cudaStream_t s) {
+  constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW, U = 4;
+  const int heads = p.q ? p.heads : 0;
   const unsigned blocks = (p.tokens + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-  // one warp a token once that fills the GPU (16 warps an SM); below, as many as the token has rows for
-  const int most = (rows + RPW - 1) / RPW;
-  int share = (int)(((int64_t)sm_count() * 16 + p.tokens - 1) / p.tokens);
-  share = share < most ? share : most;
-  const dim3 grid(blocks, share);
-  if (p.c.fmt == 8) k_kv_append<T, D, 8><<<grid, kAppendThreads, 0, s>>>(p);
-  else k_kv_append<T, D, 16><<<grid, kAppendThreads, 0, s>>>(p);
+  // one row of queries a group while that does not fill the GPU twice (16 x 1024 tokens x 14 heads of 64: 17.9 against
+  // 24.3 us with U = 1; 16 tokens: 5.0 against 5.6 us with U = 4)
+  const bool few = (int64_t)p.tokens * ((heads + RPW - 1) / RPW) < (int64_t)sm_count() * 64;
+  const int rows = few ? RPW : RPW * U;
+  p.q_warps = (heads + rows - 1) / rows;
+  const dim3 grid(blocks, p.q_warps + (2 * p.c.kv_heads + RPW - 1) / RPW);
+  if (few) k_kv_append<T, D, FMT, 1><<<grid, kAppendThreads, 0, s>>>(p);
+  else k_kv_append<T, D, FMT, U><<<grid, kAppendThreads, 0, s>>>(p);
   return check_launch("k_kv_append");
 }
 
-template <typename T>
+template <typename T, int FMT>
 int launch_append_dim(const AppendParams &p, cudaStream_t s) {
   switch (p.c.dim) {
-    case 32: return launch_append<T, 32>(p, s);
-    case 64: return launch_append<T, 64>(p, s);
-    case 96: return launch_append<T, 96>(p, s);
-    default: return launch_append<T, 128>(p, s);
+    case 32: return launch_append<T, 32, FMT>(p, s);
+    case 64: return launch_append<T, 64, FMT>(p, s);
+    case 96: return launch_append<T, 96, FMT>(p, s);
+    default: return launch_append<T, 128, FMT>(p, s);
   }
+}
+template <typename T>
+int launch_append_fmt(const AppendParams &p, cudaStream_t s) {
+  return p.c.fmt == 8 ? launch_append_dim<T, 8>(p, s) : launch_append_dim<T, 16>(p, s);
 }
 
 }  // namespace
@@ -274,7 +318,7 @@ extern "C" int bp_kv_append(const bp_kv_cache *cache, int layer, int dtype, int 
   p.k = k; p.v = v; p.q = q; p.ks = k_stride; p.vs = v_stride; p.qs = q_stride;
   p.cos = cos; p.sin = sin; p.positions = positions; p.seqs = seqs; p.places = places; p.q_out = q_out;
   cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == BP_F32) return launch_append_dim<float>(p, s);
-  if (dtype == BP_BF16) return launch_append_dim<__nv_bfloat16>(p, s);
-  return launch_append_dim<__half>(p, s);
+  if (dtype == BP_F32) return launch_append_fmt<float>(p, s);
+  if (dtype == BP_BF16) return launch_append_fmt<__nv_bfloat16>(p, s);
+  return launch_append_fmt<__half>(p, s);
 }

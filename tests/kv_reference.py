@@ -68,6 +68,18 @@ def rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tenso
     return torch.cat((a * c - b * s, b * c + a * s), dim=-1).float()
 
 
+def rotated_queries(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
+    """(rotation of x in float64, bound of an fp32 product and fma and the rounding to x's type)."""
+    a, b = x.double().cpu().chunk(2, dim=-1)
+    c, s = cos.double().cpu()[:, None], sin.double().cpu()[:, None]
+    y = torch.cat((a * c - b * s, b * c + a * s), dim=-1)
+    u, step = 2.0 ** -24, {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[x.dtype]
+    inner = u * torch.cat(((b * s).abs(), (a * s).abs()), dim=-1)      # the product that is rounded first
+    outer = inner + u * (y.abs() + inner)                              # the fma's own rounding
+    tiny = 2.0 ** -25 if x.dtype == torch.float16 else 2.0 ** -148     # half a step of the smallest numbers
+    return y, outer + step * (y.abs() + outer) + tiny
+
+
 def encode(orc, x: torch.Tensor, fmt: str):
     """Codes (numpy) and exponents (numpy int8 or None) of fp32 rows."""
     a = x.numpy()

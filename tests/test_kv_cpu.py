@@ -43,17 +43,22 @@ def test_row_encoder_matches_oracle(host, orc, e):
     assert np.array_equal(out, ref)
 
 
-def test_bp16_row_encoder_matches_oracle(host, orc):
-    """bp16_encode_rtne is the oracle's bp16 on a sweep of all patterns and on every binade's ties and edges."""
+@pytest.mark.parametrize("fmt", [8, 16])
+def test_closed_form_encoders_match_oracle(host, orc, fmt):
+    """The encoders without cases, on a sweep of all patterns and on every binade's ties and edges."""
     top = (np.arange(512, dtype=np.uint64) << 23)[:, None]
     low = np.concatenate([[0, 1, 0x7FFFFF, 0x7FFFFE, 0x400000, 0x3FFFFF, 0x400001],
-                          *[(np.array([1, 3, 5, 7]) << b) + d for b in range(10, 21) for d in (-1, 0, 1)]])
+                          *[(np.array([1, 3, 5, 7]) << b) + d for b in range(10, 23) for d in (-1, 0, 1)]])
     u = np.concatenate((np.arange(0, 1 << 32, 1021, dtype=np.uint64), (top + (low & 0x7FFFFF)[None]).reshape(-1)))
     u = np.ascontiguousarray(u.astype(np.uint32))
     out = np.empty(u.size, np.uint32)
-    host.kv_encode_bp16(u.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(u.size), out.ctypes.data_as(ctypes.c_void_p))
+    host.kv_encode_near(u.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(u.size), fmt,
+                        out.ctypes.data_as(ctypes.c_void_p))
     with np.errstate(invalid="ignore"):
-        assert np.array_equal(out, orc.encode_bp16(u.view(np.float32)).astype(np.uint32))
+        x = u.view(np.float32)
+        ref = orc.quantize_bp8(x) if fmt == 8 else orc.encode_bp16(x)
+    ref = ref[0] if isinstance(ref, tuple) else ref
+    assert np.array_equal(out, ref.astype(np.uint32))
 
 
 def test_floor_log2(host):
