@@ -12,12 +12,13 @@ struct EvictParams {
   int32_t *keep;             // optional [layers, batch, kv_heads, budget]
 };
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;   // of the streaming form
 constexpr int kQueue = 2 * kThreads;   // places given up that wait for a mover
+constexpr uint32_t kTop = 0xFF800000u; // order_key of +inf
 
 // Weights as unsigned integers of the same order: NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float w, bool guarded) {
-  if (guarded) return 0xFF800000u;                     // +inf
+  if (guarded) return kTop;
   if (w != w) return 0u;
   const uint32_t u = __float_as_uint(w + 0.0f);        // -0 + 0 = +0
   return (u >> 31) ? ~u : u | 0x80000000u;
@@ -45,15 +46,250 @@ __device__ __forceinline__ int block_rank(bool flag, Scan &s, int *total) {
   return before + __popc(mask & ((1u << lane) - 1u));
 }
 
-// One block per (layer, sequence, kv head).  A radix select over the ordered
-// weights (8 bits a pass) finds the budget-th largest; entries above it are
-// kept, and of those equal to it the first ones.  Then two scans run towards
-// each other's ends: the front scan (places < budget) queues the places given
-// up, the back scan (places >= budget) moves its kept entries into them, both
-// in order, so that a chunk's moves never write a place that is still to be
-// read: a place is queued only after it was scanned, and movers are read from
-// behind the budget, which nothing writes.
-__global__ void __launch_bounds__(kThreads) k_kv_evict(EvictParams p) {
+// Copies entry src's rows of codes, exponents, position and score to entry dst,
+// 16 bytes a thread and four entries at a time, for `moves` pairs of a row.
+template <int NT, typename Index>
+__device__ __forceinline__ void move_entries(const EvictParams &p, int64_t r, int b, int hk, int64_t layer_rows,
+                                             const Index *src, const Index *dst, int moves) {
+  const KvView &c = p.c;
+  const int tid = threadIdx.x, vecs = c.dim * (c.fmt / 8) / 16, per = 2 * vecs;
+  const int first = tid / per, piece = tid - first * per, step = NT / per;
+  const bool value = piece >= vecs;
+  const int x = value ? piece - vecs : piece;
+  uint4 *pool = reinterpret_cast<uint4 *>(value ? c.v : c.k) + x;
+  int8_t *exps = value ? c.v_exp : c.k_exp;
+  int32_t *pos = c.positions + r * c.cap;
+  float *scores = c.scores ? c.scores + r * c.cap : nullptr;
+  int32_t *keep = p.keep ? p.keep + r * p.budget : nullptr;
+  if (first < step)
+    for (int e = first; e < moves; e += 4 * step) {
+      uint4 code[4];
+      int8_t ex[4];
+      int64_t to[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        to[j] = -1;
+        const int k = e + j * step;
+        if (k >= moves) continue;
+        const int pf = c.page_of(b, src[k]), pt = c.page_of(b, dst[k]);
+        if (pf < 0 || pt < 0) continue;
+        const int64_t from = layer_rows + c.row(pf, hk, src[k]);
+        to[j] = layer_rows + c.row(pt, hk, dst[k]);
+        code[j] = pool[from * vecs];
+        if (x == 0 && exps) ex[j] = exps[from];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (to[j] >= 0) {
+          pool[to[j] * vecs] = code[j];
+          if (x == 0 && exps) exps[to[j]] = ex[j];
+        }
+    }
+  for (int k = tid; k < moves; k += NT) {
+    const int s = src[k], d = dst[k];
+    pos[d] = pos[s];
+    if (scores) scores[d] = scores[s];
+    if (keep) keep[d] = s;
+  }
+}
+
+// One block per (layer, sequence, kv head) with all its weights in registers,
+// thread t holding entries t, t + NT, ...  What bounds it is latency: the loads
+// of lengths, weights and positions, then block barriers, then the moves; so
+// the passes are few and work on registers.
+//  * The budget-th largest weight: a histogram of 2048 bins over the range that
+//    the weights have (+inf apart), then over the bin that holds it, until the
+//    bin is one value or all of it is kept -- two or three passes.
+//  * Kept entries behind the budget go, in order, to the places in front that
+//    were given up: every (chunk of NT entries, warp) counts both kinds by
+//    ballot, one scan of the counts gives everyone's rank.
+template <int NT, int KPT>
+__global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
+  constexpr int NW = NT / 32, BINS = 2048, PER = BINS / NT, E = NW * KPT;
+  const KvView &c = p.c;
+  const int r = blockIdx.x;
+  const int hk = r % c.kv_heads, lb = r / c.kv_heads, b = lb % c.batch, layer = lb / c.batch;
+  const int n = c.length(b), M = p.budget, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int32_t *keep = p.keep ? p.keep + (int64_t)r * M : nullptr;
+  if (n <= M) {
+    if (keep)
+      for (int i = tid; i < M; i += NT) keep[i] = i < n ? i : -1;
+    return;
+  }
+  __shared__ int hist[BINS], count[E + 1], warp_sum[32];
+  __shared__ uint32_t red[3][32], found[3];
+  __shared__ uint16_t src[NT * KPT / 2], dst[NT * KPT / 2];
+  const float *w = p.weights + (int64_t)r * c.cap;
+  const int32_t *pos = c.positions + (int64_t)r * c.cap;
+
+  uint32_t key[KPT];
+  {
+    float wv[KPT];
+    int ps[KPT], newest = INT_MIN;
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) {
+      const int i = j * NT + tid;
+      wv[j] = i < n ? w[i] : 0.0f;
+      ps[j] = i < n ? pos[i] : INT_MIN;
+    }
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) newest = max(newest, ps[j]);
+    newest = __reduce_max_sync(~0u, newest);
+    if (lane == 0) warp_sum[warp] = newest;
+    __syncthreads();
+    newest = __reduce_max_sync(~0u, lane < NW ? warp_sum[lane] : INT_MIN);
+    const long long guard = (long long)newest - p.recent;
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) key[j] = order_key(wv[j], ps[j] < p.sinks || ps[j] > guard);
+  }
+  auto in = [&](int j) { return j * NT + tid < n; };
+
+  // ---- thr, with the entries kept: key > thr, and `need` of those with key == thr (all of them if !ties) ----
+  uint32_t thr = kTop, lo = ~0u, hi = 0;
+  int need = M, top = 0;
+#pragma unroll
+  for (int j = 0; j < KPT; ++j)
+    if (in(j)) {
+      if (key[j] == kTop) ++top;
+      else {
+        lo = min(lo, key[j]);
+        hi = max(hi, key[j]);
+      }
+    }
+  top = __reduce_add_sync(~0u, top);
+  lo = __reduce_min_sync(~0u, lo);
+  hi = __reduce_max_sync(~0u, hi);
+  if (lane == 0) {
+    red[0][warp] = top;
+    red[1][warp] = lo;
+    red[2][warp] = hi;
+  }
+  __syncthreads();
+  top = __reduce_add_sync(~0u, lane < NW ? red[0][lane] : 0u);
+  lo = __reduce_min_sync(~0u, lane < NW ? red[1][lane] : ~0u);
+  hi = __reduce_max_sync(~0u, lane < NW ? red[2][lane] : 0u);
+  bool ties = top > M;
+  if (top < M) {
+    need = M - top;
+    while (true) {
+      const int shift = max(0, 32 - __clz(hi - lo) - 11);
+      for (int i = tid; i < BINS; i += NT) hist[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < KPT; ++j)
+        if (in(j) && key[j] >= lo && key[j] <= hi) atomicAdd(&hist[(key[j] - lo) >> shift], 1);
+      __syncthreads();
+      // counts from the top bin down; the thread that passes `need` names the bin
+      int bin[PER], mine = 0;
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        bin[q] = hist[BINS - 1 - (tid * PER + q)];
+        mine += bin[q];
+      }
+      int incl = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(~0u, incl, d);
+        if (lane >= d) incl += y;
+      }
+      if (lane == 31) warp_sum[warp] = incl;
+      __syncthreads();
+      int above = incl - mine + __reduce_add_sync(~0u, lane < warp ? warp_sum[lane] : 0);
+      if (above < need && above + mine >= need) {
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+          if (above < need && above + bin[q] >= need) {
+            found[0] = BINS - 1 - (tid * PER + q);
+            found[1] = above;
+            found[2] = bin[q];
+            break;
+          }
+          above += bin[q];
+        }
+      }
+      __syncthreads();
+      need -= (int)found[1];
+      const int held = (int)found[2];
+      const uint32_t width = (1u << shift) - 1u;
+      lo += found[0] << shift;
+      hi = hi - lo < width ? hi : lo + width;
+      if (shift == 0 || held == need) {
+        thr = lo;
+        ties = held > need;
+        break;
+      }
+    }
+  }
+  // exclusive ranks of flagged entries in entry order, from the counts per (chunk, warp) in `count`; returns the total
+  auto scan_counts = [&]() {
+    __syncthreads();
+    const int mine = tid < E ? count[tid] : 0;
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(~0u, incl, d);
+      if (lane >= d) incl += y;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    const int base = __reduce_add_sync(~0u, lane < warp ? warp_sum[lane] : 0);
+    if (tid < E) count[tid] = base + incl - mine;
+    if (tid == NT - 1) count[E] = base + incl;
+    __syncthreads();
+  };
+  static_assert(E <= NT, "a count per thread");
+  uint32_t kept = 0;
+#pragma unroll
+  for (int j = 0; j < KPT; ++j)
+    if (in(j) && (ties ? key[j] > thr : key[j] >= thr)) kept |= 1u << j;
+  const uint32_t below = (1u << lane) - 1u;
+  if (ties) {                // the first `need` of the entries at the threshold
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) {
+      const uint32_t m = __ballot_sync(~0u, in(j) && key[j] == thr);
+      if (lane == 0) count[j * NW + warp] = __popc(m);
+    }
+    scan_counts();
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) {
+      const bool tie = in(j) && key[j] == thr;
+      const uint32_t m = __ballot_sync(~0u, tie);
+      if (tie && count[j * NW + warp] + __popc(m & below) < need) kept |= 1u << j;
+    }
+    __syncthreads();
+  }
+  // holes in the low half of a count, movers in the high half: fewer than 2^15 of each
+#pragma unroll
+  for (int j = 0; j < KPT; ++j) {
+    const int i = j * NT + tid;
+    const bool k = kept >> j & 1;
+    const uint32_t holes = __ballot_sync(~0u, i < M && !k), movers = __ballot_sync(~0u, i >= M && k);
+    if (lane == 0) count[j * NW + warp] = __popc(holes) | __popc(movers) << 16;
+  }
+  scan_counts();
+#pragma unroll
+  for (int j = 0; j < KPT; ++j) {
+    const int i = j * NT + tid;
+    const bool k = kept >> j & 1;
+    const uint32_t holes = __ballot_sync(~0u, i < M && !k), movers = __ballot_sync(~0u, i >= M && k);
+    const int at = count[j * NW + warp];
+    if (i < M && !k) dst[(at & 0xFFFF) + __popc(holes & below)] = (uint16_t)i;
+    if (i >= M && k) src[(at >> 16) + __popc(movers & below)] = (uint16_t)i;
+    if (i < M && k && keep) keep[i] = i;
+  }
+  __syncthreads();
+  move_entries<NT>(p, r, b, hk, layer * c.layer_rows, src, dst, count[E] >> 16);
+}
+
+// The same for rows that do not fit a block's registers: the weights are read
+// once per pass.  A radix select over the ordered weights (8 bits a pass) finds
+// the budget-th largest.  Then two scans run towards each other's ends: the front
+// scan (places < budget) queues the places given up, the back scan (places >=
+// budget) moves its kept entries into them, both in order, so that a chunk's
+// moves never write a place that is still to be read: a place is queued only
+// after it was scanned, and movers are read from behind the budget, which nothing
+// writes.
+__global__ void __launch_bounds__(kThreads) k_kv_evict_long(EvictParams p) {
   const KvView &c = p.c;
   const int64_t r = blockIdx.x;
   const int hk = (int)(r % c.kv_heads), b = (int)(r / c.kv_heads % c.batch);
@@ -70,8 +306,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_evict(EvictParams p) {
   __shared__ int32_t queue[kQueue], src[kThreads], dst[kThreads];
   __shared__ int newest_w[kWarps];
   const float *w = p.weights + r * c.cap;
-  int32_t *pos = c.positions + r * c.cap;
-  float *scores = c.scores ? c.scores + r * c.cap : nullptr;
+  const int32_t *pos = c.positions + r * c.cap;
 
   int newest = INT_MIN;
   for (int i = tid; i < n; i += kThreads) newest = max(newest, pos[i]);
@@ -111,7 +346,6 @@ __global__ void __launch_bounds__(kThreads) k_kv_evict(EvictParams p) {
   __syncthreads();
 
   int fp = 0, bp = M, ties_f = 0, ties_b = s_front, head = 0, held = 0;
-  const int nb = c.fmt / 8, vecs = c.dim * nb / 16;      // 16-byte pieces of one row
   while (bp < n) {
     int total;
     if (held <= kQueue - kThreads && fp < M) {
@@ -147,25 +381,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_evict(EvictParams p) {
     head += total;
     held -= total;
     bp += kThreads;
-    const int64_t layer_rows = layer * c.layer_rows;
-    for (int j = tid; j < total * 2 * vecs; j += kThreads) {
-      const int e = j / (2 * vecs), piece = j % (2 * vecs);
-      const int pf = c.page_of(b, src[e]), pt = c.page_of(b, dst[e]);
-      if (pf < 0 || pt < 0) continue;
-      const int64_t from = layer_rows + c.row(pf, hk, src[e]), to = layer_rows + c.row(pt, hk, dst[e]);
-      uint8_t *pool = piece < vecs ? c.k : c.v;
-      const int x = piece < vecs ? piece : piece - vecs;
-      reinterpret_cast<uint4 *>(pool)[to * vecs + x] = reinterpret_cast<const uint4 *>(pool)[from * vecs + x];
-      if (x == 0 && c.k_exp) {
-        int8_t *ex = piece < vecs ? c.k_exp : c.v_exp;
-        ex[to] = ex[from];
-      }
-    }
-    if (tid < total) {
-      pos[dst[tid]] = pos[src[tid]];
-      if (scores) scores[dst[tid]] = scores[src[tid]];
-      if (keep) keep[dst[tid]] = src[tid];
-    }
+    move_entries<kThreads>(p, r, b, hk, layer * c.layer_rows, src, dst, total);
     __syncthreads();
   }
   // front places behind the last one scanned: the back scan found no more movers, all are kept
@@ -196,6 +412,14 @@ extern "C" int bp_kv_evict(const bp_kv_cache *cache, const float *weights, int b
   if (rc != kOk) return rc;
   p.weights = weights ? weights : cache->scores;
   p.budget = budget; p.recent = recent; p.sinks = sinks; p.keep = keep;
-  k_kv_evict<<<(unsigned)rows, kThreads, 0, (cudaStream_t)stream>>>(p);
+  cudaStream_t s = (cudaStream_t)stream;
+  const unsigned grid = (unsigned)rows;
+  // the smallest block that holds a row's weights in registers, 4 a thread while that is enough threads; longer rows
+  // stream them
+  if (p.c.cap <= 256 * 4) k_kv_evict_row<256, 4><<<grid, 256, 0, s>>>(p);
+  else if (p.c.cap <= 512 * 4) k_kv_evict_row<512, 4><<<grid, 512, 0, s>>>(p);
+  else if (p.c.cap <= 512 * 16) k_kv_evict_row<512, 16><<<grid, 512, 0, s>>>(p);
+  else if (p.c.cap <= 1024 * 16) k_kv_evict_row<1024, 16><<<grid, 1024, 0, s>>>(p);
+  else k_kv_evict_long<<<grid, kThreads, 0, s>>>(p);
   return check_launch("k_kv_evict");
 }
