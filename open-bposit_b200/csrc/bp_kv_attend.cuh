@@ -18,10 +18,13 @@
 //    pieces of the rows in shared memory, decoded in registers without a
 //    transpose; and S^T's accumulators are P's A fragment as they are.
 //  * Codes are exact in tf32: bp8 values have at most 4 significant bits, bp16
-//    values at most 11.  bp8 goes through a table of fp32 values with a copy of
-//    every entry for each lane (64 KB: bank = lane, so no conflicts, and one byte
-//    permute makes the address); bp16 codes are decoded arithmetically
-//    (decode16).
+//    values at most 11.  Both go through a table with a copy of every entry for
+//    each lane (bank = lane, so no conflicts, and one byte permute makes the
+//    address): for bp8 the fp32 value of the code, for bp16 the value of the
+//    upper byte's first code and the step to the next one, so that a permute, a
+//    look-up, a permute, a sign extension and a multiply-add decode a code (11
+//    instructions without the table: decode16, which the rare codes take that
+//    are not linear in the lower byte).
 //  * The rows of the A operand are 8 query heads twice: the upper 11 bits of q
 //    (or of the softmax weight), and what is left of it, 11 bits more.  The two
 //    sums are added in fp32, so products keep fp32 accuracy.  Each tile's sum
@@ -41,6 +44,8 @@
 // over the CTA's warps in shared memory, then over CTAs by k_kv_join.
 #pragma once
 #include <math.h>
+
+#include <type_traits>
 
 #include "bp_kv.cuh"
 
@@ -87,24 +92,25 @@ struct AttendCfg {
   static constexpr int TILEB = TT * ROWB;
   // 2^exponent of a tile's keys and values as fp32, [t][n][2] in the order that thread t of a quad needs them, with
   // a row stride that keeps the four rows in different banks
-  static constexpr int POWROW = TT / 4 + 4;
+  static constexpr int POWROW = TT / 4 + 8;
   static constexpr int POWB = FMT == 8 ? 2 * 4 * POWROW * 4 : 0;
-  // keys, values, their exponents, the powers, and the queries of the next row (read once, when it starts)
+  // keys, values, their exponents, the powers, and the queries of the next row (read once, when it starts; the widest
+  // rows have no room for them and read them then)
+  static constexpr bool QSTAGE = !(FMT == 16 && D == 128 && sizeof(T) == 4);
   static constexpr int QAT = 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;
   static constexpr int QROW = D * (int)sizeof(T) + 16;           // padded: the 8 heads' pieces in different banks
-  static constexpr int STAGE = QAT + kHeadsPerRow * QROW;
+  static constexpr int STAGE = QAT + (QSTAGE ? kHeadsPerRow * QROW : 0);
   static constexpr int REC = kHeadsPerRow * D;                   // floats of one part's output
-  // Shared memory (bp8): the decode table at shared addresses 64 K .. 128 K, so that an entry's address is the
-  // bytes {lane, code, 1, 0}; FRONT stages below it, the others above.  (bp16: no table, all stages in front.)
-  static constexpr int FRONT = FMT == 8 ? (kTableAt - kSharedReserved) / STAGE : NW;
+  // Shared memory: the decode table at shared addresses 64 K .. 128 K, so that an entry's address is the bytes {lane,
+  // code, 1, 0}; FRONT stages below it, the others above.  The table's entries fill half of its 256-byte rows; the
+  // other halves hold the units before each sequence and the lengths (kMaxBatch of each).
+  static constexpr int FRONT = (kTableAt - kSharedReserved) / STAGE;
   static constexpr int BACK = NW - (FRONT < NW ? FRONT : NW);
   // offset of what follows the table, from shared address kSharedReserved
-  static constexpr int AFTER = FMT == 8 ? 2 * kTableAt - kSharedReserved : 0;
-  // part statistics [NW][2][16], part rows [NW][2], scan [NW + 2], units before each sequence [batch + 1], lengths
-  // [batch]
-  static constexpr int META = AFTER + (FMT == 8 ? BACK : NW) * STAGE;
-  static constexpr int FIXED = META + NW * 2 * 64 + NW * 2 * 4 + (NW + 2) * 4;
-  static size_t smem(int batch) { return FIXED + (size_t)(2 * batch + 1) * 4; }
+  static constexpr int AFTER = 2 * kTableAt - kSharedReserved;
+  // part statistics [NW][2][16], part rows [NW][2], scan [NW + 2]
+  static constexpr int META = AFTER + BACK * STAGE;
+  static constexpr int SMEM = META + NW * 2 * 64 + NW * 2 * 4 + (NW + 2) * 4;
   static __device__ __forceinline__ int stage_at(int warp) {
     return warp < FRONT ? warp * STAGE : AFTER + (warp - FRONT) * STAGE;
   }
@@ -218,6 +224,28 @@ __device__ __forceinline__ uint32_t decode16(float u) {
   return v | (__float_as_uint(x) & 0x80000000u);
 }
 
+// Word i of the decode table's free halves: the units before sequence i, and
+// from kMaxBatch + 1 on the lengths.
+__device__ __forceinline__ int &spare_word(uint8_t *table, int i) {
+  return *reinterpret_cast<int *>(table + (i >> 5) * 256 + 128 + (i & 31) * 4);
+}
+
+// tf32 bits of code k of a word; `entry`: lane * 4 and the table's address.
+// bp16: the fp32 bits are linear in the code within blocks of 256 codes, but in
+// the first and last block of each sign; a code of those leaves a 1 in `odd`,
+// and the step is done again with EXACT.  (The table's low 13 bits ride along:
+// they are not part of a tf32 operand.)
+template <int FMT, bool EXACT>
+__device__ __forceinline__ uint32_t decode_code(uint32_t entry, uint32_t w, int k, uint32_t &odd) {
+  if (FMT == 8) return table_entry(__byte_perm(w, entry, 0x6504 | k << 4));
+  if (EXACT) return decode16(__uint_as_float(__byte_perm(w ^ 0x80008000u, 0x4B00u, k ? 0x5432 : 0x5410)));
+  const uint32_t e = table_entry(__byte_perm(w, entry, 0x6504 | (2 * k + 1) << 4));
+  int step;
+  asm("bfe.s32 %0, %1, 0, 13;" : "=r"(step) : "r"(e));
+  odd |= e;
+  return __byte_perm(w, 0, 0x4404 | (2 * k) << 4) * (uint32_t)step + e;
+}
+
 // A work row: 8 (or fewer) query heads of one kv head of one sequence.
 struct RowId {
   int b, hk, ch;
@@ -264,21 +292,33 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   float *const rec_ml = reinterpret_cast<float *>(smem + C::META);          // [NW][2][m 8, l 8]
   int *const rec_row = reinterpret_cast<int *>(rec_ml + NW * 32);           // [NW][2]
   int *const scan = rec_row + NW * 2;
-  int *const before = scan + NW + 2;                                        // [batch + 1]
-  int *const lens = before + p.c.batch + 1;                                 // [batch]
+  uint8_t *const table = smem + (kTableAt - kSharedReserved);
+  auto before = [=](int b) -> int & { return spare_word(table, b); };
+  auto lens = [=](int b) -> int & { return spare_word(table, kMaxBatch + 1 + b); };
+  static_assert(2 * kMaxBatch + 1 <= 256 * 32, "words in the free halves");
   const KvView &c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_seq = c.kv_heads * p.chunks;             // work rows of one sequence
   asm volatile("griddepcontrol.launch_dependents;");
 
   auto length = [&](int b) { return min(c.length(b), p.max_len); };
-  if (FMT == 8) {          // the decode table: word 64 code + lane
-    for (int i = tid; i < 256; i += NT) {
-      const uint32_t v = posit_to_f32_bits<8, 2>(i);
-      uint4 *row = reinterpret_cast<uint4 *>(smem + (kTableAt - kSharedReserved)) + i * 16;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) row[(j + i) & 7] = make_uint4(v, v, v, v);
+  // the decode table: word 64 i + lane
+  for (int i = tid; i < 256; i += NT) {
+    uint32_t v;
+    if (FMT == 8) {
+      v = posit_to_f32_bits<8, 2>(i);
+    } else {
+      // bits of code 256 i's value, and the step per code within the block (down for negative codes) over 2^8 as a
+      // signed 13-bit number; 1 for the blocks in which the steps differ
+      const bool neg = i >= 128;
+      const uint32_t m = (neg ? 256 - i : i) * 256, m1 = neg ? m - 1 : m + 1;
+      const int32_t step = (int32_t)(bp16_to_f32_bits(m1) - bp16_to_f32_bits(m)) >> 8;
+      v = i == 0 || i == 127 || i == 128 || i == 255 ? 1u
+                                                     : bp16_to_f32_bits(m) | (neg ? 0x80000000u : 0u) | (step & 0x1FFF);
     }
+    uint4 *row = reinterpret_cast<uint4 *>(table) + i * 16;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) row[(j + i) & 7] = make_uint4(v, v, v, v);
   }
   // units before each sequence
   {
@@ -288,7 +328,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       const int b = tid * each + i;
       if (b < c.batch) {
         const int n = length(b);
-        lens[b] = n;
+        lens(b) = n;
         mine += (n + 15) / 16 * per_seq;
       }
     }
@@ -306,17 +346,17 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     for (int i = 0; i < each; ++i) {
       const int b = tid * each + i;
       if (b < c.batch) {
-        before[b] = at;
-        at += (lens[b] + 15) / 16 * per_seq;
+        before(b) = at;
+        at += (lens(b) + 15) / 16 * per_seq;
       }
     }
-    if (tid == NT - 1) before[c.batch] = at;
+    if (tid == NT - 1) before(c.batch) = at;
     __syncthreads();
   }
-  const int total = before[c.batch];
+  const int total = before(c.batch);
   // empty sequences: zeros, and -inf for the logarithm
   for (int b = blockIdx.x; b < c.batch; b += gridDim.x)
-    if (before[b + 1] == before[b]) {
+    if (before(b + 1) == before(b)) {
       T *o = (T *)p.out + (int64_t)b * p.heads * D;
       for (int i = tid; i < p.heads * D; i += NT) o[i] = from_f32<T>(0.0f);
       if (p.lse)
@@ -355,8 +395,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       if (w.row == per_seq) {
         w.row = w.hk = 0;
         do ++w.b;
-        while (before[w.b + 1] == before[w.b]);
-        w.n = lens[w.b];
+        while (before(w.b + 1) == before(w.b));
+        w.n = lens(w.b);
       }
     }
     w.count = min(min(TU, units_of(w.n) - w.u), left);
@@ -370,20 +410,29 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   constexpr int PJ = CPR / 2;              // pieces per lane of 16 rows
   // piece `lane` of 16 rows; piece j * 32 + lane lies 512 j behind it, permuted alike (see below for 256-byte rows)
   const uint32_t to = swizzle<C::ROWB>(lane / CPR, lane % CPR);
-  // (looking a page up and using it are apart, so that the copies and not the look-up wait for it)
-  auto fetch = [&](const Place &w, int page, bool value, bool first) {
+  // A tile's place in the pools: the rows of its units (the look-up of the pages, this, and the copies are apart, so
+  // that none of them waits for the one before).
+  struct Rows {
+    uint32_t mine, unit[TU];               // this lane's unit's row, and all of them; kNone for a page outside the pool
+    bool plain;                            // a whole tile, all of whose pages are there
+  };
+  constexpr uint32_t kNone = ~0u;          // pools have fewer rows
+  auto rows_of = [&](const Place &w, int page, Rows &r) {
+    r.mine = (unsigned)page < (unsigned)c.pages ? (uint32_t)c.row(page, w.hk, (w.u + lane) * 16) : kNone;
+#pragma unroll
+    for (int i = 0; i < TU; ++i) r.unit[i] = __shfl_sync(~0u, r.mine, i);
+    bool all = w.n - w.u * 16 >= TT;
+#pragma unroll
+    for (int i = 0; i < TU; ++i) all = all && r.unit[i] != kNone;
+    r.plain = all;
+  };
+  auto fetch = [&](const Place &w, const Rows &r, bool value, bool first) {
     const uint8_t *pool = (value ? c.v : c.k) + lane * 16;
     const uint32_t dst = stage_s + (value ? C::TILEB : 0) + to;
-    const int valid = w.n - w.u * 16;
-    constexpr uint32_t kNone = ~0u;        // pools have fewer rows
-    const uint32_t rows = (unsigned)page < (unsigned)c.pages ? (uint32_t)c.row(page, w.hk, (w.u + lane) * 16) : kNone;
-    uint32_t row[TU];
-#pragma unroll
-    for (int i = 0; i < TU; ++i) row[i] = __shfl_sync(~0u, rows, i);
-    if (valid >= TT && __all_sync(~0u, lane >= TU || rows != kNone)) {
+    if (r.plain) {
 #pragma unroll
       for (int i = 0; i < TU; ++i) {
-        const uint8_t *src = pool + (uint64_t)row[i] * C::ROWB;
+        const uint8_t *src = pool + (uint64_t)r.unit[i] * C::ROWB;
 #pragma unroll
         for (int j = 0; j < PJ; ++j) {
           const uint32_t d = dst + i * 16 * C::ROWB + j * 512;
@@ -391,41 +440,43 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         }
       }
     } else {
+      const int valid = w.n - w.u * 16;
 #pragma unroll 1
       for (int i = 0; i < w.count; ++i) {
-        const uint32_t r = __shfl_sync(~0u, rows, i);
-        const uint8_t *src = pool + (uint64_t)r * C::ROWB;
+        const uint32_t row = __shfl_sync(~0u, r.mine, i);
+        const uint8_t *src = pool + (uint64_t)row * C::ROWB;
 #pragma unroll
         for (int j = 0; j < PJ; ++j) {
           const uint32_t d = dst + i * 16 * C::ROWB + j * 512;
-          if (r != kNone && i * 16 + (j * 32 + lane) / CPR < valid) copy16(CPR == 16 && (j & 1) ? d ^ 64 : d, src + j * 512);
+          if (row != kNone && i * 16 + (j * 32 + lane) / CPR < valid) copy16(CPR == 16 && (j & 1) ? d ^ 64 : d, src + j * 512);
         }
       }
     }
-    if (!value && (w.u == 0 || first)) {   // a new row for this warp: its queries, 4 lanes a head
+    if (C::QSTAGE && !value && (w.u == 0 || first)) {   // a new row for this warp: its queries, 4 lanes a head
       const int h = w.ch * kHeadsPerRow + g;
       const uint8_t *q = reinterpret_cast<const uint8_t *>((const T *)p.q + w.b * p.qs + (int64_t)(w.hk * p.group + h) * D);
 #pragma unroll
       for (int i = 0; i < D * (int)sizeof(T) / 64; ++i)
         if (h < p.group) copy16(stage_s + C::QAT + g * C::QROW + (i * 4 + t) * 16, q + (i * 4 + t) * 16);
     }
-    if (FMT == 8 && rows != kNone)
-      copy16(stage_s + 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + rows);
+    if (FMT == 8 && r.mine != kNone)
+      copy16(stage_s + 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + r.mine);
     copy_commit();
   };
 
   Place cur{}, nxt{};
+  Rows rows{};
   int page_c = -1, page_n = -1;
   if (wlo < whi) {
     int a = 0, z = c.batch;                // sequence of the first unit, by bisection
     while (z - a > 1) {
       const int mid = (a + z) >> 1;
-      if (before[mid] <= wlo) a = mid;
+      if (before(mid) <= wlo) a = mid;
       else z = mid;
     }
     cur.b = a;
-    cur.n = lens[a];
-    const int r = wlo - before[a], nu = units_of(cur.n);
+    cur.n = lens(a);
+    const int r = wlo - before(a), nu = units_of(cur.n);
     cur.row = r / nu;
     cur.u = r - cur.row * nu;
     cur.hk = cur.row / p.chunks;
@@ -434,15 +485,11 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     page_c = page_of(cur);
     nxt = cur;
   }
-  fetch(cur, page_c, false, true);
-  fetch(cur, page_c, true, false);
+  rows_of(cur, page_c, rows);
+  fetch(cur, rows, false, true);
+  fetch(cur, rows, true, false);
   __syncthreads();
   const uint32_t entry = lane * 4 | (kTableAt >> 16) << 8;
-  // fp32 bits of code k of a word
-  auto decode = [&](uint32_t w, int k) {
-    if (FMT == 8) return table_entry(__byte_perm(w, entry, 0x6504 | k << 4));
-    return decode16(__uint_as_float(__byte_perm(w ^ 0x80008000u, 0x4B00u, k ? 0x5432 : 0x5410)));
-  };
   constexpr int CW = 4 / C::BYTES;      // codes per word
 
   // The thread's place in the fragments: head g of A and of the accumulators; column g of S is entry `er` of its 8
@@ -458,7 +505,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
 
   // The three stages of a step over U units, from unit i0 of the stage on.
   // S[head, entry] = q K^T
-  auto scores = [&](auto &s, int i0) {
+  auto scores_with = [&](auto exact, auto &s, int i0) {
+    uint32_t odd = 0;
     constexpr int SN = sizeof(s) / sizeof(s[0]);
     // four columns at a time: an MMA waits for the one before it in its sum
     constexpr int G = SN < 4 ? SN : 4;
@@ -473,7 +521,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         const uint32_t a[4] = {qf[w][0], F32 ? qf[w][1] : 0u, qf[w][F32 ? 2 : 1], F32 ? qf[w][F32 ? 3 : 0] : 0u};
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          const uint32_t b0 = decode(kw[k][2 * w / CW], 2 * w % CW), b1 = decode(kw[k][2 * w / CW], 2 * w % CW + 1);
+          const uint32_t b0 = decode_code<FMT, decltype(exact)::value>(entry, kw[k][2 * w / CW], 2 * w % CW, odd);
+          const uint32_t b1 = decode_code<FMT, decltype(exact)::value>(entry, kw[k][2 * w / CW], 2 * w % CW + 1, odd);
           if (w == 0) mma_tf32_first(c4[k], a, b0, b1);
           else mma_tf32(c4[k], a, b0, b1);
         }
@@ -484,6 +533,11 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         s[i + k][1] = F32 ? c4[k][1] + c4[k][3] : c4[k][1];
       }
     }
+    return odd;
+  };
+  auto scores = [&](auto &s, int i0) {
+    const uint32_t odd = scores_with(std::false_type{}, s, i0);
+    if (FMT == 16 && __any_sync(~0u, odd & 1u)) scores_with(std::true_type{}, s, i0);
   };
   // S becomes e^(S - maximum), maximum and sum move on; returns the factor for what was summed before
   auto weights = [&](auto &s, int i0, int valid) {
@@ -533,9 +587,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     return alpha;
   };
   // O[head, d] = alpha O + P V
-  auto values = [&](const auto &s, int i0, float alpha) {
+  auto values_with = [&](auto exact, const auto &s, int i0, auto &acc) {
+    uint32_t odd = 0;
     constexpr int SN = sizeof(s) / sizeof(s[0]);
-    float acc[DN][4];
 #pragma unroll
     for (int i = 0; i < SN; ++i) {
       float w0 = s[i][0], w1 = s[i][1];
@@ -552,11 +606,17 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       load_words<C::ROWB>(r, e1, g * VW, v1);
 #pragma unroll
       for (int d = 0; d < DN; ++d) {
-        const uint32_t b0 = decode(v0[d / CW], d % CW), b1 = decode(v1[d / CW], d % CW);
+        const uint32_t b0 = decode_code<FMT, decltype(exact)::value>(entry, v0[d / CW], d % CW, odd), b1 = decode_code<FMT, decltype(exact)::value>(entry, v1[d / CW], d % CW, odd);
         if (i == 0) mma_tf32_first(acc[d], a, b0, b1);
         else mma_tf32(acc[d], a, b0, b1);
       }
     }
+    return odd;
+  };
+  auto values = [&](const auto &s, int i0, float alpha) {
+    float acc[DN][4];
+    const uint32_t odd = values_with(std::false_type{}, s, i0, acc);
+    if (FMT == 16 && __any_sync(~0u, odd & 1u)) values_with(std::true_type{}, s, i0, acc);
 #pragma unroll
     for (int d = 0; d < DN; ++d) {
       o[d][0] = fmaf(o[d][0], alpha, acc[d][0] + acc[d][2]);
@@ -586,7 +646,11 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
     copy_wait_but_one();
     if (x == wlo || cur.u == 0) {          // a new row: its queries, and an empty state
-      const uint4 *q = reinterpret_cast<const uint4 *>(stage + C::QAT + g * C::QROW + t * (D / 4) * (int)sizeof(T));
+      const int at = t * (D / 4) * (int)sizeof(T);
+      const uint4 *q = reinterpret_cast<const uint4 *>(
+          C::QSTAGE ? stage + C::QAT + g * C::QROW + at
+                    : reinterpret_cast<const uint8_t *>((const T *)p.q + cur.b * p.qs +
+                                                        (int64_t)(cur.hk * p.group + cur.ch * kHeadsPerRow + g) * D) + at);
       constexpr int QV = D / 4 * sizeof(T) / 16;
       const bool real = cur.ch * kHeadsPerRow + g < p.group;
       uint4 raw[QV];
@@ -617,16 +681,17 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     if (cur.count == TU && valid >= TT) {
       float s[TT / 8][2];
       scores(s, 0);
+      if (more) rows_of(nxt, page_n, rows);
       powers(ske, kpow, p.scale);
       __syncwarp();
-      if (more) fetch(nxt, page_n, false, false);
+      if (more) fetch(nxt, rows, false, false);
       else copy_commit();
       const float alpha = weights(s, 0, TT);
       copy_wait_but_one();
       powers(sve, vpow, 1.0f);
       values(s, 0, alpha);
       __syncwarp();
-      if (more) fetch(nxt, page_n, true, false);
+      if (more) fetch(nxt, rows, true, false);
       else copy_commit();
     } else {
       copy_commit();
@@ -641,8 +706,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       }
       __syncwarp();
       if (more) {
-        fetch(nxt, page_n, false, false);
-        fetch(nxt, page_n, true, false);
+        rows_of(nxt, page_n, rows);
+        fetch(nxt, rows, false, false);
+        fetch(nxt, rows, true, false);
       }
     }
 
@@ -705,8 +771,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     const uint32_t parts = __ballot_sync(~0u, in);
     left &= ~parts;
     const RowId id = row_id(p, row);
-    const int nu = units_of(lens[id.b]);
-    const int x0 = before[id.b] + (row - id.b * per_seq) * nu, x1 = x0 + nu;
+    const int nu = units_of(lens(id.b));
+    const int x0 = before(id.b) + (row - id.b * per_seq) * nu, x1 = x0 + nu;
     // (the CTA that holds the row's last unit is the last one with a part)
     if (x0 >= lo && x1 > hi) open = make_int2(row, deal.part_of(x1 - 1) - cta + 1);
     if (h >= kHeadsPerRow) continue;
@@ -765,17 +831,15 @@ int launch_kv_attend16(const AttendParams &p, int dtype, int grid, cudaStream_t 
 template <int FMT, int D, typename T>
 int launch_kv_attend_one(const AttendParams &p, int grid, cudaStream_t s) {
   using C = AttendCfg<FMT, D, T>;
-  const size_t bytes = C::smem(p.c.batch);
-  int device = 0;
+  static_assert(C::SMEM <= 232448, "shared memory per CTA");
+  int device = 0, reserved = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return set_error(kENoDev, "k_kv_attend: no device");
-  static_assert(C::FIXED + 4 * (2 * kMaxBatch + 1) <= 232448, "shared memory per CTA");
-  int reserved = 0;
-  if (FMT == 8 && (cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, device) != cudaSuccess ||
-                   reserved != kSharedReserved))
+  if (cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, device) != cudaSuccess ||
+      reserved != kSharedReserved)
     return set_error(kENoDev, "k_kv_attend: shared memory starts at %d, not %d", reserved, kSharedReserved);
-  cudaError_t e = cudaFuncSetAttribute(k_kv_attend<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  cudaError_t e = cudaFuncSetAttribute(k_kv_attend<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return set_error(kECuda, "k_kv_attend: %s", cudaGetErrorString(e));
-  k_kv_attend<FMT, D, T><<<grid, C::NW * 32, bytes, s>>>(p);
+  k_kv_attend<FMT, D, T><<<grid, C::NW * 32, C::SMEM, s>>>(p);
   return check_launch("k_kv_attend");
 }
 template <int FMT, typename T>
