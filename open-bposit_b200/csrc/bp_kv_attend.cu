@@ -10,76 +10,56 @@ namespace bp {
 namespace {
 
 constexpr int kJoinParts = 256;     // CTAs of one launch, at most
-constexpr int kJoinWarps = 4;       // warps per head
+constexpr int kJoinBatch = 16;      // parts whose outputs are loaded at once
 
 // Joins the parts of a row that several CTAs of k_kv_attend worked on: block c
-// takes the row that starts in CTA c's range and goes on behind it, four warps a
-// head.  Each of a head's warps works out all parts' statistics by itself (a lane
-// takes every 32nd) and sums every fourth part's output, so that three rounds of
-// loads (the row, the statistics, the outputs) are all that is waited for.
-// Launched early (programmatic dependent launch), its start hides behind the
-// main kernel.
+// takes the row that starts in CTA c's range and goes on behind it, a warp for
+// each head.  A lane takes every 32nd part's statistics, then D / 32 columns of
+// the output, the loads of 16 parts in flight together.  Launched early
+// (programmatic dependent launch), its start hides behind the main kernel.
 template <typename T>
-__global__ void __launch_bounds__(kHeadsPerRow *kJoinWarps * 32) k_kv_join(AttendParams p) {
-  __shared__ float sums[kHeadsPerRow * kJoinWarps][128];
+__global__ void __launch_bounds__(kHeadsPerRow * 32) k_kv_join(AttendParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 open = p.cta_row[blockIdx.x];
   if (open.x < 0) return;
-  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = warp / kJoinWarps, sub = warp % kJoinWarps;
+  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y, h = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t head = head_of(p, row_id(p, open.x), h);
   // the first part is the CTA's second record (a row that starts there), the others are first records
-  const float *base = p.cta_rec + (int64_t)blockIdx.x * 2 * (rec + 16);
-  const int64_t step = 2 * (rec + 16);
-  auto part = [&](int k) { return k ? base + k * step : base + rec + 16; };
-  float m[kJoinParts / 32], l[kJoinParts / 32], M = -INFINITY, L = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kJoinParts / 32; ++i) {
-    const int k = i * 32 + lane;
-    m[i] = k < parts ? part(k)[rec + h] : -INFINITY;
-    l[i] = k < parts ? part(k)[rec + 8 + h] : 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < kJoinParts / 32; ++i) M = fmaxf(M, m[i]);
+  const float *base = p.cta_rec + blockIdx.x * 2 * (rec + 16);
+  auto part = [&](int k) { return base + (k ? k * 2 : 1) * (rec + 16); };
+  float M = -INFINITY, L = 0.0f;
+  for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[rec + h]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
-#pragma unroll
-  for (int i = 0; i < kJoinParts / 32; ++i) {
-    m[i] = i * 32 + lane < parts ? ex2(m[i] - M) : 0.0f;       // the part's weight from here on
-    L = fmaf(l[i], m[i], L);
-  }
+  for (int k = lane; k < parts; k += 32) L = fmaf(part(k)[rec + 8 + h], ex2(part(k)[rec + h] - M), L);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
   float O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int k = 0; k < parts; k += kJoinBatch) {
+    // (past the last part: the last one again, with weight 0)
+    const int mine = k + (lane & (kJoinBatch - 1));
+    const float a = ex2(part(min(mine, parts - 1))[rec + h] - M);
+    float x[kJoinBatch][4];
 #pragma unroll
-  for (int i = 0; i < kJoinParts / 32; ++i) {
-    if (i * 32 >= parts) break;
-    float x[32 / kJoinWarps][4];       // (parts past the last have weight 0, and read the last)
-#pragma unroll
-    for (int j = 0; j < 32 / kJoinWarps; ++j) {
-      const float *r = part(min(i * 32 + j * kJoinWarps + sub, parts - 1)) + h * D + lane;
+    for (int j = 0; j < kJoinBatch; ++j) {
+      const float *r = part(min(k + j, parts - 1)) + h * D + lane;
 #pragma unroll
       for (int y = 0; y < 4; ++y) x[j][y] = y * 32 < D ? r[y * 32] : 0.0f;
     }
 #pragma unroll
-    for (int j = 0; j < 32 / kJoinWarps; ++j) {
-      const float a = __shfl_sync(~0u, m[i], j * kJoinWarps + sub);
+    for (int j = 0; j < kJoinBatch; ++j) {
+      const float f = k + j < parts ? __shfl_sync(~0u, a, j) : 0.0f;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) O[y] = fmaf(x[j][y], a, O[y]);
+      for (int y = 0; y < 4; ++y) O[y] = k + j < parts ? fmaf(x[j][y], f, O[y]) : O[y];
     }
   }
+  if (lane == 0) write_lse(p, open.x, h, head, M + log2f(L));
+  if (head < 0) return;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) sums[warp][x * 32 + lane] = O[x];
-  __syncthreads();
-  if (sub == 0 && head >= 0)
-    for (int d = lane; d < D; d += 32) {
-      float o = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) o += sums[warp + w][d];
-      ((T *)p.out)[head * D + d] = from_f32<T>(o / L);
-    }
-  if (sub == 0 && lane == 0) write_lse(p, open.x, h, head, M + log2f(L));
+  for (int y = 0; y < 4; ++y)
+    if (y * 32 < D) ((T *)p.out)[head * D + y * 32 + lane] = from_f32<T>(O[y] / L);
 }
 
 // scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2):
@@ -106,10 +86,10 @@ __global__ void __launch_bounds__(256) k_kv_scores(AttendParams p) {
 }
 
 template <typename K>
-int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t s, const char *what, int threads = 256) {
+int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t s, const char *what) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -220,9 +200,9 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   // (a batch of at most kMinUnits units is one CTA's, and no row of it is in parts)
   const int64_t units = (int64_t)cache->batch * cache->kv_heads * p.chunks * ((p.max_len + 15) / 16);
   if (rc == kOk && units > kMinUnits) {
-    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid), p, s, "k_kv_join", kHeadsPerRow * kJoinWarps * 32);
-    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid), p, s, "k_kv_join", kHeadsPerRow * kJoinWarps * 32);
-    else rc = launch_after(k_kv_join<__half>, dim3(grid), p, s, "k_kv_join", kHeadsPerRow * kJoinWarps * 32);
+    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid), p, s, "k_kv_join");
+    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid), p, s, "k_kv_join");
+    else rc = launch_after(k_kv_join<__half>, dim3(grid), p, s, "k_kv_join");
   }
   if (rc == kOk && accumulate && p.max_len)
     rc = launch_after(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), p, s, "k_kv_scores");

@@ -84,7 +84,10 @@ template <int FMT, int D, typename T>
 struct AttendCfg {
   static constexpr int BYTES = FMT / 8;
   static constexpr int ROWB = D * BYTES;
-  static constexpr int TT = FMT == 8 ? (D <= 64 ? 64 : 32) : (D <= 32 ? 64 : 32);   // entries per tile
+  // Entries per tile, and tiles in the stage: two of one unit for wide bp16 rows, whose unrolled steps would not fit
+  // the instruction cache with more (32 entries at D = 128: 84 us, a quarter of it waiting for instructions).
+  static constexpr int TT = FMT == 8 ? (D <= 64 ? 64 : 32) : (D <= 32 ? 64 : (D <= 64 ? 32 : 16));
+  static constexpr int NB = TT == 16 ? 2 : 1;
 #ifndef KV_NW
 #define KV_NW 12
 #endif
@@ -94,10 +97,10 @@ struct AttendCfg {
   // a row stride that keeps the four rows in different banks
   static constexpr int POWROW = TT / 4 + 8;
   static constexpr int POWB = FMT == 8 ? 2 * 4 * POWROW * 4 : 0;
-  // keys, values, their exponents, the powers, and the queries of the next row (read once, when it starts; the widest
-  // rows have no room for them and read them then)
-  static constexpr bool QSTAGE = !(FMT == 16 && D == 128 && sizeof(T) == 4);
-  static constexpr int QAT = 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;
+  // keys, values, their exponents, the powers, and the queries of the next row (one row's: with two tiles under way
+  // they are read from memory when a row starts)
+  static constexpr bool QSTAGE = NB == 1;
+  static constexpr int QAT = NB * 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;
   static constexpr int QROW = D * (int)sizeof(T) + 16;           // padded: the 8 heads' pieces in different banks
   static constexpr int STAGE = QAT + (QSTAGE ? kHeadsPerRow * QROW : 0);
   static constexpr int REC = kHeadsPerRow * D;                   // floats of one part's output
@@ -115,7 +118,7 @@ struct AttendCfg {
     return warp < FRONT ? warp * STAGE : AFTER + (warp - FRONT) * STAGE;
   }
   static_assert(REC * 4 <= STAGE, "a part's output fits the stage");
-  static_assert(TT % 32 == 0, "a lane converts TT / 32 exponents");
+  static_assert(FMT == 16 || (TT % 32 == 0 && NB == 1), "a lane converts TT / 32 exponents, of one tile");
   static_assert(STAGE % 16 == 0, "stages stay 16-byte aligned");
 };
 
@@ -128,9 +131,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All groups but the last one are complete, for the whole warp.
-__device__ __forceinline__ void copy_wait_but_one() {
-  asm volatile("cp.async.wait_group 1;" ::: "memory");
+// All groups but the last N are complete, for the whole warp.
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
   __syncwarp();
 }
 
@@ -283,7 +287,7 @@ template <int FMT, int D, typename T>
 __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(AttendParams p) {
   using C = AttendCfg<FMT, D, T>;
   constexpr int TT = C::TT, NW = C::NW, NT = NW * 32;
-  constexpr int TU = TT / 16;           // units per tile
+  constexpr int TU = TT / 16, NB = C::NB;
   constexpr int DN = D / 8;             // 8-wide columns of O, and MMA steps along D
   constexpr int KW = C::ROWB / 16;      // words of a key row that one thread holds
   constexpr int VW = C::ROWB / 32;      // words of a value row that one thread holds
@@ -374,9 +378,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   const int wlo = lo + share.begin(warp), whi = lo + share.begin(warp + 1);
 
   uint8_t *const stage = smem + C::stage_at(warp);
-  uint8_t *const sk = stage, *const sv = stage + C::TILEB;
-  int8_t *const ske = reinterpret_cast<int8_t *>(stage + 2 * C::TILEB), *const sve = ske + TT;
-  float *const kpow = reinterpret_cast<float *>(stage + 2 * C::TILEB + 2 * TT), *const vpow = kpow + 4 * C::POWROW;
+  uint8_t *const sk = stage, *const sv = stage + C::TILEB;   // (buffer i of NB: 2 TILEB i further)
+  int8_t *const ske = reinterpret_cast<int8_t *>(stage + NB * 2 * C::TILEB), *const sve = ske + TT;
+  float *const kpow = reinterpret_cast<float *>(stage + NB * 2 * C::TILEB + 2 * TT), *const vpow = kpow + 4 * C::POWROW;
   // ---- where tiles lie: units u .. u + count - 1 of a work row ----
   struct Place {
     int b, row, hk, ch, u, count, n;       // sequence, work row of it (hk * chunks + ch), units, entries of the row
@@ -426,9 +430,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     for (int i = 0; i < TU; ++i) all = all && r.unit[i] != kNone;
     r.plain = all;
   };
-  auto fetch = [&](const Place &w, const Rows &r, bool value, bool first) {
+  auto fetch = [&](const Place &w, const Rows &r, bool value, bool first, int buf) {
     const uint8_t *pool = (value ? c.v : c.k) + lane * 16;
-    const uint32_t dst = stage_s + (value ? C::TILEB : 0) + to;
+    const uint32_t dst = stage_s + (2 * buf + value) * C::TILEB + to;
     if (r.plain) {
 #pragma unroll
       for (int i = 0; i < TU; ++i) {
@@ -460,19 +464,22 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         if (h < p.group) copy16(stage_s + C::QAT + g * C::QROW + (i * 4 + t) * 16, q + (i * 4 + t) * 16);
     }
     if (FMT == 8 && r.mine != kNone)
-      copy16(stage_s + 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + r.mine);
+      copy16(stage_s + NB * 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + r.mine);
     copy_commit();
   };
 
-  Place cur{}, nxt{};
+  // this tile, the one behind it (NB = 2), and the next to be fetched, which starts `ax` units into the row of tiles
+  Place cur{}, mid{}, ahead{};
   Rows rows{};
-  int page_c = -1, page_n = -1;
+  int ax = wlo, page = -1;
+  uint32_t bad = 0;            // bit i: a page of tile i from here is outside the pool
+  auto is_bad = [&](const Place &w, int pg) { return __any_sync(~0u, lane < w.count && (unsigned)pg >= (unsigned)c.pages); };
   if (wlo < whi) {
     int a = 0, z = c.batch;                // sequence of the first unit, by bisection
     while (z - a > 1) {
-      const int mid = (a + z) >> 1;
-      if (before(mid) <= wlo) a = mid;
-      else z = mid;
+      const int half = (a + z) >> 1;
+      if (before(half) <= wlo) a = half;
+      else z = half;
     }
     cur.b = a;
     cur.n = lens(a);
@@ -482,12 +489,24 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     cur.hk = cur.row / p.chunks;
     cur.ch = cur.row - cur.hk * p.chunks;
     cur.count = min(min(TU, nu - cur.u), whi - wlo);
-    page_c = page_of(cur);
-    nxt = cur;
+    ahead = cur;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      if (ax < whi) {
+        page = page_of(ahead);
+        rows_of(ahead, page, rows);
+        bad |= (uint32_t)is_bad(ahead, page) << i;
+        fetch(ahead, rows, false, i == 0, i);
+        fetch(ahead, rows, true, false, i);
+        if (i == 1) mid = ahead;
+        ax += ahead.count;
+        if (ax < whi) advance(ahead, whi - ax);
+      } else {
+        copy_commit();
+        copy_commit();
+      }
+    }
   }
-  rows_of(cur, page_c, rows);
-  fetch(cur, rows, false, true);
-  fetch(cur, rows, true, false);
   __syncthreads();
   const uint32_t entry = lane * 4 | (kTableAt >> 16) << 8;
   constexpr int CW = 4 / C::BYTES;      // codes per word
@@ -505,7 +524,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
 
   // The three stages of a step over U units, from unit i0 of the stage on.
   // S[head, entry] = q K^T
-  auto scores_with = [&](auto exact, auto &s, int i0) {
+  auto scores_with = [&](auto exact, auto &s, int i0, const uint8_t *sk) {
     uint32_t odd = 0;
     constexpr int SN = sizeof(s) / sizeof(s[0]);
     // four columns at a time: an MMA waits for the one before it in its sum
@@ -535,9 +554,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
     return odd;
   };
-  auto scores = [&](auto &s, int i0) {
-    const uint32_t odd = scores_with(std::false_type{}, s, i0);
-    if (FMT == 16 && __any_sync(~0u, odd & 1u)) scores_with(std::true_type{}, s, i0);
+  auto scores = [&](auto &s, int i0, const uint8_t *sk) {
+    const uint32_t odd = scores_with(std::false_type{}, s, i0, sk);
+    if (FMT == 16 && __any_sync(~0u, odd & 1u)) scores_with(std::true_type{}, s, i0, sk);
   };
   // S becomes e^(S - maximum), maximum and sum move on; returns the factor for what was summed before
   auto weights = [&](auto &s, int i0, int valid) {
@@ -587,7 +606,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     return alpha;
   };
   // O[head, d] = alpha O + P V
-  auto values_with = [&](auto exact, const auto &s, int i0, auto &acc) {
+  auto values_with = [&](auto exact, const auto &s, int i0, auto &acc, const uint8_t *sv) {
     uint32_t odd = 0;
     constexpr int SN = sizeof(s) / sizeof(s[0]);
 #pragma unroll
@@ -613,10 +632,10 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
     return odd;
   };
-  auto values = [&](const auto &s, int i0, float alpha) {
+  auto values = [&](const auto &s, int i0, float alpha, const uint8_t *sv) {
     float acc[DN][4];
-    const uint32_t odd = values_with(std::false_type{}, s, i0, acc);
-    if (FMT == 16 && __any_sync(~0u, odd & 1u)) values_with(std::true_type{}, s, i0, acc);
+    const uint32_t odd = values_with(std::false_type{}, s, i0, acc, sv);
+    if (FMT == 16 && __any_sync(~0u, odd & 1u)) values_with(std::true_type{}, s, i0, acc, sv);
 #pragma unroll
     for (int d = 0; d < DN; ++d) {
       o[d][0] = fmaf(o[d][0], alpha, acc[d][0] + acc[d][2]);
@@ -635,16 +654,12 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
   };
 
-  for (int x = wlo; x < whi;) {
-    lost |= __any_sync(~0u, lane < cur.count && (unsigned)page_c >= (unsigned)c.pages);
-    // the next tile's pages are looked up while this one's keys are worked on
-    const int next = x + cur.count;
-    const bool more = next < whi;
-    if (more) {
-      advance(nxt, whi - next);
-      page_n = page_of(nxt);
-    }
-    copy_wait_but_one();
+  for (int x = wlo, buf = 0; x < whi; buf = NB == 2 ? buf ^ 1 : 0) {
+    // the pages of the tile to be fetched are looked up while this one's keys are worked on
+    const bool more = x + cur.count < whi, fetches = ax < whi;
+    if (fetches) page = page_of(ahead);
+    copy_wait<2 * NB - 1>();
+    lost |= bad & 1;
     if (x == wlo || cur.u == 0) {          // a new row: its queries, and an empty state
       const int at = t * (D / 4) * (int)sizeof(T);
       const uint4 *q = reinterpret_cast<const uint4 *>(
@@ -675,40 +690,41 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       m = -INFINITY;
       l = 0.0f;
       at_row = cur.u;
-      lost = __any_sync(~0u, lane < cur.count && (unsigned)page_c >= (unsigned)c.pages);
+      lost = bad & 1;
     }
+    bad >>= 1;
     const int valid = cur.n - cur.u * 16;
-    if (cur.count == TU && valid >= TT) {
+    const uint8_t *const kt = sk + buf * 2 * C::TILEB, *const vt = sv + buf * 2 * C::TILEB;
+    if (TU == 1 || (cur.count == TU && valid >= TT)) {
       float s[TT / 8][2];
-      scores(s, 0);
-      if (more) rows_of(nxt, page_n, rows);
+      scores(s, 0, kt);
+      if (fetches) rows_of(ahead, page, rows);
       powers(ske, kpow, p.scale);
       __syncwarp();
-      if (more) fetch(nxt, rows, false, false);
+      if (fetches) fetch(ahead, rows, false, false, buf);
       else copy_commit();
-      const float alpha = weights(s, 0, TT);
-      copy_wait_but_one();
+      const float alpha = weights(s, 0, valid);
+      copy_wait<2 * NB - 1>();
       powers(sve, vpow, 1.0f);
-      values(s, 0, alpha);
+      values(s, 0, alpha, vt);
       __syncwarp();
-      if (more) fetch(nxt, rows, true, false);
+      if (fetches) fetch(ahead, rows, true, false, buf);
       else copy_commit();
     } else {
-      copy_commit();
-      copy_wait_but_one();
+      copy_wait<0>();
       powers(ske, kpow, p.scale);
       powers(sve, vpow, 1.0f);
 #pragma unroll 1
       for (int i = 0; i < cur.count; ++i) {
         float s[2][2];
-        scores(s, i);
-        values(s, i, weights(s, i, valid - i * 16));
+        scores(s, i, kt);
+        values(s, i, weights(s, i, valid - i * 16), vt);
       }
       __syncwarp();
-      if (more) {
-        rows_of(nxt, page_n, rows);
-        fetch(nxt, rows, false, false);
-        fetch(nxt, rows, true, false);
+      if (fetches) {
+        rows_of(ahead, page, rows);
+        fetch(ahead, rows, false, false, buf);
+        fetch(ahead, rows, true, false, buf);
       }
     }
 
@@ -754,9 +770,14 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         if (lane == 0) rec_row[warp * 2 + slot] = row;
       }
     }
-    x = next;
-    cur = nxt;
-    page_c = page_n;
+    x += cur.count;
+    cur = NB == 2 ? mid : ahead;
+    mid = ahead;
+    if (fetches) {
+      bad |= (uint32_t)is_bad(ahead, page) << (NB - 1);
+      ax += ahead.count;
+      if (ax < whi) advance(ahead, whi - ax);
+    }
   }
   __syncthreads();
 
