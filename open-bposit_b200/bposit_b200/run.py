@@ -3,6 +3,7 @@
     python -m bposit_b200.run gemm M N K [--fmt bp8|bp16] [--group 128] [--calls 3] [--algo 0] [--timeline]
     python -m bposit_b200.run codec N [--fmt bp8|bp16] [--calls 3]
     python -m bposit_b200.run qwen05 [--batch 8] [--seq 1024] [--layers 24] [--fp32]
+    python -m bposit_b200.run generate [--batch 8] [--seq 1024] [--new 16] [--fmt bp8|bp16] [--budget 0] [--fp32]
     python -m bposit_b200.run linear M N K [--calls 3]
 
 ``gemm`` times bp_quire_gemm on operands N(0,1) * 2^U{-8..8} per row (the
@@ -11,7 +12,9 @@ adds the start and end of every kernel of one more call); ``linear`` times
 one BpositLinear (the W8A8 nn.Linear drop-in, fp32 out) of N x K random
 weights on M rows of N(0,1) activations; ``codec`` times
 the encode and decode kernels on the codec-sweep value mix; ``qwen05`` times
-the Qwen2.5-0.5B-shaped decoder forward with every linear a BpositLinear.  Each runs
+the Qwen2.5-0.5B-shaped decoder forward with every linear a BpositLinear;
+``generate`` times its decode steps (`--new` of them) behind a prompt, with
+the paged b-posit key-value cache.  Each runs
 `--calls` untimed calls and then `--calls` calls timed with CUDA events, so a
 profiler can capture a fixed, small number of launches (e.g. ``ncu -k
 regex:k_quire_gemm_tc -c 1``).
@@ -130,6 +133,29 @@ def run_qwen05(a) -> str:
             f"linears {model.linear_ops(tok) / ms / 1e9:.1f} TOPS over the whole forward")
 
 
+def run_generate(a) -> str:
+    from .forward import qwen05, synthetic_ids
+    model = qwen05(layers=a.layers, bposit=not a.fp32)
+    ids = synthetic_ids(a.batch, a.seq, seed=a.seed)
+    cap = a.seq + 2 * a.new + 2
+    cache = model.new_cache(a.batch, cap, a.fmt, track=a.budget > 0)
+    tables = model.rope_tables(cap)
+    model.prefill(ids, cache)
+    token = ids[:, -1]
+
+    def step():
+        if a.budget and cache.longest >= a.budget + cache.page_size:
+            cache.evict(a.budget, recent=cache.page_size, sinks=4)
+        return model.step(token, cache, tables)
+
+    step()
+    ms = _time(step, a.new)
+    held = 2 * cache.k.numel() * cache.k.element_size() + (0 if cache.k_exp is None else 2 * cache.k_exp.numel())
+    return (f"qwen05-shaped decode step ({'fp32 torch linears' if a.fp32 else 'bp8 W8A8 exact-quire linears'}, {a.fmt} "
+            f"cache{f', {a.budget} entries kept' if a.budget else ''}) batch={a.batch} behind {a.seq} tokens, "
+            f"layers={a.layers}: {ms:.3f} ms, {a.batch / ms * 1e3:.0f} tokens/s, cache {held / 2**20:.0f} MiB")
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="python -m bposit_b200.run")
     sub = ap.add_subparsers(dest="what", required=True)
@@ -149,17 +175,26 @@ def main(argv=None) -> int:
     w.add_argument("--seq", type=int, default=1024)
     w.add_argument("--layers", type=int, default=24)
     w.add_argument("--fp32", action="store_true", help="plain torch fp32 linears, for comparison")
+    ge = sub.add_parser("generate")
+    ge.add_argument("--batch", type=int, default=8)
+    ge.add_argument("--seq", type=int, default=1024, help="prompt tokens")
+    ge.add_argument("--new", type=int, default=16, help="decode steps timed")
+    ge.add_argument("--layers", type=int, default=24)
+    ge.add_argument("--fmt", default="bp8", choices=["bp8", "bp16"], help="cache format")
+    ge.add_argument("--budget", type=int, default=0, help="entries kept per layer and kv head (0: all)")
+    ge.add_argument("--fp32", action="store_true", help="plain torch fp32 linears")
     li = sub.add_parser("linear")
     li.add_argument("M", type=int)
     li.add_argument("N", type=int)
     li.add_argument("K", type=int)
-    for p in (g, c, w, li):
+    for p in (g, c, w, ge, li):
         p.add_argument("--calls", type=int, default=3)
         p.add_argument("--seed", type=int, default=0)
     a = ap.parse_args(argv)
     if not torch.cuda.is_available():
         raise SystemExit("no CUDA device")
-    fn = {"gemm": run_gemm, "codec": run_codec, "qwen05": run_qwen05, "linear": run_linear}[a.what]
+    fn = {"gemm": run_gemm, "codec": run_codec, "qwen05": run_qwen05, "generate": run_generate,
+          "linear": run_linear}[a.what]
     print(fn(a), flush=True)
     return 0
 
