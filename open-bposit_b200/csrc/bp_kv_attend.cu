@@ -10,56 +10,72 @@ namespace bp {
 namespace {
 
 constexpr int kJoinParts = 256;     // CTAs of one launch, at most
-constexpr int kJoinBatch = 16;      // parts whose outputs are loaded at once
+constexpr int kJoinWarps = 4, kJoinBatch = 8;   // warps of a block, parts that a warp loads at once
 
-// Joins the parts of a row that several CTAs of k_kv_attend worked on: block c
-// takes the row that starts in CTA c's range and goes on behind it, a warp for
-// each head.  A lane takes every 32nd part's statistics, then D / 32 columns of
-// the output, the loads of 16 parts in flight together.  Launched early
-// (programmatic dependent launch), its start hides behind the main kernel.
+// Joins the parts of a row that several CTAs of k_kv_attend worked on: block
+// (c, h) takes head h of the row that starts in CTA c's range and goes on behind
+// it.  Every warp reads all parts' statistics (a lane every 32nd, all at once) and
+// sums the outputs of every fourth part, eight in flight together, so that a row
+// of 74 parts (131071 entries of one sequence) waits for memory five times.
+// Launched early (programmatic dependent launch), its start hides behind the
+// main kernel.
 template <typename T>
-__global__ void __launch_bounds__(kHeadsPerRow * 32) k_kv_join(AttendParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) k_kv_join(AttendParams p) {
+  __shared__ float sums[kJoinWarps][128];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 open = p.cta_row[blockIdx.x];
   if (open.x < 0) return;
-  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y, h = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y, h = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t head = head_of(p, row_id(p, open.x), h);
   // the first part is the CTA's second record (a row that starts there), the others are first records
-  const float *base = p.cta_rec + blockIdx.x * 2 * (rec + 16);
+  const float *base = p.cta_rec + blockIdx.x * 2 * (rec + 16) + lane;
   auto part = [&](int k) { return base + (k ? k * 2 : 1) * (rec + 16); };
-  float M = -INFINITY, L = 0.0f;
-  for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[rec + h]);
+  float m[kJoinParts / 32], l[kJoinParts / 32], M = -INFINITY, L = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kJoinParts / 32; ++i) {
+    const int k = min(i * 32 + lane, parts - 1);       // (past the last part: the last one again, with weight 0)
+    m[i] = i * 32 < parts ? part(k)[rec + h - lane] : -INFINITY;
+    l[i] = i * 32 < parts ? part(k)[rec + 8 + h - lane] : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < kJoinParts / 32; ++i) M = fmaxf(M, m[i]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
-  for (int k = lane; k < parts; k += 32) L = fmaf(part(k)[rec + 8 + h], ex2(part(k)[rec + h] - M), L);
+#pragma unroll
+  for (int i = 0; i < kJoinParts / 32; ++i) {
+    m[i] = i * 32 + lane < parts ? ex2(m[i] - M) : 0.0f;       // the part's weight from here on
+    L = i * 32 + lane < parts ? fmaf(l[i], m[i], L) : L;
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
   float O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-  for (int k = 0; k < parts; k += kJoinBatch) {
-    // (past the last part: the last one again, with weight 0)
-    const int mine = k + (lane & (kJoinBatch - 1));
-    const float a = ex2(part(min(mine, parts - 1))[rec + h] - M);
+#pragma unroll
+  for (int i = 0; i < kJoinParts / 32; ++i) {
+    if (i * 32 >= parts) break;
     float x[kJoinBatch][4];
 #pragma unroll
     for (int j = 0; j < kJoinBatch; ++j) {
-      const float *r = part(min(k + j, parts - 1)) + h * D + lane;
+      const float *r = part(min(i * 32 + j * kJoinWarps + warp, parts - 1)) + h * D;
 #pragma unroll
       for (int y = 0; y < 4; ++y) x[j][y] = y * 32 < D ? r[y * 32] : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < kJoinBatch; ++j) {
-      const float f = k + j < parts ? __shfl_sync(~0u, a, j) : 0.0f;
+      const float f = __shfl_sync(~0u, m[i], j * kJoinWarps + warp);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) O[y] = k + j < parts ? fmaf(x[j][y], f, O[y]) : O[y];
+      for (int y = 0; y < 4; ++y) O[y] = i * 32 + j * kJoinWarps + warp < parts ? fmaf(x[j][y], f, O[y]) : O[y];
     }
   }
-  if (lane == 0) write_lse(p, open.x, h, head, M + log2f(L));
-  if (head < 0) return;
+  static_assert(kJoinWarps * kJoinBatch == 32, "32 parts a round");
 #pragma unroll
-  for (int y = 0; y < 4; ++y)
-    if (y * 32 < D) ((T *)p.out)[head * D + y * 32 + lane] = from_f32<T>(O[y] / L);
+  for (int y = 0; y < 4; ++y) sums[warp][y * 32 + lane] = O[y];
+  __syncthreads();
+  if (threadIdx.x == 0) write_lse(p, open.x, h, head, M + log2f(L));
+  const int d = threadIdx.x;
+  if (head >= 0 && d < D)
+    ((T *)p.out)[head * D + d] = from_f32<T>(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / L);
 }
 
 // scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2):
@@ -86,10 +102,10 @@ __global__ void __launch_bounds__(256) k_kv_scores(AttendParams p) {
 }
 
 template <typename K>
-int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t s, const char *what) {
+int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t s, const char *what, int threads = 256) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -200,9 +216,9 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   // (a batch of at most kMinUnits units is one CTA's, and no row of it is in parts)
   const int64_t units = (int64_t)cache->batch * cache->kv_heads * p.chunks * ((p.max_len + 15) / 16);
   if (rc == kOk && units > kMinUnits) {
-    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid), p, s, "k_kv_join");
-    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid), p, s, "k_kv_join");
-    else rc = launch_after(k_kv_join<__half>, dim3(grid), p, s, "k_kv_join");
+    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join", kJoinWarps * 32);
+    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join", kJoinWarps * 32);
+    else rc = launch_after(k_kv_join<__half>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join", kJoinWarps * 32);
   }
   if (rc == kOk && accumulate && p.max_len)
     rc = launch_after(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), p, s, "k_kv_scores");
