@@ -37,6 +37,29 @@ struct KvView {
 // Argument checks common to the cache's entry points; fills `view` for `layer`.
 int kv_check(const bp_kv_cache *c, int layer, const char *what, KvView *view);
 
+// Launches a kernel that begins with, or comes to, griddepcontrol.wait before it
+// touches memory that earlier work of the stream writes: its start overlaps the
+// end of the kernel ahead.
+template <typename K, typename P>
+int launch_early(K kernel, dim3 grid, int threads, size_t smem, const P &params, cudaStream_t s, const char *what) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(kECuda, "%s: %s", what, cudaGetErrorString(e));
+  }
+  return check_launch(what);
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T x) { return (float)x; }
 template <>

@@ -143,6 +143,8 @@ __device__ __forceinline__ void encode8(const float (&x)[8], int e, uint32_t (&o
 
 template <typename T, int D, int FMT, int U>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW;
   const KvView &c = p.c;
   const int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
@@ -262,9 +264,8 @@ int launch_append(AppendParams p, cudaStream_t s) {
   const int rows = few ? RPW : RPW * U;
   p.q_warps = (heads + rows - 1) / rows;
   const dim3 grid(blocks, p.q_warps + (2 * p.c.kv_heads + RPW - 1) / RPW);
-  if (few) k_kv_append<T, D, FMT, 1><<<grid, kAppendThreads, 0, s>>>(p);
-  else k_kv_append<T, D, FMT, U><<<grid, kAppendThreads, 0, s>>>(p);
-  return check_launch("k_kv_append");
+  return few ? launch_early(k_kv_append<T, D, FMT, 1>, grid, kAppendThreads, 0, p, s, "k_kv_append")
+             : launch_early(k_kv_append<T, D, FMT, U>, grid, kAppendThreads, 0, p, s, "k_kv_append");
 }
 
 template <typename T, int FMT>

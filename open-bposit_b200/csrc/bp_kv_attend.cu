@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_kv_join(AttendParams p) {
 // scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2):
 // one thread per entry, so the sum has one order and needs no atomics.
 __global__ void __launch_bounds__(256) k_kv_scores(AttendParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int bk = blockIdx.y, b = bk / p.c.kv_heads;
   const int n = min(p.c.length(b), p.max_len);
@@ -99,22 +100,6 @@ __global__ void __launch_bounds__(256) k_kv_scores(AttendParams p) {
   }
   // a sequence with a page outside the pool has NaN for all its sums and keeps its scores
   if (!isnan(p.lse2[(int64_t)bk * p.chunks * kHeadsPerRow])) p.c.scores[(int64_t)bk * p.c.cap + i] += w;
-}
-
-template <typename K>
-int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t s, const char *what, int threads = 256) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
-  if (e != cudaSuccess) return set_error(kECuda, "%s: %s", what, cudaGetErrorString(e));
-  return check_launch(what);
 }
 
 // CTAs of the main kernel: one per SM.
@@ -216,12 +201,13 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   // (a batch of at most kMinUnits units is one CTA's, and no row of it is in parts)
   const int64_t units = (int64_t)cache->batch * cache->kv_heads * p.chunks * ((p.max_len + 15) / 16);
   if (rc == kOk && units > kMinUnits) {
-    if (dtype == BP_F32) rc = launch_after(k_kv_join<float>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join", kJoinWarps * 32);
-    else if (dtype == BP_BF16) rc = launch_after(k_kv_join<__nv_bfloat16>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join", kJoinWarps * 32);
-    else rc = launch_after(k_kv_join<__half>, dim3(grid, kHeadsPerRow), p, s, "k_kv_join", kJoinWarps * 32);
+    if (dtype == BP_F32) rc = launch_early(k_kv_join<float>, dim3(grid, kHeadsPerRow), kJoinWarps * 32, 0, p, s, "k_kv_join");
+    else if (dtype == BP_BF16) rc = launch_early(k_kv_join<__nv_bfloat16>, dim3(grid, kHeadsPerRow), kJoinWarps * 32, 0, p, s, "k_kv_join");
+    else rc = launch_early(k_kv_join<__half>, dim3(grid, kHeadsPerRow), kJoinWarps * 32, 0, p, s, "k_kv_join");
   }
   if (rc == kOk && accumulate && p.max_len)
-    rc = launch_after(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), p, s, "k_kv_scores");
+    rc = launch_early(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), 256, 0, p, s,
+                      "k_kv_scores");
   if (!workspace) {
     cudaError_t f = cudaFreeAsync(ws, s);
     if (rc == kOk && f != cudaSuccess) rc = set_error(kECuda, "%s: workspace free: %s", what, cudaGetErrorString(f));

@@ -280,7 +280,7 @@ struct Deal {
 };
 // CTAs that take part: at least kMinUnits units each, so that short batches are
 // not cut into parts that cost more to join than to read.
-constexpr int kMinUnits = 32;
+constexpr int kMinUnits = 8;
 __device__ __forceinline__ int active_ctas(int units, int grid) { return min((units + kMinUnits - 1) / kMinUnits, grid); }
 
 template <int FMT, int D, typename T>
@@ -303,9 +303,6 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   const KvView &c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_seq = c.kv_heads * p.chunks;             // work rows of one sequence
-  asm volatile("griddepcontrol.launch_dependents;");
-
-  auto length = [&](int b) { return min(c.length(b), p.max_len); };
   // the decode table: word 64 i + lane
   for (int i = tid; i < 256; i += NT) {
     uint32_t v;
@@ -324,6 +321,10 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
 #pragma unroll
     for (int j = 0; j < 8; ++j) row[(j + i) & 7] = make_uint4(v, v, v, v);
   }
+  // (all of the above may run before the kernels ahead in the stream have finished)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  auto length = [&](int b) { return min(c.length(b), p.max_len); };
   // units before each sequence
   {
     const int each = (c.batch + NT - 1) / NT;
@@ -860,8 +861,7 @@ int launch_kv_attend_one(const AttendParams &p, int grid, cudaStream_t s) {
     return set_error(kENoDev, "k_kv_attend: shared memory starts at %d, not %d", reserved, kSharedReserved);
   cudaError_t e = cudaFuncSetAttribute(k_kv_attend<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return set_error(kECuda, "k_kv_attend: %s", cudaGetErrorString(e));
-  k_kv_attend<FMT, D, T><<<grid, C::NW * 32, C::SMEM, s>>>(p);
-  return check_launch("k_kv_attend");
+  return launch_early(k_kv_attend<FMT, D, T>, dim3(grid), C::NW * 32, C::SMEM, p, s, "k_kv_attend");
 }
 template <int FMT, typename T>
 int launch_kv_attend_dim(const AttendParams &p, int grid, cudaStream_t s) {

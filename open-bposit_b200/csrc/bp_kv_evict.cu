@@ -105,6 +105,8 @@ __device__ __forceinline__ void move_entries(const EvictParams &p, int64_t r, in
 //    ballot, one scan of the counts gives everyone's rank.
 template <int NT, int KPT>
 __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int NW = NT / 32, BINS = 2048, PER = BINS / NT, E = NW * KPT;
   const KvView &c = p.c;
   const int r = blockIdx.x;
@@ -290,6 +292,8 @@ __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
 // after it was scanned, and movers are read from behind the budget, which nothing
 // writes.
 __global__ void __launch_bounds__(kThreads) k_kv_evict_long(EvictParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const KvView &c = p.c;
   const int64_t r = blockIdx.x;
   const int hk = (int)(r % c.kv_heads), b = (int)(r / c.kv_heads % c.batch);
@@ -413,13 +417,13 @@ extern "C" int bp_kv_evict(const bp_kv_cache *cache, const float *weights, int b
   p.weights = weights ? weights : cache->scores;
   p.budget = budget; p.recent = recent; p.sinks = sinks; p.keep = keep;
   cudaStream_t s = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)rows;
+  const dim3 grid((unsigned)rows);
   // the smallest block that holds a row's weights in registers, 4 a thread while that is enough threads; longer rows
   // stream them
-  if (p.c.cap <= 256 * 4) k_kv_evict_row<256, 4><<<grid, 256, 0, s>>>(p);
-  else if (p.c.cap <= 512 * 4) k_kv_evict_row<512, 4><<<grid, 512, 0, s>>>(p);
-  else if (p.c.cap <= 512 * 16) k_kv_evict_row<512, 16><<<grid, 512, 0, s>>>(p);
-  else if (p.c.cap <= 1024 * 16) k_kv_evict_row<1024, 16><<<grid, 1024, 0, s>>>(p);
-  else k_kv_evict_long<<<grid, kThreads, 0, s>>>(p);
-  return check_launch("k_kv_evict");
+  static const char *const name = "k_kv_evict";
+  if (p.c.cap <= 256 * 4) return launch_early(k_kv_evict_row<256, 4>, grid, 256, 0, p, s, name);
+  if (p.c.cap <= 512 * 4) return launch_early(k_kv_evict_row<512, 4>, grid, 512, 0, p, s, name);
+  if (p.c.cap <= 512 * 16) return launch_early(k_kv_evict_row<512, 16>, grid, 512, 0, p, s, name);
+  if (p.c.cap <= 1024 * 16) return launch_early(k_kv_evict_row<1024, 16>, grid, 1024, 0, p, s, name);
+  return launch_early(k_kv_evict_long, grid, kThreads, 0, p, s, name);
 }
