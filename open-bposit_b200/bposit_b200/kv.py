@@ -119,6 +119,7 @@ class PagedKVCache:
         self._struct = _Struct(8 if bp8 else 16, layers, pages, page, heads, dim, batch, per, ptr(k), ptr(v),
                                ptr(k_exp), ptr(v_exp), ptr(table), ptr(self.lengths), ptr(positions), ptr(scores))
         self._ref = ctypes.byref(self._struct)
+        self._workspace = {}     # bytes that paged_attention needs, by its arguments
 
     def advance(self, n=1, most: int | None = None):
         """Make room for n more entries in every sequence (an int), or for n[b]

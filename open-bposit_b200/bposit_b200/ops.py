@@ -406,17 +406,16 @@ def _act(t, name: str, rows, heads, cache, dtype=None) -> torch.Tensor:
     read: heads contiguous, rows 16 bytes apart or more (copied if not)."""
     if not isinstance(t, torch.Tensor) or t.device != cache.device:
         raise ValueError(f"{name} must be a CUDA tensor on {cache.device}")
-    if t.dtype not in _ACT or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name} must be {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
-    D = cache.head_dim
-    shape = t.shape
+    dt, D, shape = t.dtype, cache.head_dim, t.shape
+    if dt not in _ACT or (dtype is not None and dt != dtype):
+        raise ValueError(f"{name} must be {dtype or 'float32, bfloat16 or float16'}, got {dt}")
     if len(shape) != 3 or shape[2] != D or (rows is not None and shape[0] != rows) or \
             (heads is not None and shape[1] != heads):
         raise ValueError(f"{name} must be {['rows' if rows is None else rows, 'heads' if heads is None else heads, D]}, "
                          f"got {list(shape)}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s1 != D and shape[1] > 1) or s0 & (3 if t.dtype == torch.float32 else 7) or \
-            s0 < shape[1] * D or t.data_ptr() & 15:
+    if s2 != 1 or (s1 != D and shape[1] > 1) or s0 & (3 if dt == torch.float32 else 7) or s0 < shape[1] * D or \
+            t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -433,7 +432,7 @@ def _ints(t, name: str, n: int, cache):
 def _like(out, q: torch.Tensor, name: str) -> torch.Tensor:
     """`out`, or a new contiguous tensor of q's shape and type."""
     if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
+        return torch.empty_like(q)      # (q's heads are contiguous: so is the new tensor)
     if not isinstance(out, torch.Tensor) or out.dtype != q.dtype or out.shape != q.shape or \
             out.device != q.device or not out.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor like q")
@@ -468,16 +467,18 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=Non
     k = _act(k, "k", None, cache.kv_heads, cache)
     dt = k.dtype
     n = k.shape[0]
-    v = _act(v, "v", n, cache.kv_heads, cache, dt)
+    if v.dtype != dt or v.shape != k.shape or v.stride() != k.stride() or v.device != cache.device or v.data_ptr() & 15:
+        v = _act(v, "v", n, cache.kv_heads, cache, dt)
     rows = heads = qs = 0
     cp = sp = qp = op = None
     if cos is not None or sin is not None:
         if cos is None or sin is None:
             raise ValueError("cos and sin come together")
-        shape = (cos.shape[0], cache.head_dim // 2)
-        for t in (cos, sin):
-            if t.dtype != torch.float32 or t.shape != shape or t.device != cache.device or not t.is_contiguous():
-                raise ValueError(f"cos and sin must be contiguous float32 CUDA tensors [rows, {shape[1]}]")
+        shape = cos.shape
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or sin.shape != shape or \
+                shape[1] * 2 != cache.head_dim or cos.device != cache.device or sin.device != cache.device or \
+                not cos.is_contiguous() or not sin.is_contiguous():
+            raise ValueError(f"cos and sin must be contiguous float32 CUDA tensors [rows, {cache.head_dim // 2}]")
         rows, cp, sp = shape[0], cos.data_ptr(), sin.data_ptr()
     if q is not None:
         if cos is None:
@@ -518,7 +519,11 @@ def paged_attention(cache, q: torch.Tensor, layer: int = 0, scale: float | None 
     elif max_length < 1:
         raise ValueError("max_length must be positive")
     L = _lib.lib()
-    need = L.bp_paged_attention_workspace_size(cache._ref, heads, max_length, accumulate)
+    need = cache._workspace.get((heads, max_length, accumulate))
+    if need is None:
+        need = L.bp_paged_attention_workspace_size(cache._ref, heads, max_length, accumulate)
+        if len(cache._workspace) < 64:
+            cache._workspace[heads, max_length, accumulate] = need
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _call(L.bp_paged_attention, dev, cache._ref, layer, _ACT[dt], heads, q.data_ptr(), q.stride(0), out.data_ptr(),
           None if lse is None else lse.data_ptr(), cache.head_dim ** -0.5 if scale is None else scale, max_length,
