@@ -84,14 +84,14 @@ template <int FMT, int D, typename T>
 struct AttendCfg {
   static constexpr int BYTES = FMT / 8;
   static constexpr int ROWB = D * BYTES;
-  // Entries per tile, and tiles in the stage: two of one unit for wide bp16 rows, whose unrolled steps would not fit
-  // the instruction cache with more (32 entries at D = 128: 84 us, a quarter of it waiting for instructions).
+  // Entries per tile, tiles in the stage, warps, and parts that an output's columns are worked on in.  Wide bp16 rows
+  // take single units, whose unrolled steps fit the instruction cache (32 entries at D = 128: 84 us, a quarter of it
+  // waiting for instructions, where single units take WIDE us).
+  static constexpr bool WIDE = FMT == 16 && D > 64;
   static constexpr int TT = FMT == 8 ? (D <= 64 ? 64 : 32) : (D <= 32 ? 64 : (D <= 64 ? 32 : 16));
-  static constexpr int NB = TT == 16 ? 2 : 1;
-#ifndef KV_NW
-#define KV_NW 12
-#endif
-  static constexpr int NW = D <= 64 ? KV_NW : 8;
+  static constexpr int NB = 1;
+  static constexpr int NW = D <= 64 ? 12 : 8;
+  static constexpr int PARTS = WIDE ? 2 : 1;
   static constexpr int TILEB = TT * ROWB;
   // 2^exponent of a tile's keys and values as fp32, [t][n][2] in the order that thread t of a quad needs them, with
   // a row stride that keeps the four rows in different banks
@@ -607,7 +607,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     return alpha;
   };
   // O[head, d] = alpha O + P V
-  auto values_with = [&](auto exact, const auto &s, int i0, auto &acc, const uint8_t *sv) {
+  // (columns part * DH .. of each thread's DN: wide rows in two parts, for fewer registers)
+  constexpr int DH = DN / C::PARTS, VH = VW / C::PARTS;
+  auto values_with = [&](auto exact, const auto &s, int i0, int part, auto &acc, const uint8_t *sv) {
     uint32_t odd = 0;
     constexpr int SN = sizeof(s) / sizeof(s[0]);
 #pragma unroll
@@ -620,13 +622,14 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       }
       const uint32_t a[4] = {tf32_high(w0), tf32_high(w0 - __uint_as_float(tf32_high(w0))), tf32_high(w1),
                              tf32_high(w1 - __uint_as_float(tf32_high(w1)))};
-      uint32_t v0[VW], v1[VW];
+      uint32_t v0[VH], v1[VH];
       const uint8_t *r = sv + (i0 * 16 + i * 8) * C::ROWB;
-      load_words<C::ROWB>(r, e0, g * VW, v0);
-      load_words<C::ROWB>(r, e1, g * VW, v1);
+      load_words<C::ROWB>(r, e0, g * VW + part * VH, v0);
+      load_words<C::ROWB>(r, e1, g * VW + part * VH, v1);
 #pragma unroll
-      for (int d = 0; d < DN; ++d) {
-        const uint32_t b0 = decode_code<FMT, decltype(exact)::value>(entry, v0[d / CW], d % CW, odd), b1 = decode_code<FMT, decltype(exact)::value>(entry, v1[d / CW], d % CW, odd);
+      for (int d = 0; d < DH; ++d) {
+        const uint32_t b0 = decode_code<FMT, decltype(exact)::value>(entry, v0[d / CW], d % CW, odd);
+        const uint32_t b1 = decode_code<FMT, decltype(exact)::value>(entry, v1[d / CW], d % CW, odd);
         if (i == 0) mma_tf32_first(acc[d], a, b0, b1);
         else mma_tf32(acc[d], a, b0, b1);
       }
@@ -634,13 +637,17 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     return odd;
   };
   auto values = [&](const auto &s, int i0, float alpha, const uint8_t *sv) {
-    float acc[DN][4];
-    const uint32_t odd = values_with(std::false_type{}, s, i0, acc, sv);
-    if (FMT == 16 && __any_sync(~0u, odd & 1u)) values_with(std::true_type{}, s, i0, acc, sv);
 #pragma unroll
-    for (int d = 0; d < DN; ++d) {
-      o[d][0] = fmaf(o[d][0], alpha, acc[d][0] + acc[d][2]);
-      o[d][1] = fmaf(o[d][1], alpha, acc[d][1] + acc[d][3]);
+    for (int part = 0; part < C::PARTS; ++part) {
+      float acc[DH][4];
+      const uint32_t odd = values_with(std::false_type{}, s, i0, part, acc, sv);
+      if (FMT == 16 && __any_sync(~0u, odd & 1u)) values_with(std::true_type{}, s, i0, part, acc, sv);
+#pragma unroll
+      for (int d = 0; d < DH; ++d) {
+        float *out = o[part * DH + d];
+        out[0] = fmaf(out[0], alpha, acc[d][0] + acc[d][2]);
+        out[1] = fmaf(out[1], alpha, acc[d][1] + acc[d][3]);
+      }
     }
   };
   // each exponent of the tile is turned into a power of two once, and read back by the four threads that need it
