@@ -84,25 +84,19 @@ template <int FMT, int D, typename T>
 struct AttendCfg {
   static constexpr int BYTES = FMT / 8;
   static constexpr int ROWB = D * BYTES;
-  // Entries per tile, tiles in the stage, warps, and parts that an output's columns are worked on in.  Wide bp16 rows
+  // Entries per tile, warps, and parts that an output's columns are worked on in.  Wide bp16 rows
   // take single units, whose unrolled steps fit the instruction cache (32 entries at D = 128: 84 us, a quarter of it
-  // waiting for instructions, where single units take WIDE us).
+  // waiting for instructions, where single units take 48 us).
   static constexpr bool WIDE = FMT == 16 && D > 64;
   static constexpr int TT = FMT == 8 ? (D <= 64 ? 64 : 32) : (D <= 32 ? 64 : (D <= 64 ? 32 : 16));
-  static constexpr int NB = 1;
-  static constexpr int NW = D <= 64 ? 12 : 8;
+    static constexpr int NW = 8;
   static constexpr int PARTS = WIDE ? 2 : 1;
   static constexpr int TILEB = TT * ROWB;
   // 2^exponent of a tile's keys and values as fp32, [t][n][2] in the order that thread t of a quad needs them, with
   // a row stride that keeps the four rows in different banks
   static constexpr int POWROW = TT / 4 + 8;
   static constexpr int POWB = FMT == 8 ? 2 * 4 * POWROW * 4 : 0;
-  // keys, values, their exponents, the powers, and the queries of the next row (one row's: with two tiles under way
-  // they are read from memory when a row starts)
-  static constexpr bool QSTAGE = NB == 1;
-  static constexpr int QAT = NB * 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;
-  static constexpr int QROW = D * (int)sizeof(T) + 16;           // padded: the 8 heads' pieces in different banks
-  static constexpr int STAGE = QAT + (QSTAGE ? kHeadsPerRow * QROW : 0);
+  static constexpr int STAGE = 2 * TILEB + (FMT == 8 ? 2 * TT : 0) + POWB;   // keys, values, exponents, powers
   static constexpr int REC = kHeadsPerRow * D;                   // floats of one part's output
   // Shared memory: the decode table at shared addresses 64 K .. 128 K, so that an entry's address is the bytes {lane,
   // code, 1, 0}; FRONT stages below it, the others above.  The table's entries fill half of its 256-byte rows; the
@@ -118,7 +112,7 @@ struct AttendCfg {
     return warp < FRONT ? warp * STAGE : AFTER + (warp - FRONT) * STAGE;
   }
   static_assert(REC * 4 <= STAGE, "a part's output fits the stage");
-  static_assert(FMT == 16 || (TT % 32 == 0 && NB == 1), "a lane converts TT / 32 exponents, of one tile");
+  static_assert(FMT == 16 || TT % 32 == 0, "a lane converts TT / 32 exponents");
   static_assert(STAGE % 16 == 0, "stages stay 16-byte aligned");
 };
 
@@ -287,7 +281,7 @@ template <int FMT, int D, typename T>
 __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(AttendParams p) {
   using C = AttendCfg<FMT, D, T>;
   constexpr int TT = C::TT, NW = C::NW, NT = NW * 32;
-  constexpr int TU = TT / 16, NB = C::NB;
+  constexpr int TU = TT / 16;           // units per tile
   constexpr int DN = D / 8;             // 8-wide columns of O, and MMA steps along D
   constexpr int KW = C::ROWB / 16;      // words of a key row that one thread holds
   constexpr int VW = C::ROWB / 32;      // words of a value row that one thread holds
@@ -379,9 +373,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   const int wlo = lo + share.begin(warp), whi = lo + share.begin(warp + 1);
 
   uint8_t *const stage = smem + C::stage_at(warp);
-  uint8_t *const sk = stage, *const sv = stage + C::TILEB;   // (buffer i of NB: 2 TILEB i further)
-  int8_t *const ske = reinterpret_cast<int8_t *>(stage + NB * 2 * C::TILEB), *const sve = ske + TT;
-  float *const kpow = reinterpret_cast<float *>(stage + NB * 2 * C::TILEB + 2 * TT), *const vpow = kpow + 4 * C::POWROW;
+  uint8_t *const sk = stage, *const sv = stage + C::TILEB;
+  int8_t *const ske = reinterpret_cast<int8_t *>(stage + 2 * C::TILEB), *const sve = ske + TT;
+  float *const kpow = reinterpret_cast<float *>(stage + 2 * C::TILEB + 2 * TT), *const vpow = kpow + 4 * C::POWROW;
   // ---- where tiles lie: units u .. u + count - 1 of a work row ----
   struct Place {
     int b, row, hk, ch, u, count, n;       // sequence, work row of it (hk * chunks + ch), units, entries of the row
@@ -431,9 +425,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     for (int i = 0; i < TU; ++i) all = all && r.unit[i] != kNone;
     r.plain = all;
   };
-  auto fetch = [&](const Place &w, const Rows &r, bool value, bool first, int buf) {
+  auto fetch = [&](const Place &w, const Rows &r, bool value) {
     const uint8_t *pool = (value ? c.v : c.k) + lane * 16;
-    const uint32_t dst = stage_s + (2 * buf + value) * C::TILEB + to;
+    const uint32_t dst = stage_s + (value ? C::TILEB : 0) + to;
     if (r.plain) {
 #pragma unroll
       for (int i = 0; i < TU; ++i) {
@@ -457,23 +451,15 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         }
       }
     }
-    if (C::QSTAGE && !value && (w.u == 0 || first)) {   // a new row for this warp: its queries, 4 lanes a head
-      const int h = w.ch * kHeadsPerRow + g;
-      const uint8_t *q = reinterpret_cast<const uint8_t *>((const T *)p.q + w.b * p.qs + (int64_t)(w.hk * p.group + h) * D);
-#pragma unroll
-      for (int i = 0; i < D * (int)sizeof(T) / 64; ++i)
-        if (h < p.group) copy16(stage_s + C::QAT + g * C::QROW + (i * 4 + t) * 16, q + (i * 4 + t) * 16);
-    }
     if (FMT == 8 && r.mine != kNone)
-      copy16(stage_s + NB * 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + r.mine);
+      copy16(stage_s + 2 * C::TILEB + (value ? TT : 0) + lane * 16, (value ? c.v_exp : c.k_exp) + r.mine);
     copy_commit();
   };
 
-  // this tile, the one behind it (NB = 2), and the next to be fetched, which starts `ax` units into the row of tiles
-  Place cur{}, mid{}, ahead{};
+  Place cur{}, ahead{};        // this tile, and the next to be fetched, `ax` units into all units
   Rows rows{};
   int ax = wlo, page = -1;
-  uint32_t bad = 0;            // bit i: a page of tile i from here is outside the pool
+  bool bad = false;            // a page of the tile is outside the pool
   auto is_bad = [&](const Place &w, int pg) { return __any_sync(~0u, lane < w.count && (unsigned)pg >= (unsigned)c.pages); };
   if (wlo < whi) {
     int a = 0, z = c.batch;                // sequence of the first unit, by bisection
@@ -491,22 +477,13 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     cur.ch = cur.row - cur.hk * p.chunks;
     cur.count = min(min(TU, nu - cur.u), whi - wlo);
     ahead = cur;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      if (ax < whi) {
-        page = page_of(ahead);
-        rows_of(ahead, page, rows);
-        bad |= (uint32_t)is_bad(ahead, page) << i;
-        fetch(ahead, rows, false, i == 0, i);
-        fetch(ahead, rows, true, false, i);
-        if (i == 1) mid = ahead;
-        ax += ahead.count;
-        if (ax < whi) advance(ahead, whi - ax);
-      } else {
-        copy_commit();
-        copy_commit();
-      }
-    }
+    page = page_of(ahead);
+    rows_of(ahead, page, rows);
+    bad = is_bad(ahead, page);
+    fetch(ahead, rows, false);
+    fetch(ahead, rows, true);
+    ax += ahead.count;
+    if (ax < whi) advance(ahead, whi - ax);
   }
   __syncthreads();
   const uint32_t entry = lane * 4 | (kTableAt >> 16) << 8;
@@ -525,7 +502,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
 
   // The three stages of a step over U units, from unit i0 of the stage on.
   // S[head, entry] = q K^T
-  auto scores_with = [&](auto exact, auto &s, int i0, const uint8_t *sk) {
+  auto scores_with = [&](auto exact, auto &s, int i0) {
     uint32_t odd = 0;
     constexpr int SN = sizeof(s) / sizeof(s[0]);
     // four columns at a time: an MMA waits for the one before it in its sum
@@ -555,9 +532,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
     return odd;
   };
-  auto scores = [&](auto &s, int i0, const uint8_t *sk) {
-    const uint32_t odd = scores_with(std::false_type{}, s, i0, sk);
-    if (FMT == 16 && __any_sync(~0u, odd & 1u)) scores_with(std::true_type{}, s, i0, sk);
+  auto scores = [&](auto &s, int i0) {
+    const uint32_t odd = scores_with(std::false_type{}, s, i0);
+    if (FMT == 16 && __any_sync(~0u, odd & 1u)) scores_with(std::true_type{}, s, i0);
   };
   // S becomes e^(S - maximum), maximum and sum move on; returns the factor for what was summed before
   auto weights = [&](auto &s, int i0, int valid) {
@@ -609,7 +586,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   // O[head, d] = alpha O + P V
   // (columns part * DH .. of each thread's DN: wide rows in two parts, for fewer registers)
   constexpr int DH = DN / C::PARTS, VH = VW / C::PARTS;
-  auto values_with = [&](auto exact, const auto &s, int i0, int part, auto &acc, const uint8_t *sv) {
+  auto values_with = [&](auto exact, const auto &s, int i0, int part, auto &acc) {
     uint32_t odd = 0;
     constexpr int SN = sizeof(s) / sizeof(s[0]);
 #pragma unroll
@@ -636,12 +613,12 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
     return odd;
   };
-  auto values = [&](const auto &s, int i0, float alpha, const uint8_t *sv) {
+  auto values = [&](const auto &s, int i0, float alpha) {
 #pragma unroll
     for (int part = 0; part < C::PARTS; ++part) {
       float acc[DH][4];
-      const uint32_t odd = values_with(std::false_type{}, s, i0, part, acc, sv);
-      if (FMT == 16 && __any_sync(~0u, odd & 1u)) values_with(std::true_type{}, s, i0, part, acc, sv);
+      const uint32_t odd = values_with(std::false_type{}, s, i0, part, acc);
+      if (FMT == 16 && __any_sync(~0u, odd & 1u)) values_with(std::true_type{}, s, i0, part, acc);
 #pragma unroll
       for (int d = 0; d < DH; ++d) {
         float *out = o[part * DH + d];
@@ -662,18 +639,15 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
   };
 
-  for (int x = wlo, buf = 0; x < whi; buf = NB == 2 ? buf ^ 1 : 0) {
+  for (int x = wlo; x < whi;) {
     // the pages of the tile to be fetched are looked up while this one's keys are worked on
     const bool more = x + cur.count < whi, fetches = ax < whi;
     if (fetches) page = page_of(ahead);
-    copy_wait<2 * NB - 1>();
-    lost |= bad & 1;
+    copy_wait<1>();
+    lost |= bad;
     if (x == wlo || cur.u == 0) {          // a new row: its queries, and an empty state
-      const int at = t * (D / 4) * (int)sizeof(T);
       const uint4 *q = reinterpret_cast<const uint4 *>(
-          C::QSTAGE ? stage + C::QAT + g * C::QROW + at
-                    : reinterpret_cast<const uint8_t *>((const T *)p.q + cur.b * p.qs +
-                                                        (int64_t)(cur.hk * p.group + cur.ch * kHeadsPerRow + g) * D) + at);
+          (const T *)p.q + cur.b * p.qs + (int64_t)(cur.hk * p.group + cur.ch * kHeadsPerRow + g) * D + t * (D / 4));
       constexpr int QV = D / 4 * sizeof(T) / 16;
       const bool real = cur.ch * kHeadsPerRow + g < p.group;
       uint4 raw[QV];
@@ -698,25 +672,23 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       m = -INFINITY;
       l = 0.0f;
       at_row = cur.u;
-      lost = bad & 1;
+      lost = bad;
     }
-    bad >>= 1;
     const int valid = cur.n - cur.u * 16;
-    const uint8_t *const kt = sk + buf * 2 * C::TILEB, *const vt = sv + buf * 2 * C::TILEB;
     if (TU == 1 || (cur.count == TU && valid >= TT)) {
       float s[TT / 8][2];
-      scores(s, 0, kt);
+      scores(s, 0);
       if (fetches) rows_of(ahead, page, rows);
       powers(ske, kpow, p.scale);
       __syncwarp();
-      if (fetches) fetch(ahead, rows, false, false, buf);
+      if (fetches) fetch(ahead, rows, false);
       else copy_commit();
       const float alpha = weights(s, 0, valid);
-      copy_wait<2 * NB - 1>();
+      copy_wait<1>();
       powers(sve, vpow, 1.0f);
-      values(s, 0, alpha, vt);
+      values(s, 0, alpha);
       __syncwarp();
-      if (fetches) fetch(ahead, rows, true, false, buf);
+      if (fetches) fetch(ahead, rows, true);
       else copy_commit();
     } else {
       copy_wait<0>();
@@ -725,14 +697,14 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
 #pragma unroll 1
       for (int i = 0; i < cur.count; ++i) {
         float s[2][2];
-        scores(s, i, kt);
-        values(s, i, weights(s, i, valid - i * 16), vt);
+        scores(s, i);
+        values(s, i, weights(s, i, valid - i * 16));
       }
       __syncwarp();
       if (fetches) {
         rows_of(ahead, page, rows);
-        fetch(ahead, rows, false, false, buf);
-        fetch(ahead, rows, true, false, buf);
+        fetch(ahead, rows, false);
+        fetch(ahead, rows, true);
       }
     }
 
@@ -779,10 +751,9 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       }
     }
     x += cur.count;
-    cur = NB == 2 ? mid : ahead;
-    mid = ahead;
+    cur = ahead;
     if (fetches) {
-      bad |= (uint32_t)is_bad(ahead, page) << (NB - 1);
+      bad = is_bad(ahead, page);
       ax += ahead.count;
       if (ax < whi) advance(ahead, whi - ax);
     }
