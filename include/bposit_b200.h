@@ -359,9 +359,12 @@ int bp_kv_append(const bp_kv_cache *cache, int layer, int dtype, int tokens, con
  * softmax's denominator.  An empty sequence gives zeros (lse -inf); one with a
  * page number outside the pool gives NaN.
  * accumulate = 1 also adds the softmax weight of each entry, summed over the
- * heads that share its kv head, to cache->scores (not for a sequence with a
- * page number outside the pool).  Products are exact in fp32 or better, sums,
- * softmax statistics and scores are fp32.  Entries at or past max_length are
+ * heads that share its kv head, to cache->scores (a kv head with a softmax that
+ * is NaN -- a page number outside the pool, a query that is not finite -- keeps
+ * its scores).  Products keep fp32 accuracy (queries and weights are split into
+ * 22 bits, codes are exact), sums, softmax statistics and scores are fp32.  The
+ * order of the sums follows from the lengths of the whole batch: the same call
+ * gives the same bits, another batch may round differently.  Entries at or past max_length are
  * left out (0: capacity); it bounds the workspace.
  * workspace: at least bp_paged_attention_workspace_size() bytes, 256-byte
  * aligned; NULL takes it stream-ordered from the device's memory pool. */

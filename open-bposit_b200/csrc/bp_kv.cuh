@@ -40,8 +40,8 @@ int kv_check(const bp_kv_cache *c, int layer, const char *what, KvView *view);
 // Launches a kernel that begins with, or comes to, griddepcontrol.wait before it
 // touches memory that earlier work of the stream writes: its start overlaps the
 // end of the kernel ahead.
-template <typename K, typename P>
-int launch_early(K kernel, dim3 grid, int threads, size_t smem, const P &params, cudaStream_t s, const char *what) {
+template <typename K, typename... P>
+int launch_early(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const char *what, const P &...params) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -52,7 +52,7 @@ int launch_early(K kernel, dim3 grid, int threads, size_t smem, const P &params,
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params...);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(kECuda, "%s: %s", what, cudaGetErrorString(e));

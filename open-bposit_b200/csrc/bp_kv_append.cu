@@ -264,8 +264,8 @@ int launch_append(AppendParams p, cudaStream_t s) {
   const int rows = few ? RPW : RPW * U;
   p.q_warps = (heads + rows - 1) / rows;
   const dim3 grid(blocks, p.q_warps + (2 * p.c.kv_heads + RPW - 1) / RPW);
-  return few ? launch_early(k_kv_append<T, D, FMT, 1>, grid, kAppendThreads, 0, p, s, "k_kv_append")
-             : launch_early(k_kv_append<T, D, FMT, U>, grid, kAppendThreads, 0, p, s, "k_kv_append");
+  return few ? launch_early(k_kv_append<T, D, FMT, 1>, grid, kAppendThreads, 0, s, "k_kv_append", p)
+             : launch_early(k_kv_append<T, D, FMT, U>, grid, kAppendThreads, 0, s, "k_kv_append", p);
 }
 
 template <typename T, int FMT>

@@ -1,7 +1,6 @@
 // bp_kv_attend.cu -- attention of one new token per sequence over the paged
-// b-posit key-value cache (bp_paged_attention): the entry
-// points, and the kernels that finish what k_kv_attend (bp_kv_attend.cuh) leaves in
-// parts.
+// b-posit key-value cache (bp_paged_attention): the entry points, and the kernel
+// that finishes what k_kv_attend (bp_kv_attend.cuh) leaves in parts.
 #include <math.h>
 
 #include "bp_kv_attend.cuh"
@@ -20,17 +19,15 @@ constexpr int kJoinWarps = 4, kJoinBatch = 8;   // warps of a block, parts that 
 // Launched early (programmatic dependent launch), its start hides behind the
 // main kernel.
 template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) k_kv_join(AttendParams p) {
+__device__ __forceinline__ void join_row(const AttendParams &p, int cta, int h) {
   __shared__ float sums[kJoinWarps][128];
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int2 open = p.cta_row[blockIdx.x];
+  const int2 open = p.cta_row[cta];
   if (open.x < 0) return;
-  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y, h = blockIdx.y;
+  const int D = p.c.dim, rec = kHeadsPerRow * D, parts = open.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t head = head_of(p, row_id(p, open.x), h);
   // the first part is the CTA's second record (a row that starts there), the others are first records
-  const float *base = p.cta_rec + blockIdx.x * 2 * (rec + 16) + lane;
+  const float *base = p.cta_rec + cta * 2 * (rec + 16) + lane;
   auto part = [&](int k) { return base + (k ? k * 2 : 1) * (rec + 16); };
   float m[kJoinParts / 32], l[kJoinParts / 32], M = -INFINITY, L = 0.0f;
 #pragma unroll
@@ -72,34 +69,82 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_kv_join(AttendParams p) {
 #pragma unroll
   for (int y = 0; y < 4; ++y) sums[warp][y * 32 + lane] = O[y];
   __syncthreads();
-  if (threadIdx.x == 0) write_lse(p, open.x, h, head, M + log2f(L));
+  // (the score blocks beside this one work the logarithm out for themselves)
+  if (threadIdx.x == 0 && p.lse && head >= 0) p.lse[head] = (M + log2f(L)) * 0.6931471805599453f;
   const int d = threadIdx.x;
   if (head >= 0 && d < D)
     ((T *)p.out)[head * D + d] = from_f32<T>(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / L);
 }
 
-// scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2):
-// one thread per entry, so the sum has one order and needs no atomics.
-__global__ void __launch_bounds__(256) k_kv_scores(AttendParams p) {
+// scores[b, hk, i] += sum over the query heads of kv head hk of 2^(raw - lse2),
+// for kScoreEntries entries: one thread per entry, so the sum has one order and
+// needs no atomics.  A row that k_kv_attend left in parts has its logarithms
+// worked out here from the parts' statistics, a head per warp in turn.
+constexpr int kScoreEntries = 256;
+__device__ __forceinline__ void add_scores(const AttendParams &p, int bk, int chunk) {
+  __shared__ float lse[kHeadsPerRow];
+  const int b = bk / p.c.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = min(p.c.length(b), p.max_len), first = chunk * kScoreEntries;
+  if (first >= n) return;
+  constexpr int PER = kScoreEntries / (kJoinWarps * 32);
+  float w[PER] = {};
+  bool lost = false;
+  for (int ch = 0; ch < p.chunks; ++ch) {
+    const int row = bk * p.chunks + ch, heads = min(kHeadsPerRow, p.group - ch * kHeadsPerRow);
+    const int2 at = p.row_parts[row];
+    for (int h = warp; h < heads; h += kJoinWarps) {
+      float y;
+      if (at.y == 0) {
+        y = p.lse2[(int64_t)row * kHeadsPerRow + h];
+      } else {
+        const int rec = kHeadsPerRow * p.c.dim;
+        const float *base = p.cta_rec + at.x * 2 * (rec + 16) + rec + h;
+        float M = -INFINITY, L = 0.0f;
+        for (int k = lane; k < at.y; k += 32) M = fmaxf(M, base[(k ? k * 2 : 1) * (rec + 16)]);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+        for (int k = lane; k < at.y; k += 32) {
+          const float *r = base + (k ? k * 2 : 1) * (rec + 16);
+          L = fmaf(r[8], ex2(r[0] - M), L);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
+        y = M + log2f(L);
+      }
+      if (lane == 0) lse[h] = y;
+    }
+    __syncthreads();
+    // (NaN: a page outside the pool, or a query that is not finite; the kv head keeps its scores)
+    for (int h = 0; h < heads; ++h) lost = lost || isnan(lse[h]);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = first + j * kJoinWarps * 32 + threadIdx.x;
+      if (i < n) {
+        const float *raw = p.raw + ((int64_t)row * p.max_len + i) * p.gp;
+        for (int h = 0; h < heads; h += 2) {
+          const float2 s = *reinterpret_cast<const float2 *>(raw + h);
+          w[j] += ex2(s.x - lse[h]);
+          if (h + 1 < heads) w[j] += ex2(s.y - lse[h + 1]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = first + j * kJoinWarps * 32 + threadIdx.x;
+    if (i < n && !lost) p.c.scores[(int64_t)bk * p.c.cap + i] += w[j];
+  }
+}
+
+// What is left after k_kv_attend: `joins` blocks join rows, the others add scores.
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) k_kv_finish(AttendParams p, int joins, int chunks) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int bk = blockIdx.y, b = bk / p.c.kv_heads;
-  const int n = min(p.c.length(b), p.max_len);
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float w = 0.0f;
-  for (int ch = 0; ch < p.chunks; ++ch) {
-    const int64_t row = (int64_t)bk * p.chunks + ch;
-    const float *raw = p.raw + (row * p.max_len + i) * p.gp;
-    const int heads = min(kHeadsPerRow, p.group - ch * kHeadsPerRow);
-    for (int h = 0; h < heads; h += 2) {
-      const float2 s = *reinterpret_cast<const float2 *>(raw + h);
-      w += ex2(s.x - p.lse2[row * kHeadsPerRow + h]);
-      if (h + 1 < heads) w += ex2(s.y - p.lse2[row * kHeadsPerRow + h + 1]);
-    }
-  }
-  // a sequence with a page outside the pool has NaN for all its sums and keeps its scores
-  if (!isnan(p.lse2[(int64_t)bk * p.chunks * kHeadsPerRow])) p.c.scores[(int64_t)bk * p.c.cap + i] += w;
+  const int i = blockIdx.x;
+  if (i < joins) join_row<T>(p, i / kHeadsPerRow, i % kHeadsPerRow);
+  else add_scores(p, (i - joins) / chunks, (i - joins) % chunks);
 }
 
 // CTAs of the main kernel: one per SM.
@@ -110,7 +155,7 @@ int attend_grid() {
 
 // Workspace layout; every part starts on 256 bytes.
 struct Layout {
-  size_t warp_rec, cta_rec, cta_row, lse2, raw, bytes;
+  size_t warp_rec, cta_rec, cta_row, lse2, row_parts, raw, bytes;
 };
 Layout layout_of(const KvView &c, int heads, int max_len, bool accumulate, int grid) {
   const int group = heads / c.kv_heads, chunks = (group + kHeadsPerRow - 1) / kHeadsPerRow;
@@ -122,7 +167,8 @@ Layout layout_of(const KvView &c, int heads, int max_len, bool accumulate, int g
   l.cta_rec = up((size_t)grid * kMaxWarps * rec * 4);
   l.cta_row = l.cta_rec + up((size_t)grid * 2 * (rec + 16) * 4);
   l.lse2 = l.cta_row + up((size_t)grid * sizeof(int2));
-  l.raw = l.lse2 + (accumulate ? up(rows * kHeadsPerRow * 4) : 0);
+  l.row_parts = l.lse2 + (accumulate ? up(rows * kHeadsPerRow * 4) : 0);
+  l.raw = l.row_parts + (accumulate ? up(rows * sizeof(int2)) : 0);
   l.bytes = l.raw + (accumulate ? up((size_t)rows * max_len * raw_heads(group) * 4) : 0);
   return l;
 }
@@ -137,7 +183,8 @@ int attend_check(const bp_kv_cache *cache, int layer, int heads, int max_length,
   if (accumulate && !cache->scores) return set_error(kEInval, "%s: the cache keeps no scores", what);
   *max_len = max_length && max_length < c->cap ? max_length : c->cap;
   const int64_t rows = (int64_t)cache->batch * cache->kv_heads * ((heads / cache->kv_heads + 7) / 8);
-  if (rows * ((*max_len + 15) / 16) > 0x7FFFFFFF || (accumulate && cache->batch * (int64_t)cache->kv_heads > 65535))
+  if (rows * ((*max_len + 15) / 16) > 0x7FFFFFFF ||
+      (accumulate && (int64_t)cache->batch * cache->kv_heads * ((*max_len + 255) / 256) > 0x7FFF0000))
     return set_error(kERange, "%s: more work than the call can number", what);
   return kOk;
 }
@@ -195,19 +242,21 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   p.cta_rec = (float *)(base + l.cta_rec);
   p.cta_row = (int2 *)(base + l.cta_row);
   p.lse2 = accumulate ? (float *)(base + l.lse2) : nullptr;
+  p.row_parts = accumulate ? (int2 *)(base + l.row_parts) : nullptr;
   p.raw = accumulate ? (float *)(base + l.raw) : nullptr;
   p.gp = raw_heads(p.group);
   rc = p.c.fmt == 8 ? launch_kv_attend8(p, dtype, grid, s) : launch_kv_attend16(p, dtype, grid, s);
   // (a batch of at most kMinUnits units is one CTA's, and no row of it is in parts)
   const int64_t units = (int64_t)cache->batch * cache->kv_heads * p.chunks * ((p.max_len + 15) / 16);
-  if (rc == kOk && units > kMinUnits) {
-    if (dtype == BP_F32) rc = launch_early(k_kv_join<float>, dim3(grid, kHeadsPerRow), kJoinWarps * 32, 0, p, s, "k_kv_join");
-    else if (dtype == BP_BF16) rc = launch_early(k_kv_join<__nv_bfloat16>, dim3(grid, kHeadsPerRow), kJoinWarps * 32, 0, p, s, "k_kv_join");
-    else rc = launch_early(k_kv_join<__half>, dim3(grid, kHeadsPerRow), kJoinWarps * 32, 0, p, s, "k_kv_join");
+  const int joins = units > kMinUnits ? grid * kHeadsPerRow : 0;
+  const int chunks = accumulate ? (p.max_len + kScoreEntries - 1) / kScoreEntries : 0;
+  const int64_t blocks = joins + (int64_t)chunks * cache->batch * cache->kv_heads;
+  if (rc == kOk && blocks) {
+    const dim3 g((unsigned)blocks);
+    const auto kernel = dtype == BP_F32 ? k_kv_finish<float>
+                                        : (dtype == BP_BF16 ? k_kv_finish<__nv_bfloat16> : k_kv_finish<__half>);
+    rc = launch_early(kernel, g, kJoinWarps * 32, 0, s, "k_kv_finish", p, joins, chunks);
   }
-  if (rc == kOk && accumulate && p.max_len)
-    rc = launch_early(k_kv_scores, dim3((p.max_len + 255) / 256, cache->batch * cache->kv_heads), 256, 0, p, s,
-                      "k_kv_scores");
   if (!workspace) {
     cudaError_t f = cudaFreeAsync(ws, s);
     if (rc == kOk && f != cudaSuccess) rc = set_error(kECuda, "%s: workspace free: %s", what, cudaGetErrorString(f));

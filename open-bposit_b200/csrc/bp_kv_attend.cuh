@@ -41,7 +41,7 @@
 // the other way round.  Rows lie in the stage with their 16-byte pieces permuted
 // (Swizzle) so that no fragment load has bank conflicts.  A row that lies within
 // one warp's range is finished by that warp; parts of a row are joined first
-// over the CTA's warps in shared memory, then over CTAs by k_kv_join.
+// over the CTA's warps in shared memory, then over CTAs by k_kv_finish.
 #pragma once
 #include <math.h>
 
@@ -67,11 +67,12 @@ struct AttendParams {
   float *cta_rec;            // [CTA][2][8 D + 16]: o, m, l of rows that cross CTAs
   int2 *cta_row;             // [CTA]: {row that starts here and goes on behind it, or -1; CTAs that share it}
   float *lse2;               // [rows][8], base 2; null unless scores are accumulated
+  int2 *row_parts;           // [rows]: {first CTA, parts} of a row that crosses CTAs, {-, 0}: its lse2 is there; or null
   float *raw;                // [rows][max_len][gp] scores, base 2; null unless accumulated
   int gp;                    // heads kept per entry in raw (even)
 };
 
-constexpr int kMaxWarps = 16;
+constexpr int kMaxWarps = 8;                        // warps of a CTA
 constexpr int kMaxBatch = 2048;
 constexpr int kTableAt = 65536;                     // shared address of the bp8 decode table
 constexpr int kSharedReserved = 1024;               // shared address where a block's own memory starts
@@ -89,7 +90,7 @@ struct AttendCfg {
   // waiting for instructions, where single units take 48 us).
   static constexpr bool WIDE = FMT == 16 && D > 64;
   static constexpr int TT = FMT == 8 ? (D <= 64 ? 64 : 32) : (D <= 32 ? 64 : (D <= 64 ? 32 : 16));
-    static constexpr int NW = 8;
+    static constexpr int NW = kMaxWarps;
   static constexpr int PARTS = WIDE ? 2 : 1;
   static constexpr int TILEB = TT * ROWB;
   // 2^exponent of a tile's keys and values as fp32, [t][n][2] in the order that thread t of a quad needs them, with
@@ -258,7 +259,10 @@ __device__ __forceinline__ int64_t head_of(const AttendParams &p, const RowId &r
   return g < p.group ? (int64_t)r.b * p.heads + r.hk * p.group + g : -1;
 }
 __device__ __forceinline__ void write_lse(const AttendParams &p, int row, int h, int64_t head, float lse2) {
-  if (p.lse2) p.lse2[(int64_t)row * kHeadsPerRow + h] = lse2;
+  if (p.lse2) {
+    p.lse2[(int64_t)row * kHeadsPerRow + h] = lse2;
+    if (h == 0) p.row_parts[row] = make_int2(0, 0);
+  }
   if (p.lse && head >= 0) p.lse[head] = lse2 * 0.6931471805599453f;
 }
 
@@ -774,7 +778,10 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     const int nu = units_of(lens(id.b));
     const int x0 = before(id.b) + (row - id.b * per_seq) * nu, x1 = x0 + nu;
     // (the CTA that holds the row's last unit is the last one with a part)
-    if (x0 >= lo && x1 > hi) open = make_int2(row, deal.part_of(x1 - 1) - cta + 1);
+    if (x0 >= lo && x1 > hi) {
+      open = make_int2(row, deal.part_of(x1 - 1) - cta + 1);
+      if (p.row_parts && tid == 0) p.row_parts[row] = make_int2(cta, open.y);
+    }
     if (h >= kHeadsPerRow) continue;
     const float mp = in ? rec_ml[lane * 16 + h] : -INFINITY;
     float M = mp;
@@ -839,7 +846,7 @@ int launch_kv_attend_one(const AttendParams &p, int grid, cudaStream_t s) {
     return set_error(kENoDev, "k_kv_attend: shared memory starts at %d, not %d", reserved, kSharedReserved);
   cudaError_t e = cudaFuncSetAttribute(k_kv_attend<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return set_error(kECuda, "k_kv_attend: %s", cudaGetErrorString(e));
-  return launch_early(k_kv_attend<FMT, D, T>, dim3(grid), C::NW * 32, C::SMEM, p, s, "k_kv_attend");
+  return launch_early(k_kv_attend<FMT, D, T>, dim3(grid), C::NW * 32, C::SMEM, s, "k_kv_attend", p);
 }
 template <int FMT, typename T>
 int launch_kv_attend_dim(const AttendParams &p, int grid, cudaStream_t s) {

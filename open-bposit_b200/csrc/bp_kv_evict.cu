@@ -421,9 +421,9 @@ extern "C" int bp_kv_evict(const bp_kv_cache *cache, const float *weights, int b
   // the smallest block that holds a row's weights in registers, 4 a thread while that is enough threads; longer rows
   // stream them
   static const char *const name = "k_kv_evict";
-  if (p.c.cap <= 256 * 4) return launch_early(k_kv_evict_row<256, 4>, grid, 256, 0, p, s, name);
-  if (p.c.cap <= 512 * 4) return launch_early(k_kv_evict_row<512, 4>, grid, 512, 0, p, s, name);
-  if (p.c.cap <= 512 * 16) return launch_early(k_kv_evict_row<512, 16>, grid, 512, 0, p, s, name);
-  if (p.c.cap <= 1024 * 16) return launch_early(k_kv_evict_row<1024, 16>, grid, 1024, 0, p, s, name);
-  return launch_early(k_kv_evict_long, grid, kThreads, 0, p, s, name);
+  if (p.c.cap <= 256 * 4) return launch_early(k_kv_evict_row<256, 4>, grid, 256, 0, s, name, p);
+  if (p.c.cap <= 512 * 4) return launch_early(k_kv_evict_row<512, 4>, grid, 512, 0, s, name, p);
+  if (p.c.cap <= 512 * 16) return launch_early(k_kv_evict_row<512, 16>, grid, 512, 0, s, name, p);
+  if (p.c.cap <= 1024 * 16) return launch_early(k_kv_evict_row<1024, 16>, grid, 1024, 0, s, name, p);
+  return launch_early(k_kv_evict_long, grid, kThreads, 0, s, name, p);
 }

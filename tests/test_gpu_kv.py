@@ -178,6 +178,19 @@ def test_non_finite_queries_give_nan_and_touch_no_other_head(orc):
     assert got[hit].isnan().all() and torch.equal(got[~hit], good[~hit])
 
 
+@pytest.mark.parametrize("length", [20, 3000])
+def test_scores_of_a_kv_head_with_a_nan_query_stay(orc, length):
+    from bposit_b200 import ops
+    cache = make(2, 2, 64, [length, 50], "bp8", 16, track=True)
+    q = queries(2, 8, 64)
+    q[0, 6, 1] = float("nan")                       # kv head 1 of sequence 0
+    start = cache.scores.clone()
+    ops.paged_attention(cache, q, accumulate=True)
+    assert torch.equal(cache.scores[0, 0, 1], start[0, 0, 1])
+    assert cache.scores[0, 0, 0, :length].gt(start[0, 0, 0, :length]).any()
+    assert cache.scores[0, 1, :, :50].gt(start[0, 1, :, :50]).any() and cache.scores.isfinite().all()
+
+
 @pytest.mark.parametrize("fmt,heads,kv_heads,dim", [("bp8", 9, 3, 64), ("bp16", 4, 4, 32), ("bp8", 20, 2, 128)])
 def test_accumulated_weights(orc, fmt, heads, kv_heads, dim):
     from bposit_b200 import ops
