@@ -12,8 +12,10 @@ struct EvictParams {
   int32_t *keep;             // optional [layers, batch, kv_heads, budget]
 };
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;   // of the streaming form
+constexpr int kThreads = 1024, kWarps = kThreads / 32;  // of the streaming form
+constexpr int kBatch = 4;              // entries that one of its threads reads at once
 constexpr int kQueue = 2 * kThreads;   // places given up that wait for a mover
+constexpr int kBins = 2048;            // of a histogram of weights
 constexpr uint32_t kTop = 0xFF800000u; // order_key of +inf
 
 // Weights as unsigned integers of the same order: NaN lowest, -0 equal to +0.
@@ -22,6 +24,42 @@ __device__ __forceinline__ uint32_t order_key(float w, bool guarded) {
   if (w != w) return 0u;
   const uint32_t u = __float_as_uint(w + 0.0f);        // -0 + 0 = +0
   return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+// The bin of `hist`, from the top down, in which the count passes `need`:
+// found = {bin, entries in bins above it, entries in it}.
+template <int NT>
+__device__ __forceinline__ void find_bin(const int *hist, int need, int *warp_sum, uint32_t *found) {
+  constexpr int PER = kBins / NT;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int bin[PER], mine = 0;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    bin[q] = hist[kBins - 1 - (tid * PER + q)];
+    mine += bin[q];
+  }
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(~0u, incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int above = incl - mine + __reduce_add_sync(~0u, lane < warp ? warp_sum[lane] : 0);
+  if (above < need && above + mine >= need) {
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      if (above < need && above + bin[q] >= need) {
+        found[0] = kBins - 1 - (tid * PER + q);
+        found[1] = above;
+        found[2] = bin[q];
+        break;
+      }
+      above += bin[q];
+    }
+  }
+  __syncthreads();
 }
 
 struct Scan {
@@ -34,15 +72,10 @@ __device__ __forceinline__ int block_rank(bool flag, Scan &s, int *total) {
   const uint32_t mask = __ballot_sync(~0u, flag);
   if (lane == 0) s.warp_sum[warp] = __popc(mask);
   __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const int n = s.warp_sum[w];
-    before += w < warp ? n : 0;
-    all += n;
-  }
+  static_assert(kWarps == 32, "a warp's sum per lane");
+  const int n = s.warp_sum[lane], before = __reduce_add_sync(~0u, lane < warp ? n : 0);
+  *total = __reduce_add_sync(~0u, n);
   __syncthreads();
-  *total = all;
   return before + __popc(mask & ((1u << lane) - 1u));
 }
 
@@ -107,7 +140,7 @@ template <int NT, int KPT>
 __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int NW = NT / 32, BINS = 2048, PER = BINS / NT, E = NW * KPT;
+  constexpr int NW = NT / 32, E = NW * KPT;
   const KvView &c = p.c;
   const int r = blockIdx.x;
   const int hk = r % c.kv_heads, lb = r / c.kv_heads, b = lb % c.batch, layer = lb / c.batch;
@@ -118,7 +151,7 @@ __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
       for (int i = tid; i < M; i += NT) keep[i] = i < n ? i : -1;
     return;
   }
-  __shared__ int hist[BINS], count[E + 1], warp_sum[32];
+  __shared__ int hist[kBins], count[E + 1], warp_sum[32];
   __shared__ uint32_t red[3][32], found[3];
   __shared__ uint16_t src[NT * KPT / 2], dst[NT * KPT / 2];
   const float *w = p.weights + (int64_t)r * c.cap;
@@ -175,41 +208,13 @@ __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
     need = M - top;
     while (true) {
       const int shift = max(0, 32 - __clz(hi - lo) - 11);
-      for (int i = tid; i < BINS; i += NT) hist[i] = 0;
+      for (int i = tid; i < kBins; i += NT) hist[i] = 0;
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < KPT; ++j)
         if (in(j) && key[j] >= lo && key[j] <= hi) atomicAdd(&hist[(key[j] - lo) >> shift], 1);
       __syncthreads();
-      // counts from the top bin down; the thread that passes `need` names the bin
-      int bin[PER], mine = 0;
-#pragma unroll
-      for (int q = 0; q < PER; ++q) {
-        bin[q] = hist[BINS - 1 - (tid * PER + q)];
-        mine += bin[q];
-      }
-      int incl = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(~0u, incl, d);
-        if (lane >= d) incl += y;
-      }
-      if (lane == 31) warp_sum[warp] = incl;
-      __syncthreads();
-      int above = incl - mine + __reduce_add_sync(~0u, lane < warp ? warp_sum[lane] : 0);
-      if (above < need && above + mine >= need) {
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-          if (above < need && above + bin[q] >= need) {
-            found[0] = BINS - 1 - (tid * PER + q);
-            found[1] = above;
-            found[2] = bin[q];
-            break;
-          }
-          above += bin[q];
-        }
-      }
-      __syncthreads();
+      find_bin<NT>(hist, need, warp_sum, found);
       need -= (int)found[1];
       const int held = (int)found[2];
       const uint32_t width = (1u << shift) - 1u;
@@ -284,7 +289,7 @@ __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
 }
 
 // The same for rows that do not fit a block's registers: the weights are read
-// once per pass.  A radix select over the ordered weights (8 bits a pass) finds
+// once per pass.  A radix select over the ordered weights (11, 11 and 10 bits) finds
 // the budget-th largest.  Then two scans run towards each other's ends: the front
 // scan (places < budget) queues the places given up, the back scan (places >=
 // budget) moves its kept entries into them, both in order, so that a chunk's
@@ -306,46 +311,53 @@ __global__ void __launch_bounds__(kThreads) k_kv_evict_long(EvictParams p) {
     return;
   }
   __shared__ Scan scan;
-  __shared__ int hist[256], s_bin, s_above, s_front;
+  __shared__ int hist[kBins], warp_sum[kWarps], s_front;
+  __shared__ uint32_t found[3];
   __shared__ int32_t queue[kQueue], src[kThreads], dst[kThreads];
-  __shared__ int newest_w[kWarps];
   const float *w = p.weights + r * c.cap;
   const int32_t *pos = c.positions + r * c.cap;
 
   int newest = INT_MIN;
+#pragma unroll 4
   for (int i = tid; i < n; i += kThreads) newest = max(newest, pos[i]);
   newest = __reduce_max_sync(~0u, newest);
-  if ((tid & 31) == 0) newest_w[tid >> 5] = newest;
+  if ((tid & 31) == 0) warp_sum[tid >> 5] = newest;
   __syncthreads();
-  for (int i = 0; i < kWarps; ++i) newest = max(newest, newest_w[i]);
+  newest = __reduce_max_sync(~0u, warp_sum[tid & 31]);
   const long long guard = (long long)newest - p.recent;
   auto key_of = [&](int i) { return order_key(w[i], pos[i] < p.sinks || pos[i] > guard); };
+  // each(i, key) for this thread's entries below `end`, kBatch loads in flight
+  auto for_keys = [&](int end, auto each) {
+    for (int i = tid; i < end; i += kBatch * kThreads) {
+      uint32_t k[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) k[j] = i + j * kThreads < end ? key_of(i + j * kThreads) : 0u;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i + j * kThreads < end) each(k[j]);
+    }
+  };
 
   uint32_t prefix = 0;
   int need = M;              // how many of the entries that match the prefix so far are kept
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+  for (int shift = 21; shift >= 0; shift = shift > 10 ? shift - 11 : shift - 10) {
+    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-      const uint32_t k = key_of(i);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
-    }
+    const int width = shift ? 11 : 10;
+    const uint32_t above = shift == 21 ? 0u : ~0u << (shift + width), bins = (1u << width) - 1u;
+    for_keys(n, [&](uint32_t k) {
+      if (((k ^ prefix) & above) == 0) atomicAdd(&hist[(k >> shift) & bins], 1);
+    });
     __syncthreads();
-    if (tid == 0) {
-      int above = 0, bin = 255;
-      while (bin > 0 && above + hist[bin] < need) above += hist[bin--];
-      s_bin = bin;
-      s_above = above;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)s_bin << shift;
-    need -= s_above;
+    find_bin<kThreads>(hist, need, warp_sum, found);
+    prefix |= found[0] << shift;
+    need -= (int)found[1];
   }
   // entries with key == prefix before place M
   if (tid == 0) s_front = 0;
   __syncthreads();
   int mine = 0;
-  for (int i = tid; i < M; i += kThreads) mine += key_of(i) == prefix;
+  for_keys(M, [&](uint32_t k) { mine += k == prefix; });
   if (mine) atomicAdd(&s_front, mine);
   __syncthreads();
 
@@ -418,8 +430,10 @@ extern "C" int bp_kv_evict(const bp_kv_cache *cache, const float *weights, int b
   p.budget = budget; p.recent = recent; p.sinks = sinks; p.keep = keep;
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)rows);
-  // the smallest block that holds a row's weights in registers, 4 a thread while that is enough threads; longer rows
-  // stream them
+  // The smallest block that holds a row's weights in its registers; longer rows stream them.  us for 384 rows (one row)
+  // of 64-wide bp8 heads cut by half, at each limit and in the next larger form:
+  //   1024: 4.1 (2.8) and 7.4 (3.5)     2048: 7.8 (3.7) and 15.5 (6.6)     8192: 19.3 (7.1) and 34.9 (11.0)
+  //   16384: 36.8 (11.4) and 89.8 (28.2); streamed, 32768: 202 (52)
   static const char *const name = "k_kv_evict";
   if (p.c.cap <= 256 * 4) return launch_early(k_kv_evict_row<256, 4>, grid, 256, 0, s, name, p);
   if (p.c.cap <= 512 * 4) return launch_early(k_kv_evict_row<512, 4>, grid, 512, 0, s, name, p);

@@ -211,6 +211,25 @@ def test_accumulated_weights(orc, fmt, heads, kv_heads, dim):
                 assert (got[:n] - want).abs().le(tol).all()
 
 
+@pytest.mark.parametrize("fmt,heads,kv_heads,dim,dtype", [
+    ("bp8", 14, 2, 64, torch.float32), ("bp8", 3, 3, 96, torch.bfloat16), ("bp16", 12, 1, 128, torch.float32),
+    ("bp16", 8, 4, 32, torch.float16), ("bp8", 17, 1, 32, torch.float32), ("bp16", 2, 2, 96, torch.float32)])
+def test_accumulated_weights_of_long_rows(orc, fmt, heads, kv_heads, dim, dtype):
+    """Rows that are split over several blocks, one that is not, and an empty one."""
+    lens = [5003, 0, 777, 31]
+    cache = make(4, kv_heads, dim, lens, fmt, 64, track=True)
+    start = cache.scores.clone()
+    weights = check_attention(orc, cache, queries(4, heads, dim, dtype), accumulate=True)
+    for b, n in enumerate(lens):
+        for hk in range(kv_heads):
+            got, was = cache.scores[0, b, hk].double().cpu(), start[0, b, hk].double().cpu()
+            assert torch.equal(got[n:], was[n:])
+            if n:
+                want = was[:n] + weights[b, hk]
+                tol = weights[b, hk, "bound"] + (heads // kv_heads + 1) * 2.0 ** -24 * want.abs()
+                assert (got[:n] - want).abs().le(tol).all()
+
+
 def test_attention_results_repeat_bit_for_bit(orc):
     from bposit_b200 import ops
     cache = make(6, 2, 64, [2000, 3, 700, 0, 64, 1234], "bp8", 64, track=True)
@@ -295,6 +314,13 @@ def test_append_is_exact(orc, fmt, dim, heads, kv_heads, dtype, tokens):
     cache.positions[1][b, :, i] = was[2][1][b, :, i]
     cache.scores[1][b, :, i] = was[3][1][b, :, i]
     assert torch.equal(cache.positions, was[2]) and torch.equal(cache.scores, was[3])
+
+
+@pytest.mark.parametrize("fmt", ["bp8", "bp16"])
+@pytest.mark.parametrize("dim,heads,kv_heads,dtype", [(64, 14, 2, torch.bfloat16), (32, 20, 1, torch.float16),
+                                                      (96, 8, 1, torch.float32), (128, 9, 1, torch.float32)])
+def test_append_of_many_tokens(orc, fmt, dim, heads, kv_heads, dtype):
+    test_append_is_exact(orc, fmt, dim, heads, kv_heads, dtype, 2999)
 
 
 @pytest.mark.parametrize("fmt", ["bp8", "bp16"])
@@ -398,6 +424,19 @@ def test_evict_with_more_guarded_entries_than_the_budget():
     check_evict(cache, 30, 0, 0)
     cache.positions.fill_((1 << 31) - 1)
     check_evict(cache, 20, (1 << 31) - 1, (1 << 31) - 1)
+
+
+@pytest.mark.parametrize("length,budget", [(1024, 1000), (1025, 512), (2048, 3), (2049, 1024), (5000, 4096), (8192, 4096),
+                                           (8193, 8192), (16384, 5000), (16385, 8192), (20001, 20000), (33000, 1)])
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+def test_evict_at_every_capacity(length, budget, kind):
+    cache = make(2, 1, 32, [length, budget], "bp8", 16, track=True, seed=length, per=-(-length // 16))
+    if kind == "ties":
+        g = torch.Generator(device="cuda").manual_seed(budget)
+        w = torch.randint(-2, 3, cache.scores.shape, generator=g, device="cuda").float() / 4
+        w[..., 5::11], w[..., 6::13], w[..., 7::17] = math.nan, -0.0, math.inf
+        cache.scores.copy_(w)
+    check_evict(cache, budget, min(40, length // 30), 3)
 
 
 def test_evict_long_rows_and_own_scores():
