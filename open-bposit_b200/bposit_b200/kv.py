@@ -35,6 +35,9 @@ class _Struct(ctypes.Structure):
                                                "scores")]
 
 
+_TENSORS = ("k", "v", "k_exp", "v_exp", "page_table", "lengths", "positions", "scores")
+
+
 class PagedKVCache:
     """See the module docstring.  ``max_tokens`` is each sequence's capacity,
     rounded up to whole pages; every sequence gets its own pages."""
@@ -66,7 +69,9 @@ class PagedKVCache:
         page_size, head_dim] uint8 (bp8, with k_exp, v_exp [layers, pages,
         kv_heads, page_size] int8) or uint16 (bp16); page_table [batch,
         max_pages] and lengths [batch] int32; positions int32 and scores float32
-        [layers, batch, kv_heads, max_pages * page_size].  Nothing is copied."""
+        [layers, batch, kv_heads, max_pages * page_size].  Nothing is copied.
+        ``longest``, the host's bound of the lengths, starts at the capacity: set
+        it to what the lengths really are before the first ``advance``."""
         c = cls.__new__(cls)
         if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
             raise ValueError("lengths must be a [batch] int32 tensor")
@@ -121,6 +126,12 @@ class PagedKVCache:
         self._ref = ctypes.byref(self._struct)
         self._workspace = {}     # bytes that paged_attention needs, by its arguments
 
+    def __setattr__(self, name, value):
+        # the kernels are given the addresses of the tensors that the cache was made of
+        if name in _TENSORS and name in self.__dict__:
+            raise AttributeError(f"write into {name} in place, or make another cache over the tensors")
+        super().__setattr__(name, value)
+
     def advance(self, n=1, most: int | None = None):
         """Make room for n more entries in every sequence (an int), or for n[b]
         in sequence b (an int32 tensor of which no value is above `most`); they
@@ -128,7 +139,10 @@ class PagedKVCache:
         the host as a bound of all lengths."""
         if not isinstance(n, int) and most is None:
             raise ValueError("give `most`, a bound of the counts that the host knows")
-        longest = self.longest + (n if isinstance(n, int) else int(most))
+        more = n if isinstance(n, int) else int(most)
+        if more < 0:
+            raise ValueError("counts of new entries are not negative")
+        longest = self.longest + more
         if longest > self.capacity:
             raise ValueError(f"{longest} entries do not fit a capacity of {self.capacity}")
         (self.lengths if self._counts is None else self._counts).add_(n)

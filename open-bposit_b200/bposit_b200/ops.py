@@ -467,13 +467,14 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=Non
     k = _act(k, "k", None, cache.kv_heads, cache)
     dt = k.dtype
     n = k.shape[0]
-    if v.dtype != dt or v.shape != k.shape or v.stride() != k.stride() or v.device != cache.device or v.data_ptr() & 15:
+    if not isinstance(v, torch.Tensor) or v.dtype != dt or v.shape != k.shape or v.stride() != k.stride() or \
+            v.device != cache.device or v.data_ptr() & 15:
         v = _act(v, "v", n, cache.kv_heads, cache, dt)
     rows = heads = qs = 0
     cp = sp = qp = op = None
     if cos is not None or sin is not None:
-        if cos is None or sin is None:
-            raise ValueError("cos and sin come together")
+        if not isinstance(cos, torch.Tensor) or not isinstance(sin, torch.Tensor):
+            raise ValueError("cos and sin are tensors and come together")
         shape = cos.shape
         if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or sin.shape != shape or \
                 shape[1] * 2 != cache.head_dim or cos.device != cache.device or sin.device != cache.device or \
@@ -488,6 +489,8 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=Non
         heads, qs, qp, op = q.shape[1], q.stride(0), q.data_ptr(), q_out.data_ptr()
     if (places is None) != (seqs is None):
         raise ValueError("seqs and places come together")
+    if not 0 <= layer < cache.layers:
+        raise ValueError(f"layer {layer} of {cache.layers}")
     if places is None and n != cache.batch:
         raise ValueError(f"{n} tokens for {cache.batch} sequences: give seqs and places")
     _call(_lib.lib().bp_kv_append, cache.device, cache._ref, layer, _ACT[dt], n, k.data_ptr(), k.stride(0),
@@ -518,6 +521,10 @@ def paged_attention(cache, q: torch.Tensor, layer: int = 0, scale: float | None 
         max_length = 0
     elif max_length < 1:
         raise ValueError("max_length must be positive")
+    elif max_length >= cache.capacity:
+        max_length = 0
+    if not 0 <= layer < cache.layers:
+        raise ValueError(f"layer {layer} of {cache.layers}")
     L = _lib.lib()
     need = cache._workspace.get((heads, max_length, accumulate))
     if need is None:
@@ -548,6 +555,8 @@ def kv_evict(cache, budget: int, recent: int = 0, sinks: int = 0, weights=None) 
         raise ValueError(f"weights must be a contiguous float32 CUDA tensor {list(cache.positions.shape)}")
     if budget < 1 or recent < 0 or sinks < 0:
         raise ValueError("budget must be positive, recent and sinks not negative")
+    if max(budget, recent, sinks) > 0x7FFFFFFF:
+        raise ValueError("budget, recent and sinks are 32-bit numbers")
     keep = torch.empty((cache.layers, cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
     _call(_lib.lib().bp_kv_evict, cache.device, cache._ref, None if weights is None else weights.data_ptr(), budget,
           recent, sinks, keep.data_ptr())

@@ -301,7 +301,7 @@ extern "C" int bp_kv_append(const bp_kv_cache *cache, int layer, int dtype, int 
   if (dtype < BP_F32 || dtype > BP_F16) return set_error(kEFmt, "%s: unknown dtype %d", what, dtype);
   if (tokens < 0 || (q && heads < 1) || heads > 65536) return set_error(kEInval, "%s: bad token or head count", what);
   if (!seqs != !places) return set_error(kEInval, "%s: seqs and places come together", what);
-  if (!places && tokens != cache->batch)
+  if (!places && tokens && tokens != cache->batch)   // (no tokens: the lists are null too)
     return set_error(kEInval, "%s: %d tokens for %d sequences (give seqs and places)", what, tokens, cache->batch);
   if (!cos != !sin || (cos && rope_rows < 1) || (q && !cos))
     return set_error(kEInval, "%s: q and the rotation need both tables", what);

@@ -183,7 +183,7 @@ int attend_check(const bp_kv_cache *cache, int layer, int heads, int max_length,
   if (accumulate && !cache->scores) return set_error(kEInval, "%s: the cache keeps no scores", what);
   *max_len = max_length && max_length < c->cap ? max_length : c->cap;
   const int64_t rows = (int64_t)cache->batch * cache->kv_heads * ((heads / cache->kv_heads + 7) / 8);
-  if (rows * ((*max_len + 15) / 16) > 0x7FFFFFFF ||
+  if (rows * ((*max_len + 15) / 16) > 0x7FFFFF00 ||
       (accumulate && (int64_t)cache->batch * cache->kv_heads * ((*max_len + 255) / 256) > 0x7FFF0000))
     return set_error(kERange, "%s: more work than the call can number", what);
   return kOk;

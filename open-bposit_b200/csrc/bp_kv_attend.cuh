@@ -90,7 +90,7 @@ struct AttendCfg {
   // waiting for instructions, where single units take 48 us).
   static constexpr bool WIDE = FMT == 16 && D > 64;
   static constexpr int TT = FMT == 8 ? (D <= 64 ? 64 : 32) : (D <= 32 ? 64 : (D <= 64 ? 32 : 16));
-    static constexpr int NW = kMaxWarps;
+  static constexpr int NW = kMaxWarps;
   static constexpr int PARTS = WIDE ? 2 : 1;
   static constexpr int TILEB = TT * ROWB;
   // 2^exponent of a tile's keys and values as fp32, [t][n][2] in the order that thread t of a quad needs them, with

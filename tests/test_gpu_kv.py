@@ -179,6 +179,18 @@ def test_non_finite_queries_give_nan_and_touch_no_other_head(orc):
 
 
 @pytest.mark.parametrize("length", [20, 3000])
+def test_scores_behind_a_page_outside_the_pool_stay(orc, length):
+    from bposit_b200 import ops
+    cache = make(2, 2, 64, [length, 50], "bp8", 16, track=True)
+    q = queries(2, 8, 64)
+    good, start = ops.paged_attention(cache, q), cache.scores.clone()
+    cache.page_table[0, 0] = cache.pages
+    got = ops.paged_attention(cache, q, accumulate=True)
+    assert torch.equal(cache.scores[0, 0], start[0, 0]) and got[0].isnan().all() and torch.equal(got[1], good[1])
+    assert cache.scores[0, 1, :, :50].gt(start[0, 1, :, :50]).any() and cache.scores.isfinite().all()
+
+
+@pytest.mark.parametrize("length", [20, 3000])
 def test_scores_of_a_kv_head_with_a_nan_query_stay(orc, length):
     from bposit_b200 import ops
     cache = make(2, 2, 64, [length, 50], "bp8", 16, track=True)
@@ -242,6 +254,127 @@ def test_attention_results_repeat_bit_for_bit(orc):
     cache.scores.copy_(start)
     b = ops.paged_attention(cache, q, accumulate=True), cache.scores.clone()
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_results_may_replace_the_queries(orc, dtype):
+    from bposit_b200 import ops
+    cache = make(3, 2, 64, [4000, 5, 0], "bp8", 64)
+    q = queries(3, 14, 64, dtype)
+    want = ops.paged_attention(cache, q)
+    mine = q.clone()
+    assert ops.paged_attention(cache, mine, out=mine) is mine and torch.equal(mine, want)
+    for tokens in (3, 2600):
+        x = queries(tokens, 14, 64, dtype, seed=3)
+        k = queries(tokens, 2, 64, dtype, seed=4)
+        cos = torch.rand(4000, 32, device="cuda")
+        at = torch.arange(tokens, device="cuda", dtype=torch.int32)
+        args = dict(cos=cos, sin=1 - cos, seqs=torch.zeros_like(at), places=at)
+        want = ops.kv_append(cache, k, k, q=x, **args)
+        mine = x.clone()
+        assert ops.kv_append(cache, k, k, q=mine, q_out=mine, **args) is mine and torch.equal(mine, want)
+
+
+def test_calls_with_nothing_to_do(orc):
+    from bposit_b200 import ops
+    cache = make(3, 2, 64, [0, 0, 0], "bp8", 16, track=True, per=2)
+    out, lse = ops.paged_attention(cache, queries(3, 4, 64), accumulate=True, return_lse=True)
+    assert not out.any() and lse.eq(-math.inf).all()
+    was = cache.k.clone(), cache.scores.clone()
+    none = torch.zeros(0, device="cuda", dtype=torch.int32)
+    cos = torch.rand(8, 32, device="cuda")
+    q = ops.kv_append(cache, queries(0, 2, 64), queries(0, 2, 64), q=queries(0, 4, 64), cos=cos, sin=cos, seqs=none,
+                      places=none)
+    assert q.shape == (0, 4, 64)
+    assert ops.kv_evict(cache, 3).eq(-1).all()
+    assert torch.equal(cache.k, was[0]) and torch.equal(cache.scores, was[1])
+
+
+def test_calls_on_two_streams_at_once_and_in_one_graph(orc):
+    """Two caches whose calls run beside each other, eagerly, from two threads, and as branches of a graph."""
+    import threading
+    from bposit_b200 import ops
+
+    def world(seed):
+        cache = make(2, 2, 64, [2100, 60], "bp8", 64, track=True, seed=seed)
+        x = [queries(2, n, 64, seed=seed + i) for i, n in enumerate((14, 2, 2))]
+        cos = torch.rand(3000, 32, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+
+        def step():
+            q = ops.kv_append(cache, x[1], x[2], q=x[0], cos=cos, sin=1 - cos)
+            out = ops.paged_attention(cache, q, accumulate=True)
+            return out, ops.kv_evict(cache, 1500, recent=10, sinks=2)
+        return cache, step
+
+    def state(cache):
+        return [t.clone() for t in (cache.k, cache.k_exp, cache.v, cache.positions, cache.scores)]
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    want = []
+    for seed in (10, 20):
+        cache, step = world(seed)
+        want.append([t.clone() for _ in range(3) for t in step()] + state(cache))
+    torch.cuda.synchronize()
+    for how in ("eager", "threads", "graph"):
+        worlds = [world(10), world(20)]
+        got = [[], []]
+        torch.cuda.synchronize()
+
+        def run(i, times=3):
+            with torch.cuda.stream(streams[i]):
+                for _ in range(times):
+                    got[i] += [t.clone() for t in worlds[i][1]()]
+        if how == "eager":
+            for i in range(2):
+                run(i)
+        elif how == "threads":
+            threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+        else:
+            graph, main, results = torch.cuda.CUDAGraph(), torch.cuda.Stream(), [None, None]
+            with torch.cuda.graph(graph, stream=main):
+                for i in range(2):
+                    streams[i].wait_stream(main)
+                    with torch.cuda.stream(streams[i]):
+                        results[i] = worlds[i][1]()
+                for s in streams:
+                    main.wait_stream(s)
+            for _ in range(3):
+                graph.replay()
+                torch.cuda.synchronize()
+                for i in range(2):
+                    got[i] += [t.clone() for t in results[i]]
+        torch.cuda.synchronize()
+        for i in range(2):
+            for a, b in zip(got[i] + state(worlds[i][0]), want[i], strict=True):
+                assert torch.equal(a, b), (how, i)
+
+
+def test_cache_tensors_are_written_in_place(orc):
+    from bposit_b200 import ops
+    from bposit_b200.kv import PagedKVCache
+    cache = PagedKVCache(2, 2, 64, 100, track=True)
+    with pytest.raises(AttributeError):
+        cache.page_table = cache.page_table.clone()
+    with pytest.raises(ValueError):
+        cache.advance(-1)
+    cache.advance(3)
+    q = queries(2, 4, 64)
+    for layer in (-1, 1, 1 << 32):
+        with pytest.raises(ValueError):
+            ops.paged_attention(cache, q, layer=layer)
+        with pytest.raises(ValueError):
+            ops.kv_append(cache, q[:, :2], q[:, 2:], layer=layer)
+    for kw in (dict(budget=1 << 32), dict(budget=2, recent=1 << 40), dict(budget=2, sinks=1 << 31)):
+        with pytest.raises(ValueError):
+            ops.kv_evict(cache, **kw)
+    assert torch.equal(ops.paged_attention(cache, q, max_length=(1 << 32) + 1), ops.paged_attention(cache, q))
+    for v, kw in ((None, {}), (q[:, 2:], dict(cos=1.0, sin=1.0))):
+        with pytest.raises(ValueError):
+            ops.kv_append(cache, q[:, :2], v, **kw)
 
 
 def test_sequences_may_share_pages(orc):

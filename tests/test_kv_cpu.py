@@ -163,6 +163,7 @@ def test_empty_calls_succeed_without_a_device():
     none = struct(batch=0)
     assert append(L, none, tokens=0) == 0 and attend(L, none) == 0 and evict(L, none) == 0
     assert append(L, struct(), tokens=0, seqs=16, places=16) == 0
+    assert append(L, struct(), tokens=0, q=None, heads=0) == 0
 
 
 # ---- the Python layer ----
