@@ -85,8 +85,9 @@ class DecoderLayer(torch.nn.Module):
         qkv = self.qkv(self.ln1(x)).view(B, nh + 2 * nkv, hd)
         q, k, v = qkv.split([nh, nkv, nkv], dim=1)
         q = ops.kv_append(cache, k, v, q=q, cos=cos, sin=sin, positions=positions, layer=layer)
-        a = ops.paged_attention(cache, q, layer=layer, max_length=cache.longest,
-                                accumulate=cache.scores is not None)
+        # (a captured step is replayed on longer sequences than the host knows of now)
+        bound = None if torch.cuda.is_current_stream_capturing() else cache.longest
+        a = ops.paged_attention(cache, q, layer=layer, max_length=bound, accumulate=cache.scores is not None)
         x = x + self.o(a.reshape(B, nh * hd))
         g, u = self.gate_up(self.ln2(x)).chunk(2, dim=-1)
         return x + self.down(F.silu(g) * u)
@@ -187,7 +188,8 @@ class QwenShaped(torch.nn.Module):
     def step(self, ids, cache, tables):
         """The next token of every sequence, ids [B]: its final hidden state
         [B, hidden], its keys and values appended to `cache`.  tables:
-        rope_tables of at least the tokens that the sequences will have seen."""
+        rope_tables of at least the tokens that the sequences will have seen.
+        May be captured into a graph: each replay is one step further."""
         cache.advance()
         positions = cache.seen - 1
         x = self.embed(ids)
@@ -210,6 +212,10 @@ class QwenShaped(torch.nn.Module):
         if new_tokens < 1:
             raise ValueError("new_tokens must be positive")
         B, S = ids.shape
+        if S < 1 or (lengths is not None and min(int(x) for x in lengths) < 1):
+            raise ValueError("prompts have at least one token")
+        if budget is not None and budget < 1:
+            raise ValueError("budget must be positive")
         cache = self.new_cache(B, S + new_tokens if budget is None else max(S, budget + page_size) + 1, fmt, page_size,
                                track=budget is not None)
         tables = self.rope_tables(S + new_tokens)

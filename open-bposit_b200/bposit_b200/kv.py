@@ -136,7 +136,8 @@ class PagedKVCache:
         """Make room for n more entries in every sequence (an int), or for n[b]
         in sequence b (an int32 tensor of which no value is above `most`); they
         are written by ``ops.kv_append`` in every layer.  ``longest`` follows on
-        the host as a bound of all lengths."""
+        the host as a bound of all lengths (not when a captured graph replays
+        this: then add to ``longest`` what the replays added)."""
         if not isinstance(n, int) and most is None:
             raise ValueError("give `most`, a bound of the counts that the host knows")
         more = n if isinstance(n, int) else int(most)

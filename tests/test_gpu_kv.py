@@ -594,3 +594,41 @@ def test_evict_with_a_page_outside_the_pool_writes_nothing_there():
     assert torch.equal(cache.k[0, t[0, 1]], old[0, t[0, 1]])   # sources on the missing page 5
     untouched = sorted(set(range(cache.pages)) - {int(t[1, 0]), int(t[1, 1])})
     assert torch.equal(cache.k[0, untouched], old[0, untouched])
+
+
+@pytest.mark.parametrize("fmt", ["bp8", "bp16"])
+def test_pools_of_more_than_4_gib(fmt):
+    """Rows behind 2^32 bytes of codes, in both layers, against a small cache with the same entries."""
+    from bposit_b200 import ops
+    from bposit_b200.kv import PagedKVCache
+    dim, page, heads = 128, 64, 2
+    small = make(2, heads, dim, [300, 130], fmt, page, layers=2, track=True)
+    pages = (1 << 32) // (heads * page * dim * (1 if fmt == "bp8" else 2)) // 2 + 50   # a layer: 2^31 bytes and more
+    shape = (2, pages, heads, page)
+    k, v = (torch.empty(shape + (dim,), dtype=small.k.dtype, device="cuda") for _ in range(2))
+    ke = ve = None
+    if fmt == "bp8":
+        ke, ve = (torch.empty(shape, dtype=torch.int8, device="cuda") for _ in range(2))
+    move = torch.arange(pages - small.pages, pages, dtype=torch.int32, device="cuda")
+    for x, y in ((k, small.k), (v, small.v), (ke, small.k_exp), (ve, small.v_exp)):
+        if x is not None:
+            x[:, -small.pages:] = y
+    big = PagedKVCache.over(k, v, move[small.page_table.long()], small.lengths.clone(), k_exp=ke, v_exp=ve,
+                            positions=small.positions.clone(), scores=small.scores.clone())
+    new = queries(2, 8, dim, seed=7)
+    cos = torch.rand(400, dim // 2, device="cuda")
+    results = []
+    for c in (small, big):
+        out = []
+        for layer in (0, 1):
+            q = ops.kv_append(c, new[:, :2], new[:, 2:4], q=new[:, 4:], cos=cos, sin=1 - cos, layer=layer)
+            out += [q, ops.paged_attention(c, q, layer=layer, accumulate=True)]
+        out.append(ops.kv_evict(c, 100, recent=20, sinks=2))
+        c.lengths.clamp_(max=100)
+        out += [ops.paged_attention(c, q, layer=layer) for layer in (0, 1)] + [c.positions, c.scores]
+        results.append(out)
+    for a, b in zip(*results, strict=True):
+        assert torch.equal(a, b)
+    for x, y in ((k, small.k), (v, small.v), (ke, small.k_exp), (ve, small.v_exp)):
+        if x is not None:
+            assert torch.equal(x[:, -small.pages:].view(torch.uint8), y.view(torch.uint8))

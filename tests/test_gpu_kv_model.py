@@ -84,8 +84,37 @@ def test_generate_with_and_without_a_budget():
     assert torch.equal(m.generate(ids, 6, page_size=16, budget=64), all_of_it)
     assert m.generate(ids, 30, page_size=16, budget=24, recent=8, sinks=2).shape == (3, 30)
     assert torch.equal(m.generate(ids, 6, lengths=[40, 40, 40], page_size=16), all_of_it)
-    with pytest.raises(ValueError):
-        m.generate(ids, 0)
+    for kw in (dict(new_tokens=0), dict(new_tokens=2, lengths=[3, 0, 1]), dict(new_tokens=2, budget=0)):
+        with pytest.raises(ValueError):
+            m.generate(ids, **kw)
+
+
+@pytest.mark.parametrize("track", [False, True])
+def test_a_captured_step_goes_on_with_every_replay(track):
+    m = small(2)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.randint(0, 500, (2, 30), generator=g, device="cuda")
+    tokens = torch.randint(0, 500, (6, 2), generator=g, device="cuda")
+    tables = m.rope_tables(64)
+    caches = [m.new_cache(2, 40, page_size=16, track=track) for _ in range(2)]
+    for c in caches:
+        m.prefill(ids, c, [30, 17])
+    want = [m.step(t, caches[0], tables) for t in tokens]
+    token = tokens[0].clone()
+    got = [m.step(token, caches[1], tables)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.step(token, caches[1], tables)
+    for t in tokens[1:]:
+        token.copy_(t)
+        graph.replay()
+        got.append(out.clone())
+    # the entries are the same; the split of the sums does not depend on max_length
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert caches[1].lengths.tolist() == [36, 23] and torch.equal(caches[0].k, caches[1].k)
+    if track:
+        assert torch.equal(caches[0].scores, caches[1].scores)
 
 
 def test_steps_and_evictions_keep_what_they_promise():
