@@ -89,16 +89,6 @@ __device__ __forceinline__ void store4(T *p, const float *x) {
   *reinterpret_cast<uint2 *>(p) = w;
 }
 
-// A warp works on rows of one token, either keys and values or queries (a row is
-// a head): a group of GW lanes takes a row, a lane four pairs (i, i + D/2) of it,
-// so that loads and stores are 16 bytes (fp32) and a row's maximum is a shuffle
-// within the group.  Keys are rotated in float64: both products are exact there,
-// so the result is the exact sum rounded to float64 and then to fp32 whatever
-// the order of evaluation, and the codes that are stored do not depend on it.
-// Queries are rotated in fp32 (a product and an fma): converting all their values
-// to float64 and back took the conversion unit longer than the memory needs for
-// them.  With many tokens a group takes U rows of queries at a time, all loaded
-// before the first is worked on.
 // Codes of eight values of a row (bp8: of x / 2^e), four to a word or two.
 __device__ __noinline__ void encode_any(const float *x, int e, int fmt, uint32_t *o) {
   for (int i = 0; i < 8; ++i) {
@@ -141,11 +131,26 @@ __device__ __forceinline__ void encode8(const float (&x)[8], int e, uint32_t (&o
   }
 }
 
+// Rows of keys or values that a group takes at a time, with U rows of queries: two where there are many tokens (16384
+// fp32 tokens of 32 and 8 heads of 128 into bp16: 122 us, 6.0 TB/s, against 133 with one; 20001 bf16 tokens of 9 and 3
+// heads of 64 into bp16: 26.3 against 28.0, where rotation and encoding take 60% of the issue slots).
+constexpr int kv_unroll(int U) { return U > 1 ? 2 : 1; }
+
+// A warp works on rows of one token, either keys and values or queries (a row is
+// a head): a group of GW lanes takes a row, a lane four pairs (i, i + D/2) of it,
+// so that loads and stores are 16 bytes (fp32) and a row's maximum is a shuffle
+// within the group.  Keys are rotated in float64: both products are exact there,
+// so the result is the exact sum rounded to float64 and then to fp32 whatever
+// the order of evaluation, and the codes that are stored do not depend on it.
+// Queries are rotated in fp32 (a product and an fma): converting all their values
+// to float64 and back took the conversion unit longer than the memory needs for
+// them.  With many tokens a group takes U rows of queries (two of keys or values)
+// at a time, all loaded before the first is worked on.
 template <typename T, int D, int FMT, int U>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW;
+  constexpr int GL = D / 8, GW = GL <= 4 ? 4 : (GL <= 8 ? 8 : 16), RPW = 32 / GW, KU = kv_unroll(U);
   const KvView &c = p.c;
   const int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, sub = lane & (GW - 1), grp = lane / GW;
@@ -161,30 +166,10 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
     place = c.length(t) - 1;
   }
   const int at = p.positions ? p.positions[t] : place;
-
-  float x[U][8];
-  const T *src;
-  const int r0 = chunk * (queries ? RPW * U : RPW) + grp;
-  if (queries) {
-    src = (const T *)p.q + t * p.qs + r0 * D + sub * 4;
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (on && r0 + i * RPW < p.heads) {
-        load4(src + i * RPW * D, x[i]);
-        load4(src + i * RPW * D + D / 2, x[i] + 4);
-      }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[0][i] = 0.0f;
-    src = r0 < c.kv_heads ? (const T *)p.k + t * p.ks + r0 * D : (const T *)p.v + t * p.vs + (r0 - c.kv_heads) * D;
-    if (on && r0 < kv_rows) {
-      load4(src + sub * 4, x[0]);
-      load4(src + sub * 4 + D / 2, x[0] + 4);
-    }
-  }
-  const bool key = r0 < c.kv_heads;
+  const int r0 = chunk * RPW * (queries ? U : KU) + grp;
+  const bool turn = p.cos && (queries || r0 < c.kv_heads);      // some row is rotated: r0 is, if any
   float cs[4], sn[4];
-  if (p.cos && (queries || key)) {
+  auto angles = [&]() {
     const bool known = (unsigned)at < (unsigned)p.rope_rows;
 #pragma unroll
     for (int i = 0; i < 4; ++i) cs[i] = sn[i] = NAN;
@@ -192,9 +177,18 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
       load4(p.cos + (int64_t)at * (D / 2) + sub * 4, cs);
       load4(p.sin + (int64_t)at * (D / 2) + sub * 4, sn);
     }
-  }
+  };
 
   if (queries) {
+    float x[U][8];
+    const T *src = (const T *)p.q + t * p.qs + r0 * D + sub * 4;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (on && r0 + i * RPW < p.heads) {
+        load4(src + i * RPW * D, x[i]);
+        load4(src + i * RPW * D + D / 2, x[i] + 4);
+      }
+    angles();
     T *dst = (T *)p.q_out + ((int64_t)t * p.heads + r0) * D + sub * 4;
 #pragma unroll
     for (int i = 0; i < U; ++i)
@@ -210,46 +204,64 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
       }
     return;
   }
-  if (key && p.cos) {
+  float x[KU][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double u = x[0][i], w = x[0][4 + i], cc = cs[i], ss = sn[i];
-      x[0][i] = (float)__fma_rn(u, cc, -__dmul_rn(w, ss));
-      x[0][4 + i] = (float)__fma_rn(w, cc, __dmul_rn(u, ss));
+  for (int k = 0; k < KU; ++k) {
+    const int r = r0 + k * RPW;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[k][i] = 0.0f;
+    const T *src = r < c.kv_heads ? (const T *)p.k + t * p.ks + r * D : (const T *)p.v + t * p.vs + (r - c.kv_heads) * D;
+    if (on && r < kv_rows) {
+      load4(src + sub * 4, x[k]);
+      load4(src + sub * 4 + D / 2, x[k] + 4);
     }
   }
-  int e = 0;
-  if (FMT == 8) {
-    uint32_t top = 0;
+  if (turn) angles();
+  const bool placed = on && (unsigned)b < (unsigned)c.batch && (unsigned)place < (unsigned)c.cap;
+  const int page = placed ? c.page_of(b, place) : -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t a = __float_as_uint(x[0][i]) & 0x7FFFFFFFu;
-      top = a < 0x7F800000u && a > top ? a : top;
+  for (int k = 0; k < KU; ++k) {
+    const int r = r0 + k * RPW;
+    const bool key = r < c.kv_heads;
+    if (key && p.cos) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const double u = x[k][i], w = x[k][4 + i], cc = cs[i], ss = sn[i];
+        x[k][i] = (float)__fma_rn(u, cc, -__dmul_rn(w, ss));
+        x[k][4 + i] = (float)__fma_rn(w, cc, __dmul_rn(u, ss));
+      }
     }
+    int e = 0;
+    if (FMT == 8) {
+      uint32_t top = 0;
 #pragma unroll
-    for (int d = GW / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
-    e = top ? max(f32_floor_log2(top) - 3, -126) : 0;
-  }
-  if (!on || r0 >= kv_rows || (unsigned)b >= (unsigned)c.batch || (unsigned)place >= (unsigned)c.cap) return;
-  const int page = c.page_of(b, place);
-  if (page < 0) return;
-  const int h = key ? r0 : r0 - c.kv_heads;
-  const int64_t row = c.row(page, h, place);
-  uint8_t *pool = (key ? c.k : c.v) + row * (D * FMT / 8);
-  uint32_t o[FMT / 4];
-  encode8<FMT>(x[0], e, o);
-  if (FMT == 8) {
-    reinterpret_cast<uint32_t *>(pool)[sub] = o[0];
-    reinterpret_cast<uint32_t *>(pool)[D / 8 + sub] = o[1];
-    if (sub == 0) (key ? c.k_exp : c.v_exp)[row] = (int8_t)e;
-  } else {
-    reinterpret_cast<uint2 *>(pool)[sub] = make_uint2(o[0], o[1]);
-    reinterpret_cast<uint2 *>(pool)[D / 8 + sub] = make_uint2(o[FMT / 4 - 2], o[FMT / 4 - 1]);
-  }
-  if (key && sub == 0) {
-    const int64_t i = ((int64_t)b * c.kv_heads + h) * c.cap + place;
-    if (c.positions) c.positions[i] = at;
-    if (c.scores) c.scores[i] = 0.0f;
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = __float_as_uint(x[k][i]) & 0x7FFFFFFFu;
+        top = a < 0x7F800000u && a > top ? a : top;
+      }
+#pragma unroll
+      for (int d = GW / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+      e = top ? max(f32_floor_log2(top) - 3, -126) : 0;
+    }
+    if (page < 0 || r >= kv_rows) continue;
+    const int h = key ? r : r - c.kv_heads;
+    const int64_t row = c.row(page, h, place);
+    uint8_t *pool = (key ? c.k : c.v) + row * (D * FMT / 8);
+    uint32_t o[FMT / 4];
+    encode8<FMT>(x[k], e, o);
+    if (FMT == 8) {
+      reinterpret_cast<uint32_t *>(pool)[sub] = o[0];
+      reinterpret_cast<uint32_t *>(pool)[D / 8 + sub] = o[1];
+      if (sub == 0) (key ? c.k_exp : c.v_exp)[row] = (int8_t)e;
+    } else {
+      reinterpret_cast<uint2 *>(pool)[sub] = make_uint2(o[0], o[1]);
+      reinterpret_cast<uint2 *>(pool)[D / 8 + sub] = make_uint2(o[FMT / 4 - 2], o[FMT / 4 - 1]);
+    }
+    if (key && sub == 0) {
+      const int64_t i = ((int64_t)b * c.kv_heads + h) * c.cap + place;
+      if (c.positions) c.positions[i] = at;
+      if (c.scores) c.scores[i] = 0.0f;
+    }
   }
 }
 
@@ -264,7 +276,8 @@ int launch_append(AppendParams p, cudaStream_t s) {
   const bool few = (int64_t)p.tokens * ((heads + RPW - 1) / RPW) < (int64_t)sm_count() * 48;
   const int rows = few ? RPW : RPW * U;
   p.q_warps = (heads + rows - 1) / rows;
-  const dim3 grid(blocks, p.q_warps + (2 * p.c.kv_heads + RPW - 1) / RPW);
+  const int kv = RPW * (few ? 1 : kv_unroll(U));
+  const dim3 grid(blocks, p.q_warps + (2 * p.c.kv_heads + kv - 1) / kv);
   return few ? launch_early(k_kv_append<T, D, FMT, 1>, grid, kAppendThreads, 0, s, "k_kv_append", p)
              : launch_early(k_kv_append<T, D, FMT, U>, grid, kAppendThreads, 0, s, "k_kv_append", p);
 }
