@@ -401,9 +401,10 @@ def bp32_to_f64(codes: torch.Tensor, row_exp=None, col_exp=None) -> torch.Tensor
 _ACT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _act(t, name: str, rows, heads, cache, dtype=None) -> torch.Tensor:
+def _act(t, name: str, rows, heads, cache, dtype=None):
     """`t` as [rows, heads, head_dim] activations that the cache's kernels can
-    read: heads contiguous, rows 16 bytes apart or more (copied if not)."""
+    read: heads contiguous, rows 16 bytes apart or more (copied if not); its
+    address and row stride."""
     if not isinstance(t, torch.Tensor) or t.device != cache.device:
         raise ValueError(f"{name} must be a CUDA tensor on {cache.device}")
     dt, D, shape = t.dtype, cache.head_dim, t.shape
@@ -414,10 +415,11 @@ def _act(t, name: str, rows, heads, cache, dtype=None) -> torch.Tensor:
         raise ValueError(f"{name} must be {['rows' if rows is None else rows, 'heads' if heads is None else heads, D]}, "
                          f"got {list(shape)}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s1 != D and shape[1] > 1) or s0 & (3 if dt == torch.float32 else 7) or s0 < shape[1] * D or \
-            t.data_ptr() & 15:
+    at = t.data_ptr()
+    if s2 != 1 or (s1 != D and shape[1] > 1) or s0 & (3 if dt == torch.float32 else 7) or s0 < shape[1] * D or at & 15:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        return t, t.data_ptr(), shape[1] * D
+    return t, at, s0
 
 
 def _ints(t, name: str, n: int, cache):
@@ -441,8 +443,8 @@ def _like(out, q: torch.Tensor, name: str) -> torch.Tensor:
 
 def _call(fn, device, *args):
     """fn(*args, stream) on `device`'s current stream, with `device` current."""
-    i = device.index
-    if torch.cuda.current_device() != i:
+    i = device.index          # (tensors of the device exist: CUDA is initialised)
+    if torch._C._cuda_getDevice() != i:
         with torch.cuda.device(i):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
@@ -464,38 +466,36 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=Non
     and rounded once, queries in fp32; returns the rotated queries (or None).
     A bp8 cache stores each row as round-to-nearest bp8 codes of x / 2^e, e =
     floor(log2 max|x|) - 3; a bp16 cache as round-to-nearest-even bp16 codes."""
-    k = _act(k, "k", None, cache.kv_heads, cache)
+    k, kp, ks = _act(k, "k", None, cache.kv_heads, cache)
     dt = k.dtype
     n = k.shape[0]
-    if not isinstance(v, torch.Tensor) or v.dtype != dt or v.shape != k.shape or v.stride() != k.stride() or \
-            v.device != cache.device or v.data_ptr() & 15:
-        v = _act(v, "v", n, cache.kv_heads, cache, dt)
+    v, vp, vs = _act(v, "v", n, cache.kv_heads, cache, dt)
     rows = heads = qs = 0
     cp = sp = qp = op = None
     if cos is not None or sin is not None:
         if not isinstance(cos, torch.Tensor) or not isinstance(sin, torch.Tensor):
             raise ValueError("cos and sin are tensors and come together")
-        shape = cos.shape
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or sin.shape != shape or \
-                shape[1] * 2 != cache.head_dim or cos.device != cache.device or sin.device != cache.device or \
+        shape, dev = cos.shape, cache.device
+        if not cos.dtype == sin.dtype == torch.float32 or len(shape) != 2 or sin.shape != shape or \
+                shape[1] * 2 != cache.head_dim or cos.device != dev or sin.device != dev or \
                 not cos.is_contiguous() or not sin.is_contiguous():
             raise ValueError(f"cos and sin must be contiguous float32 CUDA tensors [rows, {cache.head_dim // 2}]")
         rows, cp, sp = shape[0], cos.data_ptr(), sin.data_ptr()
     if q is not None:
         if cos is None:
             raise ValueError("queries are only rotated: give cos and sin")
-        q = _act(q, "q", n, None, cache, dt)
+        q, qp, qs = _act(q, "q", n, None, cache, dt)
         q_out = _like(q_out, q, "q_out")
-        heads, qs, qp, op = q.shape[1], q.stride(0), q.data_ptr(), q_out.data_ptr()
+        heads, op = q.shape[1], q_out.data_ptr()
     if (places is None) != (seqs is None):
         raise ValueError("seqs and places come together")
     if not 0 <= layer < cache.layers:
         raise ValueError(f"layer {layer} of {cache.layers}")
     if places is None and n != cache.batch:
         raise ValueError(f"{n} tokens for {cache.batch} sequences: give seqs and places")
-    _call(_lib.lib().bp_kv_append, cache.device, cache._ref, layer, _ACT[dt], n, k.data_ptr(), k.stride(0),
-          v.data_ptr(), v.stride(0), qp, heads, qs, cp, sp, rows, _ints(positions, "positions", n, cache),
-          _ints(seqs, "seqs", n, cache), _ints(places, "places", n, cache), op)
+    _call(_lib.lib().bp_kv_append, cache.device, cache._ref, layer, _ACT[dt], n, kp, ks, vp, vs, qp, heads, qs, cp,
+          sp, rows, _ints(positions, "positions", n, cache), _ints(seqs, "seqs", n, cache),
+          _ints(places, "places", n, cache), op)
     return None if q is None else q_out
 
 
@@ -513,7 +513,7 @@ def paged_attention(cache, q: torch.Tensor, layer: int = 0, scale: float | None 
     bound of the lengths keeps the workspace of `accumulate` small.  The order of
     the sums follows from the lengths of the whole batch: the same call gives
     the same bits, another batch may round differently."""
-    q = _act(q, "q", cache.batch, None, cache)
+    q, qp, qs = _act(q, "q", cache.batch, None, cache)
     heads, dev, dt = q.shape[1], cache.device, q.dtype
     out = _like(out, q, "out")
     lse = torch.empty((cache.batch, heads), dtype=torch.float32, device=dev) if return_lse else None
@@ -531,8 +531,8 @@ def paged_attention(cache, q: torch.Tensor, layer: int = 0, scale: float | None 
         need = L.bp_paged_attention_workspace_size(cache._ref, heads, max_length, accumulate)
         if len(cache._workspace) < 64:
             cache._workspace[heads, max_length, accumulate] = need
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _call(L.bp_paged_attention, dev, cache._ref, layer, _ACT[dt], heads, q.data_ptr(), q.stride(0), out.data_ptr(),
+    ws = q.new_empty(need >> 1 if dt != torch.float32 else need >> 2)      # (need is a multiple of 256)
+    _call(L.bp_paged_attention, dev, cache._ref, layer, _ACT[dt], heads, qp, qs, out.data_ptr(),
           None if lse is None else lse.data_ptr(), cache.head_dim ** -0.5 if scale is None else scale, max_length,
           accumulate, ws.data_ptr(), need)
     return (out, lse) if return_lse else out

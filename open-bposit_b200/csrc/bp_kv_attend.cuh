@@ -45,6 +45,7 @@
 #pragma once
 #include <math.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "bp_kv.cuh"
@@ -839,13 +840,18 @@ template <int FMT, int D, typename T>
 int launch_kv_attend_one(const AttendParams &p, int grid, cudaStream_t s) {
   using C = AttendCfg<FMT, D, T>;
   static_assert(C::SMEM <= 232448, "shared memory per CTA");
+  static std::atomic<bool> ready[128];       // per device: the opt-in to shared memory, and where it starts
   int device = 0, reserved = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return set_error(kENoDev, "k_kv_attend: no device");
-  if (cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, device) != cudaSuccess ||
-      reserved != kSharedReserved)
-    return set_error(kENoDev, "k_kv_attend: shared memory starts at %d, not %d", reserved, kSharedReserved);
-  cudaError_t e = cudaFuncSetAttribute(k_kv_attend<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) return set_error(kECuda, "k_kv_attend: %s", cudaGetErrorString(e));
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 128)
+    return set_error(kENoDev, "k_kv_attend: no device");
+  if (!ready[device].load(std::memory_order_relaxed)) {
+    if (cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, device) != cudaSuccess ||
+        reserved != kSharedReserved)
+      return set_error(kENoDev, "k_kv_attend: shared memory starts at %d, not %d", reserved, kSharedReserved);
+    cudaError_t e = cudaFuncSetAttribute(k_kv_attend<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return set_error(kECuda, "k_kv_attend: %s", cudaGetErrorString(e));
+    ready[device].store(true, std::memory_order_relaxed);
+  }
   return launch_early(k_kv_attend<FMT, D, T>, dim3(grid), C::NW * 32, C::SMEM, s, "k_kv_attend", p);
 }
 template <int FMT, typename T>
