@@ -79,50 +79,60 @@ __device__ __forceinline__ int block_rank(bool flag, Scan &s, int *total) {
   return before + __popc(mask & ((1u << lane) - 1u));
 }
 
-// Copies entry src's rows of codes, exponents, position and score to entry dst,
-// 16 bytes a thread and four entries at a time, for `moves` pairs of a row.
+// Moves `moves` entries of a row from places src to places dst, NT at a time: a
+// thread per entry looks up the pages and moves exponents, position and score,
+// then all threads copy the codes, 16 bytes each, several on their way at once.
+// 192 rows of 8192 64-wide bp8 entries cut to 2048, about 1500 entries moved in
+// each: 37 us, 27 of them for the moves, whose scattered 32-byte sectors are 120
+// MB (43 us when each of an entry's threads looked up its pages).
+constexpr uint32_t kNone = ~0u;        // row of an entry whose page is outside the pool; pools have fewer rows
 template <int NT, typename Index>
 __device__ __forceinline__ void move_entries(const EvictParams &p, int64_t r, int b, int hk, int64_t layer_rows,
-                                             const Index *src, const Index *dst, int moves) {
+                                             const Index *src, const Index *dst, int moves, uint2 *rows) {
   const KvView &c = p.c;
   const int tid = threadIdx.x, vecs = c.dim * (c.fmt / 8) / 16, per = 2 * vecs;
   const int first = tid / per, piece = tid - first * per, step = NT / per;
   const bool value = piece >= vecs;
-  const int x = value ? piece - vecs : piece;
-  uint4 *pool = reinterpret_cast<uint4 *>(value ? c.v : c.k) + x;
-  int8_t *exps = value ? c.v_exp : c.k_exp;
+  uint4 *pool = reinterpret_cast<uint4 *>(value ? c.v : c.k) + layer_rows * vecs + (value ? piece - vecs : piece);
+  int8_t *ke = c.k_exp + layer_rows, *ve = c.v_exp + layer_rows;
   int32_t *pos = c.positions + r * c.cap;
   float *scores = c.scores ? c.scores + r * c.cap : nullptr;
   int32_t *keep = p.keep ? p.keep + r * p.budget : nullptr;
-  if (first < step)
-    for (int e = first; e < moves; e += 4 * step) {
-      uint4 code[4];
-      int8_t ex[4];
-      int64_t to[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        to[j] = -1;
-        const int k = e + j * step;
-        if (k >= moves) continue;
-        const int pf = c.page_of(b, src[k]), pt = c.page_of(b, dst[k]);
-        if (pf < 0 || pt < 0) continue;
-        const int64_t from = layer_rows + c.row(pf, hk, src[k]);
-        to[j] = layer_rows + c.row(pt, hk, dst[k]);
-        code[j] = pool[from * vecs];
-        if (x == 0 && exps) ex[j] = exps[from];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (to[j] >= 0) {
-          pool[to[j] * vecs] = code[j];
-          if (x == 0 && exps) exps[to[j]] = ex[j];
+  for (int base = 0; base < moves; base += NT) {
+    if (base + tid < moves) {
+      const int s = src[base + tid], d = dst[base + tid];
+      const int pf = c.page_of(b, s), pt = c.page_of(b, d), ps = pos[s];
+      const float score = scores ? scores[s] : 0.0f;
+      uint2 row = make_uint2(kNone, kNone);
+      if (pf >= 0 && pt >= 0) {
+        row = make_uint2((uint32_t)c.row(pf, hk, s), (uint32_t)c.row(pt, hk, d));
+        if (c.fmt == 8) {
+          const int8_t x = ke[row.x], y = ve[row.x];
+          ke[row.y] = x;
+          ve[row.y] = y;
         }
+      }
+      pos[d] = ps;
+      if (scores) scores[d] = score;
+      if (keep) keep[d] = s;
+      rows[tid] = row;
     }
-  for (int k = tid; k < moves; k += NT) {
-    const int s = src[k], d = dst[k];
-    pos[d] = pos[s];
-    if (scores) scores[d] = scores[s];
-    if (keep) keep[d] = s;
+    __syncthreads();
+    const int n = min(NT, moves - base);
+    if (first < step)
+      for (int e = first; e < n; e += 4 * step) {
+        uint4 code[4];
+        uint2 row[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          row[j] = e + j * step < n ? rows[e + j * step] : make_uint2(kNone, kNone);
+          if (row[j].y != kNone) code[j] = pool[(int64_t)row[j].x * vecs];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (row[j].y != kNone) pool[(int64_t)row[j].y * vecs] = code[j];
+      }
+    __syncthreads();
   }
 }
 
@@ -151,7 +161,9 @@ __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
       for (int i = tid; i < M; i += NT) keep[i] = i < n ? i : -1;
     return;
   }
-  __shared__ int hist[kBins], count[E + 1], warp_sum[32];
+  __shared__ __align__(8) int hist[kBins];          // and then the rows of entries that move
+  static_assert(NT * 8 <= kBins * 4, "a pair of rows per thread");
+  __shared__ int count[E + 1], warp_sum[32];
   __shared__ uint32_t red[3][32], found[3];
   __shared__ uint16_t src[NT * KPT / 2], dst[NT * KPT / 2];
   const float *w = p.weights + (int64_t)r * c.cap;
@@ -285,7 +297,7 @@ __global__ void __launch_bounds__(NT) k_kv_evict_row(EvictParams p) {
     if (i < M && k && keep) keep[i] = i;
   }
   __syncthreads();
-  move_entries<NT>(p, r, b, hk, layer * c.layer_rows, src, dst, count[E] >> 16);
+  move_entries<NT>(p, r, b, hk, layer * c.layer_rows, src, dst, count[E] >> 16, reinterpret_cast<uint2 *>(hist));
 }
 
 // The same for rows that do not fit a block's registers: the weights are read
@@ -311,7 +323,8 @@ __global__ void __launch_bounds__(kThreads) k_kv_evict_long(EvictParams p) {
     return;
   }
   __shared__ Scan scan;
-  __shared__ int hist[kBins], warp_sum[kWarps], s_front;
+  __shared__ __align__(8) int hist[kBins];          // and then the rows of entries that move
+  __shared__ int warp_sum[kWarps], s_front;
   __shared__ uint32_t found[3];
   __shared__ int32_t queue[kQueue], src[kThreads], dst[kThreads];
   const float *w = p.weights + r * c.cap;
@@ -397,8 +410,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_evict_long(EvictParams p) {
     head += total;
     held -= total;
     bp += kThreads;
-    move_entries<kThreads>(p, r, b, hk, layer * c.layer_rows, src, dst, total);
-    __syncthreads();
+    move_entries<kThreads>(p, r, b, hk, layer * c.layer_rows, src, dst, total, reinterpret_cast<uint2 *>(hist));
   }
   // front places behind the last one scanned: the back scan found no more movers, all are kept
   if (keep)
