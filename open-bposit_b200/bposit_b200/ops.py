@@ -557,7 +557,7 @@ def kv_evict(cache, budget: int, recent: int = 0, sinks: int = 0, weights=None) 
         raise ValueError("budget must be positive, recent and sinks not negative")
     if max(budget, recent, sinks) > 0x7FFFFFFF:
         raise ValueError("budget, recent and sinks are 32-bit numbers")
-    keep = torch.empty((cache.layers, cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
+    keep = cache.lengths.new_empty((cache.layers, cache.batch, cache.kv_heads, budget))
     _call(_lib.lib().bp_kv_evict, cache.device, cache._ref, None if weights is None else weights.data_ptr(), budget,
           recent, sinks, keep.data_ptr())
     return keep
