@@ -85,9 +85,7 @@ class DecoderLayer(torch.nn.Module):
         qkv = self.qkv(self.ln1(x)).view(B, nh + 2 * nkv, hd)
         q, k, v = qkv.split([nh, nkv, nkv], dim=1)
         q = ops.kv_append(cache, k, v, q=q, cos=cos, sin=sin, positions=positions, layer=layer)
-        # (a captured step is replayed on longer sequences than the host knows of now)
-        bound = None if torch.cuda.is_current_stream_capturing() else cache.longest
-        a = ops.paged_attention(cache, q, layer=layer, max_length=bound, accumulate=cache.scores is not None)
+        a = ops.paged_attention(cache, q, layer=layer, max_length=cache.bound, accumulate=cache.scores is not None)
         x = x + self.o(a.reshape(B, nh * hd))
         g, u = self.gate_up(self.ln2(x)).chunk(2, dim=-1)
         return x + self.down(F.silu(g) * u)

@@ -124,6 +124,7 @@ class PagedKVCache:
         self._struct = _Struct(8 if bp8 else 16, layers, pages, page, heads, dim, batch, per, ptr(k), ptr(v),
                                ptr(k_exp), ptr(v_exp), ptr(table), ptr(self.lengths), ptr(positions), ptr(scores))
         self._ref = ctypes.byref(self._struct)
+        self._replayed = False   # a change of the lengths was captured
         self._workspace = {}     # bytes that paged_attention needs, by its arguments
 
     def __setattr__(self, name, value):
@@ -136,8 +137,8 @@ class PagedKVCache:
         """Make room for n more entries in every sequence (an int), or for n[b]
         in sequence b (an int32 tensor of which no value is above `most`); they
         are written by ``ops.kv_append`` in every layer.  ``longest`` follows on
-        the host as a bound of all lengths (not when a captured graph replays
-        this: then add to ``longest`` what the replays added)."""
+        the host as a bound of all lengths, but not when a captured graph replays
+        this: entries that replays put past the capacity are dropped."""
         if not isinstance(n, int) and most is None:
             raise ValueError("give `most`, a bound of the counts that the host knows")
         more = n if isinstance(n, int) else int(most)
@@ -146,18 +147,33 @@ class PagedKVCache:
         longest = self.longest + more
         if longest > self.capacity:
             raise ValueError(f"{longest} entries do not fit a capacity of {self.capacity}")
+        self._note_capture()
         (self.lengths if self._counts is None else self._counts).add_(n)
         self.longest = longest
+
+    def _note_capture(self) -> bool:
+        now = torch.cuda.is_current_stream_capturing()
+        self._replayed = self._replayed or now
+        return now
+
+    @property
+    def bound(self) -> int | None:
+        """``longest`` as the ``max_length`` of ``ops.paged_attention``; None, the
+        capacity, in a call that is captured and once a change of the lengths was,
+        since replays move them without the host's knowledge."""
+        return None if self._replayed or torch.cuda.is_current_stream_capturing() else self.longest
 
     def evict(self, budget: int, recent: int = 0, sinks: int = 0, weights=None):
         """``ops.kv_evict`` on all layers; lengths above `budget` become `budget`.
         Returns the places that the kept entries came from."""
         keep = ops.kv_evict(self, budget, recent=recent, sinks=sinks, weights=weights)
         self.lengths.clamp_(max=budget)
-        self.longest = min(self.longest, budget)
+        if not self._note_capture():
+            self.longest = min(self.longest, budget)
         return keep
 
     def reset(self):
         """Forget all entries (pages keep their contents)."""
         (self.lengths if self._counts is None else self._counts).zero_()
-        self.longest = 0
+        if not self._note_capture():
+            self.longest = 0

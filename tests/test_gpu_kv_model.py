@@ -105,16 +105,21 @@ def test_a_captured_step_goes_on_with_every_replay(track):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = m.step(token, caches[1], tables)
-    for t in tokens[1:]:
+    for t in tokens[1:5]:
         token.copy_(t)
         graph.replay()
         got.append(out.clone())
+    assert caches[1].longest == 32 and caches[1].bound is None and caches[0].bound == 36
+    got.append(m.step(tokens[5], caches[1], tables))      # and without the graph again
     # the entries are the same; the split of the sums does not depend on max_length
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert caches[1].lengths.tolist() == [36, 23] and torch.equal(caches[0].k, caches[1].k)
     if track:
         assert torch.equal(caches[0].scores, caches[1].scores)
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            caches[0].evict(5)                            # captured, not run: the host still knows the lengths
+        assert caches[0].longest == 36 and caches[0].bound is None
 
 
 def test_steps_and_evictions_keep_what_they_promise():
