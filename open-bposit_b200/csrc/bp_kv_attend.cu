@@ -183,7 +183,7 @@ int attend_check(const bp_kv_cache *cache, int layer, int heads, int max_length,
   if (accumulate && !cache->scores) return set_error(kEInval, "%s: the cache keeps no scores", what);
   *max_len = max_length && max_length < c->cap ? max_length : c->cap;
   const int64_t rows = (int64_t)cache->batch * cache->kv_heads * ((heads / cache->kv_heads + 7) / 8);
-  if (rows * ((*max_len + 15) / 16) > 0x7FFFFF00 ||
+  if (rows * ((*max_len + 15) / 16 + kRowUnits) > 0x7FFFFF00 ||
       (accumulate && (int64_t)cache->batch * cache->kv_heads * ((*max_len + 255) / 256) > 0x7FFF0000))
     return set_error(kERange, "%s: more work than the call can number", what);
   return kOk;
@@ -246,9 +246,9 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
   p.raw = accumulate ? (float *)(base + l.raw) : nullptr;
   p.gp = raw_heads(p.group);
   rc = p.c.fmt == 8 ? launch_kv_attend8(p, dtype, grid, s) : launch_kv_attend16(p, dtype, grid, s);
-  // (a batch of at most kMinUnits units is one CTA's, and no row of it is in parts)
-  const int64_t units = (int64_t)cache->batch * cache->kv_heads * p.chunks * ((p.max_len + 15) / 16);
-  const int joins = units > kMinUnits ? grid * kHeadsPerRow : 0;
+  // (a batch of at most kOneCta units is one CTA's, and no row of it is in parts)
+  const int64_t units = (int64_t)cache->batch * cache->kv_heads * p.chunks * ((p.max_len + 15) / 16 + kRowUnits);
+  const int joins = units > kOneCta ? grid * kHeadsPerRow : 0;
   const int chunks = accumulate ? (p.max_len + kScoreEntries - 1) / kScoreEntries : 0;
   const int64_t blocks = joins + (int64_t)chunks * cache->batch * cache->kv_heads;
   if (rc == kOk && blocks) {

@@ -32,8 +32,9 @@
 //    their sums, which would drift over thousands of tiles.
 //
 // Work split: rows are cut into units of 16 entries; the units of all rows, in
-// order, are dealt to the CTAs (one per SM) in equal contiguous ranges and
-// within a CTA to its warps, whatever the lengths are.  A warp takes its units
+// order and with some more for every row's start, are dealt to the CTAs (one per
+// SM) in equal contiguous ranges and within a CTA to its warps, whatever the
+// lengths are.  A warp takes its units
 // four at a time (a tile; single ones at the end of a row or of its range),
 // fetches tiles into its own stage (cp.async, 16 bytes a lane: a page table look-up per
 // page and no address work per row) and needs no other warp until its range
@@ -280,9 +281,18 @@ struct Deal {
 // CTAs that take part: at least kMinUnits units each, so that short batches are
 // not cut into parts that cost more to join than to read (8 sequences of 1 to
 // 1500 entries, 14 and 2 heads of 64, bp8: 10.1 us with 8 units, 12.0 with 16,
-// 14.5 with 32; one sequence of 17 entries is one CTA's either way).
-constexpr int kMinUnits = 8;
-__device__ __forceinline__ int active_ctas(int units, int grid) { return min((units + kMinUnits - 1) / kMinUnits, grid); }
+// 14.5 with 32).  What fits kOneCta units stays in one CTA and needs no second
+// kernel (one sequence of 17 entries: 5.3 us, against 5.9 in two).
+constexpr int kMinUnits = 8, kOneCta = 16;
+// Units that a row counts for besides its own, in front of them, when work is
+// dealt: its end and the next one's start leave the pipeline of fetches empty
+// (64 sequences of up to 16384 entries: 52.7 us with 0, 51.5 with 1, 51.3 with 2
+// to 6, 51.7 with 8; 16 sequences of up to 4096 entries of 8 x 128 in bp16: 50.1,
+// 48.4, 48.7 with 2 and 3, 49.5 with 6; 16 x 4096 with scores: 16.7, 16.0, 15.6 from 3 on).
+constexpr int kRowUnits = 3;
+__device__ __forceinline__ int active_ctas(int units, int grid) {
+  return units <= kOneCta ? min(units, 1) : min((units + kMinUnits - 1) / kMinUnits, grid);
+}
 
 template <int FMT, int D, typename T>
 __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(AttendParams p) {
@@ -326,6 +336,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   auto length = [&](int b) { return min(c.length(b), p.max_len); };
+  auto row_cost = [](int n) { return n > 0 ? (n + 15) / 16 + kRowUnits : 0; };
   // units before each sequence
   {
     const int each = (c.batch + NT - 1) / NT;
@@ -335,7 +346,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       if (b < c.batch) {
         const int n = length(b);
         lens(b) = n;
-        mine += (n + 15) / 16 * per_seq;
+        mine += row_cost(n) * per_seq;
       }
     }
     int incl = mine;
@@ -353,7 +364,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       const int b = tid * each + i;
       if (b < c.batch) {
         before(b) = at;
-        at += (lens(b) + 15) / 16 * per_seq;
+        at += row_cost(lens(b)) * per_seq;
       }
     }
     if (tid == NT - 1) before(c.batch) = at;
@@ -388,10 +399,15 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     int b, row, hk, ch, u, count, n;       // sequence, work row of it (hk * chunks + ch), units, entries of the row
   };
   auto units_of = [](int n) { return (n + 15) / 16; };
-  // the tile behind w, which must exist; `left`: units of this warp's range from there on
-  auto advance = [&](Place &w, int left) {
+  int ax = whi;                // where the tile that is fetched next lies in all the work; from whi on: there is none
+  // from tile w, at ax, to the next one
+  auto advance = [&](Place &w) {
+    ax += w.count;
     w.u += w.count;
-    if (w.u >= units_of(w.n)) {
+    const bool next = w.u >= units_of(w.n);
+    if (next) ax += kRowUnits;
+    if (ax >= whi) return;
+    if (next) {
       w.u = 0;
       ++w.row;
       if (++w.ch == p.chunks) {
@@ -405,7 +421,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         w.n = lens(w.b);
       }
     }
-    w.count = min(min(TU, units_of(w.n) - w.u), left);
+    w.count = min(min(TU, units_of(w.n) - w.u), whi - ax);
   };
   // Page of the tile's unit `lane` (-1: the tile has no such unit).
   auto page_of = [&](const Place &w) {
@@ -463,11 +479,12 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     copy_commit();
   };
 
-  Place cur{}, ahead{};        // this tile, and the next to be fetched, `ax` units into all units
+  Place cur{}, ahead{};        // this tile, and the next to be fetched
   Rows rows{};
-  int ax = wlo, page = -1;
+  int page = -1;
   bool bad = false;            // a page of the tile is outside the pool
   auto is_bad = [&](const Place &w, int pg) { return __any_sync(~0u, lane < w.count && (unsigned)pg >= (unsigned)c.pages); };
+  bool first = false;          // there is a tile, and it is the first one
   if (wlo < whi) {
     int a = 0, z = c.batch;                // sequence of the first unit, by bisection
     while (z - a > 1) {
@@ -478,19 +495,23 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     cur.b = a;
     cur.n = lens(a);
     const int r = wlo - before(a), nu = units_of(cur.n);
-    cur.row = r / nu;
-    cur.u = r - cur.row * nu;
+    cur.row = r / (nu + kRowUnits);
+    const int in_row = r - cur.row * (nu + kRowUnits) - kRowUnits;
+    cur.u = max(in_row, 0);
+    ax = wlo + max(-in_row, 0);
+    first = ax < whi;
     cur.hk = cur.row / p.chunks;
     cur.ch = cur.row - cur.hk * p.chunks;
-    cur.count = min(min(TU, nu - cur.u), whi - wlo);
+    cur.count = min(min(TU, nu - cur.u), whi - ax);
+  }
+  if (first) {
     ahead = cur;
     page = page_of(ahead);
     rows_of(ahead, page, rows);
     bad = is_bad(ahead, page);
     fetch(ahead, rows, false);
     fetch(ahead, rows, true);
-    ax += ahead.count;
-    if (ax < whi) advance(ahead, whi - ax);
+    advance(ahead);
   }
   __syncthreads();
   const uint32_t entry = lane * 4 | (kTableAt >> 16) << 8;
@@ -646,13 +667,13 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     }
   };
 
-  for (int x = wlo; x < whi;) {
+  for (bool go = first; go;) {
     // the pages of the tile to be fetched are looked up while this one's keys are worked on
-    const bool more = x + cur.count < whi, fetches = ax < whi;
-    if (fetches) page = page_of(ahead);
+    const bool more = ax < whi;
+    if (more) page = page_of(ahead);
     copy_wait<1>();
     lost |= bad;
-    if (x == wlo || cur.u == 0) {          // a new row: its queries, and an empty state
+    if (first || cur.u == 0) {             // a new row: its queries, and an empty state
       const uint4 *q = reinterpret_cast<const uint4 *>(
           (const T *)p.q + cur.b * p.qs + (int64_t)(cur.hk * p.group + cur.ch * kHeadsPerRow + g) * D + t * (D / 4));
       constexpr int QV = D / 4 * sizeof(T) / 16;
@@ -685,17 +706,17 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     if (TU == 1 || (cur.count == TU && valid >= TT)) {
       float s[TT / 8][2];
       scores(s, 0);
-      if (fetches) rows_of(ahead, page, rows);
+      if (more) rows_of(ahead, page, rows);
       powers(ske, kpow, p.scale);
       __syncwarp();
-      if (fetches) fetch(ahead, rows, false);
+      if (more) fetch(ahead, rows, false);
       else copy_commit();
       const float alpha = weights(s, 0, valid);
       copy_wait<1>();
       powers(sve, vpow, 1.0f);
       values(s, 0, alpha);
       __syncwarp();
-      if (fetches) fetch(ahead, rows, true);
+      if (more) fetch(ahead, rows, true);
       else copy_commit();
     } else {
       copy_wait<0>();
@@ -708,7 +729,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         values(s, i, weights(s, i, valid - i * 16));
       }
       __syncwarp();
-      if (fetches) {
+      if (more) {
         rows_of(ahead, page, rows);
         fetch(ahead, rows, false);
         fetch(ahead, rows, true);
@@ -757,12 +778,12 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         if (lane == 0) rec_row[warp * 2 + slot] = row;
       }
     }
-    x += cur.count;
+    go = more;
+    first = false;
     cur = ahead;
-    if (fetches) {
+    if (more) {
       bad = is_bad(ahead, page);
-      ax += ahead.count;
-      if (ax < whi) advance(ahead, whi - ax);
+      advance(ahead);
     }
   }
   __syncthreads();
@@ -779,7 +800,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     left &= ~parts;
     const RowId id = row_id(p, row);
     const int nu = units_of(lens(id.b));
-    const int x0 = before(id.b) + (row - id.b * per_seq) * nu, x1 = x0 + nu;
+    const int x0 = before(id.b) + (row - id.b * per_seq) * (nu + kRowUnits) + kRowUnits, x1 = x0 + nu;
     // (the CTA that holds the row's last unit is the last one with a part)
     if (x0 >= lo && x1 > hi) {
       open = make_int2(row, deal.part_of(x1 - 1) - cta + 1);
