@@ -108,9 +108,9 @@ struct AttendCfg {
   static constexpr int BACK = NW - (FRONT < NW ? FRONT : NW);
   // offset of what follows the table, from shared address kSharedReserved
   static constexpr int AFTER = 2 * kTableAt - kSharedReserved;
-  // part statistics [NW][2][16], part rows [NW][2], scan [NW + 2]
+  // part statistics [NW][2][16], part rows and their sequences [NW][2], scan [NW + 2]
   static constexpr int META = AFTER + BACK * STAGE;
-  static constexpr int SMEM = META + NW * 2 * 64 + NW * 2 * 4 + (NW + 2) * 4;
+  static constexpr int SMEM = META + NW * 2 * 64 + NW * 2 * 8 + (NW + 2) * 4;
   static __device__ __forceinline__ int stage_at(int warp) {
     return warp < FRONT ? warp * STAGE : AFTER + (warp - FRONT) * STAGE;
   }
@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   constexpr bool F32 = sizeof(T) == 4;
   extern __shared__ __align__(128) uint8_t smem[];
   float *const rec_ml = reinterpret_cast<float *>(smem + C::META);          // [NW][2][m 8, l 8]
-  int *const rec_row = reinterpret_cast<int *>(rec_ml + NW * 32);           // [NW][2]
-  int *const scan = rec_row + NW * 2;
+  int2 *const rec_row = reinterpret_cast<int2 *>(rec_ml + NW * 32);         // [NW][2]: row, sequence
+  int *const scan = reinterpret_cast<int *>(rec_row + NW * 2);
   uint8_t *const table = smem + (kTableAt - kSharedReserved);
   auto before = [=](int b) -> int & { return spare_word(table, b); };
   auto lens = [=](int b) -> int & { return spare_word(table, kMaxBatch + 1 + b); };
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       if (lane >= d) incl += x;
     }
     if (lane == 31) scan[warp] = incl;
-    if (tid < NW * 2) rec_row[tid] = -1;
+    if (tid < NW * 2) rec_row[tid] = make_int2(-1, 0);
     __syncthreads();
     int at = incl - mine;
     for (int w = 0; w < warp; ++w) at += scan[w];
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     cur.u = max(in_row, 0);
     ax = wlo + max(-in_row, 0);
     first = ax < whi;
-    cur.hk = cur.row / p.chunks;
+    cur.hk = p.chunks == 1 ? cur.row : cur.row / p.chunks;
     cur.ch = cur.row - cur.hk * p.chunks;
     cur.count = min(min(TU, nu - cur.u), whi - ax);
   }
@@ -775,7 +775,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
           rec_ml[(warp * 2 + slot) * 16 + g] = m;
           rec_ml[(warp * 2 + slot) * 16 + 8 + g] = l;
         }
-        if (lane == 0) rec_row[warp * 2 + slot] = row;
+        if (lane == 0) rec_row[warp * 2 + slot] = make_int2(row, cur.b);
       }
     }
     go = more;
@@ -792,15 +792,15 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
   // (a row has at most one part in the workspace, its last one here: it ended inside a warp's range)
   static_assert(NW * 2 <= 32 && NW >= kHeadsPerRow, "a part per lane, a head per warp");
   int2 open = make_int2(-1, 0);
-  const int mine = lane < NW * 2 ? rec_row[lane] : -1;
-  for (uint32_t left = __ballot_sync(~0u, mine >= 0); left;) {
-    const int row = __shfl_sync(~0u, mine, __ffs(left) - 1), h = warp;
-    const bool in = mine == row;
+  const int2 mine = lane < NW * 2 ? rec_row[lane] : make_int2(-1, 0);
+  for (uint32_t left = __ballot_sync(~0u, mine.x >= 0); left;) {
+    const int from = __ffs(left) - 1, h = warp;
+    const int row = __shfl_sync(~0u, mine.x, from), b = __shfl_sync(~0u, mine.y, from);
+    const bool in = mine.x == row;
     const uint32_t parts = __ballot_sync(~0u, in);
     left &= ~parts;
-    const RowId id = row_id(p, row);
-    const int nu = units_of(lens(id.b));
-    const int x0 = before(id.b) + (row - id.b * per_seq) * (nu + kRowUnits) + kRowUnits, x1 = x0 + nu;
+    const int in_seq = row - b * per_seq, nu = units_of(lens(b));
+    const int x0 = before(b) + in_seq * (nu + kRowUnits) + kRowUnits, x1 = x0 + nu;
     // (the CTA that holds the row's last unit is the last one with a part)
     if (x0 >= lo && x1 > hi) {
       open = make_int2(row, deal.part_of(x1 - 1) - cta + 1);
@@ -817,13 +817,15 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) O[i] = 0.0f;
+    // (read from every stage at once; what is no part of this row is left out)
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float f = __shfl_sync(~0u, a, 2 * w + 1);
-      if (parts >> (2 * w + 1) & 1) {
-        const float *r = reinterpret_cast<const float *>(smem + C::stage_at(w)) + h * D + lane;
+      const float *r = reinterpret_cast<const float *>(smem + C::stage_at(w)) + h * D + lane;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) O[i] = fmaf(r[i * 32], f, O[i]);
+      for (int i = 0; i < D / 32; ++i) {
+        const float y = r[i * 32];
+        O[i] = parts >> (2 * w + 1) & 1 ? fmaf(y, f, O[i]) : O[i];
       }
     }
     if (const uint32_t last = parts & 0x55555555u) {
@@ -834,7 +836,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       for (int i = 0; i < D / 32; ++i) O[i] = fmaf(r[i * 32], f, O[i]);
     }
     if (x0 >= lo && x1 <= hi) {
-      const int64_t head = head_of(p, id, h);
+      const int hk = p.chunks == 1 ? in_seq : in_seq / p.chunks;
+      const int64_t head = head_of(p, RowId{b, hk, in_seq - hk * p.chunks}, h);
       if (head >= 0) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) ((T *)p.out)[head * D + i * 32 + lane] = from_f32<T>(O[i] / L);
