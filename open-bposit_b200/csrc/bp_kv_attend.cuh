@@ -671,9 +671,8 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     // the pages of the tile to be fetched are looked up while this one's keys are worked on
     const bool more = ax < whi;
     if (more) page = page_of(ahead);
-    copy_wait<1>();
     lost |= bad;
-    if (first || cur.u == 0) {             // a new row: its queries, and an empty state
+    if (first || cur.u == 0) {             // a new row: its queries (while its keys are on their way), an empty state
       const uint4 *q = reinterpret_cast<const uint4 *>(
           (const T *)p.q + cur.b * p.qs + (int64_t)(cur.hk * p.group + cur.ch * kHeadsPerRow + g) * D + t * (D / 4));
       constexpr int QV = D / 4 * sizeof(T) / 16;
@@ -702,6 +701,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       at_row = cur.u;
       lost = bad;
     }
+    copy_wait<1>();
     const int valid = cur.n - cur.u * 16;
     if (TU == 1 || (cur.count == TU && valid >= TT)) {
       float s[TT / 8][2];
