@@ -299,6 +299,8 @@ int bp_bp32_to_f32(const uint32_t *codes, int M, int N, const int32_t *row_exp, 
  * capacity] counts as the nearer bound, and a page number outside [0, pages)
  * is never followed (each call says what it gives instead).
  * head_dim: 32, 64, 96 or 128.  page_size: a power of two from 16 to 1024.
+ * At most 2048 sequences, 1024 kv heads, 2^30 entries a sequence, and fewer
+ * than 2^32 (page, kv head, entry) rows a layer.
  * No reference counterpart (the reference has no model and no cache). */
 typedef struct bp_kv_cache {
   int32_t fmt;         /* 8 or 16 */
