@@ -663,7 +663,6 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
         const int e = i * 32 + lane, y = e & 7;
         pow[(y < 4 ? y : (y - 4) ^ 1) * C::POWROW + (e >> 3) * 2 + (y >> 2)] = exp2_int(exps[e]) * scale;
       }
-      __syncwarp();
     }
   };
 
@@ -707,14 +706,13 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       float s[TT / 8][2];
       scores(s, 0);
       if (more) rows_of(ahead, page, rows);
+      copy_wait<0>();
       powers(ske, kpow, p.scale);
+      powers(sve, vpow, 1.0f);
       __syncwarp();
       if (more) fetch(ahead, rows, false);
       else copy_commit();
-      const float alpha = weights(s, 0, valid);
-      copy_wait<1>();
-      powers(sve, vpow, 1.0f);
-      values(s, 0, alpha);
+      values(s, 0, weights(s, 0, valid));
       __syncwarp();
       if (more) fetch(ahead, rows, true);
       else copy_commit();
@@ -722,6 +720,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
       copy_wait<0>();
       powers(ske, kpow, p.scale);
       powers(sve, vpow, 1.0f);
+      __syncwarp();
 #pragma unroll 1
       for (int i = 0; i < cur.count; ++i) {
         float s[2][2];
