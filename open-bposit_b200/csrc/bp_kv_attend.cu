@@ -40,9 +40,10 @@ __device__ __forceinline__ void join_row(const AttendParams &p, int cta, int h) 
   for (int i = 0; i < kJoinParts / 32; ++i) M = fmaxf(M, m[i]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+  const float at = finite_max(M);
 #pragma unroll
   for (int i = 0; i < kJoinParts / 32; ++i) {
-    m[i] = i * 32 + lane < parts ? ex2(m[i] - M) : 0.0f;       // the part's weight from here on
+    m[i] = i * 32 + lane < parts ? ex2(m[i] - at) : 0.0f;      // the part's weight from here on
     L = i * 32 + lane < parts ? fmaf(l[i], m[i], L) : L;
   }
 #pragma unroll
@@ -103,9 +104,10 @@ __device__ __forceinline__ void add_scores(const AttendParams &p, int bk, int ch
         for (int k = lane; k < at.y; k += 32) M = fmaxf(M, base[(k ? k * 2 : 1) * (rec + 16)]);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+        const float from = finite_max(M);
         for (int k = lane; k < at.y; k += 32) {
           const float *r = base + (k ? k * 2 : 1) * (rec + 16);
-          L = fmaf(r[8], ex2(r[0] - M), L);
+          L = fmaf(r[8], ex2(r[0] - from), L);
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
@@ -114,8 +116,9 @@ __device__ __forceinline__ void add_scores(const AttendParams &p, int bk, int ch
       if (lane == 0) lse[h] = y;
     }
     __syncthreads();
-    // (NaN: a page outside the pool, or a query that is not finite; the kv head keeps its scores)
-    for (int h = 0; h < heads; ++h) lost = lost || isnan(lse[h]);
+    // (NaN: a page outside the pool, or a query that is not finite; -inf: every score is.  Either way the softmax is
+    // NaN and the kv head keeps its scores)
+    for (int h = 0; h < heads; ++h) lost = lost || !(lse[h] > -INFINITY);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int i = first + j * kJoinWarps * 32 + threadIdx.x;

@@ -200,6 +200,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What scores and parts are weighed against: where there is nothing but -inf so far, any number gives them the weight 0.
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ __forceinline__ uint32_t to_tf32(float x) {
   uint32_t y;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
@@ -597,7 +599,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
     mx = fmaxf(m, mx);
-    const float at = mx == -INFINITY ? 0.0f : mx;       // nothing but -inf so far: weigh it with 0
+    const float at = finite_max(mx);
     const float alpha = ex2(m - at);
     m = mx;
     float sum[4] = {l * alpha, 0.0f, 0.0f, 0.0f};
@@ -810,7 +812,7 @@ __global__ void __launch_bounds__(AttendCfg<FMT, D, T>::NW * 32, 1) k_kv_attend(
     float M = mp;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
-    const float a = in ? ex2(mp - M) : 0.0f;
+    const float a = in ? ex2(mp - finite_max(M)) : 0.0f;
     float L = in ? rec_ml[lane * 16 + 8 + h] * a : 0.0f, O[D / 32];
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(~0u, L, d);

@@ -1,0 +1,73 @@
+"""Calls at the edges of what the paged key-value cache documents."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kv_reference as ref
+from test_gpu_kv import make, queries
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- scores of minus infinity ----
+@pytest.mark.parametrize("fmt,dim,page", [("bp8", 64, 64), ("bp16", 128, 16)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("length", [1, 20, 64, 3000])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_an_infinite_query_leaves_the_scores(fmt, dim, page, dtype, length, sign):
+    """Element 0 of every key is positive, so that one infinite element of a query makes every score of its head
+    infinite with one sign: the softmax is NaN whichever it is, in one part or in several."""
+    from bposit_b200 import ops
+    cache = make(2, 2, dim, [length, 50], fmt, page, track=True)
+    (cache.k if fmt == "bp8" else cache.k.view(torch.int16))[..., 0] = 0x50 if fmt == "bp8" else 0x5000
+    q = queries(2, 8, dim, dtype)
+    good, start = ops.paged_attention(cache, q), cache.scores.clone()
+    q[0, 6, 0] = sign * math.inf                    # kv head 1 of sequence 0
+    got, lse = ops.paged_attention(cache, q, accumulate=True, return_lse=True)
+    assert got[0, 6].isnan().all()
+    assert lse[0, 6] == -math.inf if sign < 0 else lse[0, 6].isnan()
+    keep = torch.ones(2, 8, dtype=torch.bool, device="cuda")
+    keep[0, 6] = False
+    assert torch.equal(got[keep], good[keep]) and lse[keep].isfinite().all()
+    assert torch.equal(cache.scores[0, 0, 1], start[0, 0, 1]) and cache.scores.isfinite().all()
+    assert cache.scores[0, 0, 0, :length].ge(start[0, 0, 0, :length]).all()
+    assert cache.scores[0, 0, 0, :length].gt(start[0, 0, 0, :length]).any()
+
+
+@pytest.mark.parametrize("n", [40, 300, 3000])
+def test_scores_that_overflow_downwards_weigh_nothing(orc, n):
+    """The first half of the entries has scores near -1e39, which fp32 does not hold; the others count as if they were
+    alone, also where whole parts of a long row have no other score."""
+    from bposit_b200 import ops
+    cache = make(1, 1, 64, [n], "bp8", 64, track=True)
+    cache.k_exp.zero_()
+    half = n // 2
+    for i in range(-(-n // 64)):
+        p = int(cache.page_table[0, i])
+        lost = (torch.arange(64, device="cuda") + i * 64 < half)
+        cache.k[0, p, 0, :, 0] = torch.where(lost, 0x50, 0).to(torch.uint8)
+    q = queries(1, 4, 64)
+    q[..., 0] = -3e38
+    start = cache.scores.clone()
+    got, lse = ops.paged_attention(cache, q, accumulate=True, return_lse=True)
+    tab = ref.code_values(orc, "bp8")
+    k, v = (ref.held(cache, tab, w, 0, 0, 0, n)[half:] for w in ("k", "v"))
+    x = q[0].double().cpu()
+    s = x @ k.T * 0.125
+    p = torch.softmax(s, dim=-1)
+    # the terms of kv_reference.attention's bound, of the entries that count (element 0 adds exact zeros to them)
+    u = 2.0 ** -24
+    ds = 2 * u * (64 + 8) * (x[:, 1:].abs() @ k[:, 1:].abs().T * 0.125).amax(-1) + u * s.abs().amax(-1) * 4
+    rel = 2 * ds + u * (400 + n / 32)
+    bound = 2 * rel[:, None] * (p @ v.abs())
+    want = p @ v
+    assert ((got[0].double().cpu() - want).abs() <= bound + u * 1.01 * (want.abs() + bound)).all()
+    want = torch.logsumexp(s, dim=-1)
+    assert ((lse[0].double().cpu() - want).abs() <= rel + 4 * u * want.abs()).all()
+    assert torch.equal(cache.scores[0, 0, 0, :half], start[0, 0, 0, :half])
+    want = start[0, 0, 0, half:n].double().cpu() + p.sum(0)
+    tol = (2 * rel[:, None] * p).sum(0) + 5 * u * want.abs()
+    assert ((cache.scores[0, 0, 0, half:n].double().cpu() - want).abs() <= tol).all()
