@@ -296,8 +296,9 @@ int bp_bp32_to_f32(const uint32_t *codes, int M, int N, const int32_t *row_exp, 
  * kv_heads, capacity], indexed by the entry and not by the page.  All arrays
  * are contiguous device memory; k, v, k_exp and v_exp are 16-byte aligned.
  * Every kernel checks what it reads on the device: a length outside [0,
- * capacity] counts as the nearer bound, and a page number outside [0, pages)
- * is never followed (each call says what it gives instead).
+ * capacity] counts as the nearer bound (but the last entry of a sequence longer
+ * than its capacity has no place, see bp_kv_append), and a page number outside
+ * [0, pages) is never followed (each call says what it gives instead).
  * head_dim: 32, 64, 96 or 128.  page_size: a power of two from 16 to 1024.
  * At most 2048 sequences, 1024 kv heads, 2^30 entries a sequence, and fewer
  * than 2^32 (page, kv head, entry) rows a layer.
@@ -340,7 +341,9 @@ typedef struct bp_kv_cache {
  * Token t goes to entry places[t] of sequence seqs[t]; with both NULL, to the
  * last entry (lengths[t] - 1) of sequence t, and tokens must equal batch.  A
  * sequence, entry or page outside the cache drops the write of that token (its
- * q row is still rotated).  Two tokens of a call must not share an entry.
+ * q row is still rotated): an empty sequence has no last entry, and that of a
+ * sequence longer than its capacity is outside the cache.  Two tokens of a call
+ * must not share an entry.
  * positions[t] is token t's rotary position (NULL: its place); where the cache
  * keeps positions and scores they are set to it and to 0.
  * fmt 8: exponent floor(log2(largest finite |x| of the row)) - 3, at least

@@ -460,10 +460,11 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, q=None, cos=None, sin=Non
     layer of a kv.PagedKVCache.  Token t goes to entry places[t] of sequence
     seqs[t] (int32; a pair outside the cache, such as -1, drops the token; two
     tokens must not share an entry), or, without them, to the last entry of
-    sequence t.  With cos, sin [rows, head_dim/2] (float32) keys, and queries q
-    [tokens, heads, head_dim], are rotated by the tables' rows positions[t]
-    (int32; default: the place; NaN outside the tables) on the way, keys in float64
-    and rounded once, queries in fp32; returns the rotated queries (or None).
+    sequence t (dropped if its length is 0 or above the capacity).  With cos, sin
+    [rows, head_dim/2] (float32) keys, and queries q [tokens, heads, head_dim],
+    are rotated by the tables' rows positions[t] (int32; default: the place; NaN
+    outside the tables) on the way, keys in float64 and rounded once, queries in
+    fp32; returns the rotated queries (or None).
     A bp8 cache stores each row as round-to-nearest bp8 codes of x / 2^e, e =
     floor(log2 max|x|) - 3; a bp16 cache as round-to-nearest-even bp16 codes."""
     k, kp, ks = _act(k, "k", None, cache.kv_heads, cache)

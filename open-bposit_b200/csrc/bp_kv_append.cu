@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(AppendParams p) {
     b = p.seqs[t];
     place = p.places[t];
   } else {
-    place = c.length(t) - 1;
+    place = max(c.lengths[t], 0) - 1;      // not cut to the capacity: a token behind it is dropped
   }
   const int at = p.positions ? p.positions[t] : place;
   const int r0 = chunk * RPW * (queries ? U : KU) + grp;

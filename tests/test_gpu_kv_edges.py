@@ -8,6 +8,7 @@ import torch
 
 import kv_reference as ref
 from test_gpu_kv import make, queries
+from test_gpu_kv_model import small
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +72,55 @@ def test_scores_that_overflow_downwards_weigh_nothing(orc, n):
     want = start[0, 0, 0, half:n].double().cpu() + p.sum(0)
     tol = (2 * rel[:, None] * p).sum(0) + 5 * u * want.abs()
     assert ((cache.scores[0, 0, 0, half:n].double().cpu() - want).abs() <= tol).all()
+
+
+# ---- lengths behind the capacity ----
+def contents(cache):
+    return [t.clone().view(torch.uint8) for t in (cache.k, cache.v, cache.k_exp, cache.v_exp, cache.positions,
+                                                  cache.scores) if t is not None]
+
+
+@pytest.mark.parametrize("fmt", ["bp8", "bp16"])
+def test_a_token_behind_the_capacity_is_dropped(fmt):
+    from bposit_b200 import ops
+    cache = make(6, 2, 64, [32] * 6, fmt, 16, track=True)
+    cap = cache.capacity
+    cache.lengths.copy_(torch.tensor([cap + 1, (1 << 31) - 1, cap, -(1 << 31), cap + 2, -1]))
+    old = contents(cache)
+    x = queries(6, 8, 64)
+    ones = torch.ones(cap + 2, 32, device="cuda")
+    got = ops.kv_append(cache, x[:, :2], x[:, 2:4], q=x[:, 4:], cos=ones, sin=ones * 0)
+    held = cache.page_table[2].long()               # sequence 2 alone has a last entry
+    for was, now in zip(old, contents(cache)):
+        if was.shape[1] == cache.pages:
+            was[:, held] = now[:, held]
+        else:
+            was[:, 2] = now[:, 2]
+        assert torch.equal(was, now)
+    assert cache.positions[0, 2, :, cap - 1].eq(cap - 1).all() and not cache.scores[0, 2, :, cap - 1].any()
+    # queries are turned by the token's place: there are rows for cap + 1 and cap + 2, none for the others
+    assert torch.equal(got[[0, 2, 4]], x[[0, 2, 4], 4:]) and got[[1, 3, 5]].isnan().all()
+
+
+def test_steps_replayed_past_the_capacity_lose_no_entry():
+    m = small(2)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    ids = torch.randint(0, 500, (2, 30), generator=g, device="cuda")
+    token = torch.randint(0, 500, (2,), generator=g, device="cuda")
+    tables = m.rope_tables(64)
+    cache = m.new_cache(2, 32, page_size=16, track=True)
+    m.prefill(ids, cache, [30, 10])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m.step(token, cache, tables)
+    for _ in range(2):
+        graph.replay()
+    full = [t.clone() for t in (cache.k, cache.v, cache.k_exp, cache.v_exp)]
+    pages, pos = cache.page_table[0].long(), cache.positions[:, 0].clone()
+    for _ in range(3):
+        graph.replay()
+    assert cache.lengths.tolist() == [35, 15]
+    for was, now in zip(full, (cache.k, cache.v, cache.k_exp, cache.v_exp)):
+        assert torch.equal(was[:, pages], now[:, pages])
+    assert torch.equal(pos, cache.positions[:, 0])
+    assert cache.positions[:, 1, :, :15].eq(torch.arange(15, device="cuda")).all()
