@@ -162,7 +162,7 @@ class QwenShaped(torch.nn.Module):
         enter the empty `cache`.  Returns forward(ids)."""
         B, S = ids.shape
         dev = ids.device
-        if cache.longest or B != cache.batch:
+        if B != cache.batch or not cache.is_empty():
             raise ValueError("prefill needs an empty cache of the batch's size")
         n = [S] * B if lengths is None else [int(x) for x in lengths]
         if len(n) != B or min(n) < 0 or max(n) > S:

@@ -70,8 +70,8 @@ class PagedKVCache:
         kv_heads, page_size] int8) or uint16 (bp16); page_table [batch,
         max_pages] and lengths [batch] int32; positions int32 and scores float32
         [layers, batch, kv_heads, max_pages * page_size].  Nothing is copied.
-        ``longest``, the host's bound of the lengths, starts at the capacity: set
-        it to what the lengths really are before the first ``advance``."""
+        ``longest``, the host's bound of the lengths, starts at the capacity; set
+        it to what the lengths really are, or ``advance`` has to look."""
         c = cls.__new__(cls)
         if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
             raise ValueError("lengths must be a [batch] int32 tensor")
@@ -136,20 +136,30 @@ class PagedKVCache:
     def advance(self, n=1, most: int | None = None):
         """Make room for n more entries in every sequence (an int), or for n[b]
         in sequence b (an int32 tensor of which no value is above `most`); they
-        are written by ``ops.kv_append`` in every layer.  ``longest`` follows on
-        the host as a bound of all lengths, but not when a captured graph replays
-        this: entries that replays put past the capacity are dropped."""
+        are written by ``ops.kv_append`` in every layer.  Refused where they do
+        not fit.  ``longest`` follows on the host as a bound of all lengths; the
+        lengths themselves are read from the device (the host waits for it) only
+        where that bound says that the entries do not fit, or cannot be trusted
+        since such a call was captured.  Replays of a captured call are not
+        refused: entries that they put past the capacity are dropped."""
         if not isinstance(n, int) and most is None:
             raise ValueError("give `most`, a bound of the counts that the host knows")
         more = n if isinstance(n, int) else int(most)
         if more < 0:
             raise ValueError("counts of new entries are not negative")
         longest = self.longest + more
+        if (longest > self.capacity or self._replayed) and not torch.cuda.is_current_stream_capturing() and \
+                (more <= self.capacity or not isinstance(n, int)):
+            longest = self._longest_held(n)
         if longest > self.capacity:
             raise ValueError(f"{longest} entries do not fit a capacity of {self.capacity}")
         self._note_capture()
         (self.lengths if self._counts is None else self._counts).add_(n)
         self.longest = longest
+
+    def _longest_held(self, n=0) -> int:
+        """The longest length once n entries more are held, read from the device."""
+        return max(0, int((self.lengths.long() + n).max())) if self.batch else 0
 
     def _note_capture(self) -> bool:
         now = torch.cuda.is_current_stream_capturing()
@@ -169,8 +179,13 @@ class PagedKVCache:
         keep = ops.kv_evict(self, budget, recent=recent, sinks=sinks, weights=weights)
         self.lengths.clamp_(max=budget)
         if not self._note_capture():
-            self.longest = min(self.longest, budget)
+            self.longest = min(self.capacity if self._replayed else self.longest, budget)
         return keep
+
+    def is_empty(self) -> bool:
+        """Whether no sequence holds an entry; reads the lengths from the device
+        unless the host knows that there is none."""
+        return (self.longest == 0 and not self._replayed) or self._longest_held() == 0
 
     def reset(self):
         """Forget all entries (pages keep their contents)."""

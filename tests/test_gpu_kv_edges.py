@@ -124,3 +124,67 @@ def test_steps_replayed_past_the_capacity_lose_no_entry():
         assert torch.equal(was[:, pages], now[:, pages])
     assert torch.equal(pos, cache.positions[:, 0])
     assert cache.positions[:, 1, :, :15].eq(torch.arange(15, device="cuda")).all()
+
+
+# ---- lengths that the host does not know ----
+def test_sequences_that_grow_in_turn_fill_the_cache():
+    from bposit_b200.kv import PagedKVCache
+    cache = PagedKVCache(2, 1, 64, 64, page_size=16)
+    for n in ([30, 0], [0, 40], [34, 0], [0, 24]):
+        cache.advance(torch.tensor(n, dtype=torch.int32, device="cuda"), most=max(n))
+    assert cache.lengths.tolist() == [64, 64] and cache.seen.tolist() == [64, 64] and cache.longest == 64
+    for n, most in ((1, None), (torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 1)):
+        with pytest.raises(ValueError, match="capacity"):
+            cache.advance(n, most=most)
+    assert cache.lengths.tolist() == [64, 64] and cache.longest == 64
+    cache.lengths[0], cache.seen[0] = 0, 0              # one sequence ends, another starts in its place
+    cache.advance(torch.tensor([20, 0], dtype=torch.int32, device="cuda"), most=20)
+    assert cache.lengths.tolist() == [20, 64] and cache.longest == 64
+    for n, most in ((1 << 40, None), (torch.tensor([45, 0], dtype=torch.int32, device="cuda"), 1 << 40),
+                    (torch.full((2,), (1 << 31) - 1, dtype=torch.int32, device="cuda"), (1 << 31) - 1)):
+        with pytest.raises(ValueError, match="capacity"):
+            cache.advance(n, most=most)
+    cache.advance(torch.tensor([44, 0], dtype=torch.int32, device="cuda"), most=1 << 40)
+    assert cache.lengths.tolist() == [64, 64]
+
+
+def test_a_cache_over_tensors_finds_its_room():
+    cache = make(2, 2, 64, [30, 5], "bp8", 16)          # capacity 32
+    cache.advance(2)
+    assert cache.lengths.tolist() == [32, 7] and cache.longest == 32
+    with pytest.raises(ValueError, match="capacity"):
+        cache.advance()
+    assert not cache.is_empty()
+    cache.lengths.zero_()
+    assert cache.is_empty()
+
+
+def test_the_host_looks_at_the_lengths_once_they_were_captured():
+    m = small(1)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    ids = torch.randint(0, 500, (2, 20), generator=g, device="cuda")
+    token = torch.randint(0, 500, (2,), generator=g, device="cuda")
+    tables = m.rope_tables(64)
+    cache = m.new_cache(2, 32, page_size=16, track=True)
+    m.prefill(ids, cache, [20, 10])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m.step(token, cache, tables)
+    for _ in range(11):
+        graph.replay()
+    m.step(token, cache, tables)
+    assert cache.lengths.tolist() == [32, 22] and cache.longest == 32
+    with pytest.raises(ValueError, match="capacity"):
+        m.step(token, cache, tables)
+    assert cache.lengths.tolist() == [32, 22]
+    cache.evict(29, recent=4, sinks=1)
+    assert cache.lengths.tolist() == [29, 22] and cache.longest == 29
+    cache.reset()
+    graph.replay()
+    cache.evict(16)
+    assert cache.longest >= 1                           # still a bound
+    with pytest.raises(ValueError, match="empty"):
+        m.prefill(ids, cache)
+    cache.reset()
+    m.prefill(ids, cache)
+    assert cache.lengths.tolist() == [20, 20] and cache.longest == 20
