@@ -16,7 +16,8 @@ also keeps, per (layer, sequence, kv head), the rotary position of every entry
 and the attention weight it has received (``ops.paged_attention(...,
 accumulate=True)``); ``evict`` keeps the entries that were attended to most.
 Tables, lengths and pools may be written by the caller at any time, on the
-stream that the ops run on.
+stream that the ops run on; whoever makes a sequence longer than ``longest``, the
+host's bound of the lengths, sets that too.
 """
 from __future__ import annotations
 
@@ -168,10 +169,11 @@ class PagedKVCache:
 
     @property
     def bound(self) -> int | None:
-        """``longest`` as the ``max_length`` of ``ops.paged_attention``; None, the
-        capacity, in a call that is captured and once a change of the lengths was,
-        since replays move them without the host's knowledge."""
-        return None if self._replayed or torch.cuda.is_current_stream_capturing() else self.longest
+        """``longest`` (1 where nothing is held) as the ``max_length`` of
+        ``ops.paged_attention``; None, the capacity, in a call that is captured
+        and once a change of the lengths was, since replays move them without the
+        host's knowledge."""
+        return None if self._replayed or torch.cuda.is_current_stream_capturing() else max(1, self.longest)
 
     def evict(self, budget: int, recent: int = 0, sinks: int = 0, weights=None):
         """``ops.kv_evict`` on all layers; lengths above `budget` become `budget`.

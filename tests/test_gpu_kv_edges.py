@@ -188,3 +188,11 @@ def test_the_host_looks_at_the_lengths_once_they_were_captured():
     cache.reset()
     m.prefill(ids, cache)
     assert cache.lengths.tolist() == [20, 20] and cache.longest == 20
+
+
+def test_an_empty_cache_has_a_bound():
+    from bposit_b200 import ops
+    from bposit_b200.kv import PagedKVCache
+    cache = PagedKVCache(2, 2, 64, 64)
+    out = ops.paged_attention(cache, queries(2, 4, 64), max_length=cache.bound)
+    assert not out.any()
