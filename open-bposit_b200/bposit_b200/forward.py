@@ -21,7 +21,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
-from .kv import PagedKVCache
+from .kv import PagedKVCache, protected
 from .nn import bpositify
 
 QWEN05 = dict(hidden=896, inter=4864, heads=14, kv_heads=2, head_dim=64, layers=24, vocab=151936,
@@ -201,19 +201,19 @@ class QwenShaped(torch.nn.Module):
 
     @torch.no_grad()
     def generate(self, ids, new_tokens: int, lengths=None, fmt="bp8", page_size: int = 64, budget: int | None = None,
-                 recent: int = 64, sinks: int = 4):
+                 recent: int | None = None, sinks: int | None = None):
         """Greedy continuation of prompts ids [B, S]: [B, new_tokens] token ids.
         With `budget` the cache of every layer and kv head is cut down to that
         many entries whenever a page more has been filled: the `sinks` first and
-        `recent` last ones and, of the others, those that the new tokens
-        attended to most."""
+        `recent` last ones (default 4 and 64, fewer in a budget that does not hold
+        them) and, of the others, those that the new tokens attended to most."""
         if new_tokens < 1:
             raise ValueError("new_tokens must be positive")
         B, S = ids.shape
         if S < 1 or (lengths is not None and min(int(x) for x in lengths) < 1):
             raise ValueError("prompts have at least one token")
-        if budget is not None and budget < 1:
-            raise ValueError("budget must be positive")
+        if budget is not None:
+            recent, sinks = protected(budget, recent, sinks)
         cache = self.new_cache(B, S + new_tokens if budget is None else max(S, budget + page_size) + 1, fmt, page_size,
                                track=budget is not None)
         tables = self.rope_tables(S + new_tokens)

@@ -36,6 +36,21 @@ class _Struct(ctypes.Structure):
                                                "scores")]
 
 
+def protected(budget: int, recent: int | None = None, sinks: int | None = None) -> tuple[int, int]:
+    """(recent, sinks) for evictions to `budget` entries, checked or chosen: the
+    4 first and 64 last tokens, fewer where the budget does not hold them.  More
+    than `budget` of them would compete by place, and the newest would go."""
+    if budget < 1:
+        raise ValueError("budget must be positive")
+    if sinks is None:
+        sinks = min(4, budget // 2 if recent is None else max(0, budget - recent))
+    if recent is None:
+        recent = min(64, budget - sinks)
+    if min(recent, sinks) < 0 or recent + sinks > budget:
+        raise ValueError(f"a budget of {budget} entries does not hold the {sinks} first and {recent} last tokens")
+    return recent, sinks
+
+
 _TENSORS = ("k", "v", "k_exp", "v_exp", "page_table", "lengths", "positions", "scores")
 
 
@@ -177,6 +192,8 @@ class PagedKVCache:
 
     def evict(self, budget: int, recent: int = 0, sinks: int = 0, weights=None):
         """``ops.kv_evict`` on all layers; lengths above `budget` become `budget`.
+        Give no more than `budget` `recent` and `sinks` together: of more, those
+        at the lower places stay, the older ones (``protected`` chooses them).
         Returns the places that the kept entries came from."""
         keep = ops.kv_evict(self, budget, recent=recent, sinks=sinks, weights=weights)
         self.lengths.clamp_(max=budget)

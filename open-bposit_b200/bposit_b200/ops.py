@@ -544,10 +544,13 @@ def kv_evict(cache, budget: int, recent: int = 0, sinks: int = 0, weights=None) 
     more than `budget` entries down to its `budget` best, in place: larger
     weights first (default: cache.scores), equal ones by lower place, NaN last;
     entries at positions below `sinks` or within `recent` of the row's largest
-    position always rank first.  Kept entries behind the budget move into the
-    places in front that were given up.  Returns keep [layers, batch, kv_heads,
-    budget] int32, the place that each entry came from (-1 past the length).
-    The lengths are not changed (PagedKVCache.evict does that too)."""
+    position always rank first (of more than `budget` such entries the lower
+    places stay: keep recent + sinks within the budget).  Kept entries behind the
+    budget move into the places in front that were given up.  Returns keep
+    [layers, batch, kv_heads, budget] int32, the place that each entry came from
+    (-1 past the length).
+    The lengths are not changed (PagedKVCache.evict does that too).  No two
+    sequences may share a page here: each would move entries in it."""
     if cache.positions is None:
         raise ValueError("the cache keeps no positions (track=True)")
     if weights is not None and (not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or

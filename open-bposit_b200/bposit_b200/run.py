@@ -135,6 +135,8 @@ def run_qwen05(a) -> str:
 
 def run_generate(a) -> str:
     from .forward import qwen05, synthetic_ids
+    from .kv import protected
+    recent, sinks = protected(a.budget) if a.budget else (0, 0)
     model = qwen05(layers=a.layers, bposit=not a.fp32)
     ids = synthetic_ids(a.batch, a.seq, seed=a.seed)
     cap = a.seq + 2 * a.new + 2
@@ -145,7 +147,7 @@ def run_generate(a) -> str:
 
     def step():
         if a.budget and cache.longest >= a.budget + cache.page_size:
-            cache.evict(a.budget, recent=cache.page_size, sinks=4)
+            cache.evict(a.budget, recent=recent, sinks=sinks)
         return model.step(token, cache, tables)
 
     step()

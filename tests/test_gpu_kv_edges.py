@@ -196,3 +196,35 @@ def test_an_empty_cache_has_a_bound():
     cache = PagedKVCache(2, 2, 64, 64)
     out = ops.paged_attention(cache, queries(2, 4, 64), max_length=cache.bound)
     assert not out.any()
+
+
+# ---- small budgets ----
+@pytest.mark.parametrize("budget", [1, 2, 5, 12, 30, 67])
+def test_a_small_budget_keeps_the_newest_tokens(budget, monkeypatch):
+    from bposit_b200.kv import PagedKVCache
+    cuts = []
+    evict = PagedKVCache.evict
+
+    def watched(self, *a, **kw):
+        keep = evict(self, *a, **kw)
+        first = self.seen - self.lengths.clamp(max=1)       # position of each row's newest token
+        cuts.append((self.positions[..., :budget] == first[None, :, None, None]).any(-1).all().item())
+        return keep
+
+    monkeypatch.setattr(PagedKVCache, "evict", watched)
+    m = small(2)
+    g = torch.Generator(device="cuda").manual_seed(10)
+    ids = torch.randint(0, 500, (2, 70), generator=g, device="cuda")
+    assert m.generate(ids, 40, lengths=[70, 50], page_size=16, budget=budget).shape == (2, 40)
+    assert len(cuts) >= 2 and all(cuts)
+
+
+def test_a_budget_below_what_it_must_keep_is_refused():
+    m = small(1)
+    ids = torch.zeros(1, 8, dtype=torch.int64, device="cuda")
+    for kw in (dict(recent=21, sinks=4), dict(recent=24, sinks=1), dict(sinks=25), dict(recent=25),
+               dict(recent=-1), dict(sinks=-1), dict(recent=1 << 40)):
+        with pytest.raises(ValueError):
+            m.generate(ids, 4, budget=24, **kw)
+    assert m.generate(ids, 2, budget=24, recent=20, sinks=4).shape == (1, 2)
+    assert m.generate(ids, 2, budget=24, recent=24, sinks=0).shape == (1, 2)
