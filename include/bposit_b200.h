@@ -330,8 +330,8 @@ typedef struct bp_kv_cache {
  * k, v: [tokens, kv_heads, head_dim] of `dtype`, rows of a token contiguous,
  * token stride k_stride / v_stride elements; q (optional): [tokens, heads,
  * head_dim], token stride q_stride, rotated into q_out [tokens, heads,
- * head_dim] (contiguous; it may be q).  16-byte aligned pointers, strides of a
- * multiple of 16 bytes.
+ * head_dim] (contiguous; it may be a contiguous q, and lie on no input in any
+ * other way).  16-byte aligned pointers, strides of a multiple of 16 bytes.
  * cos, sin: fp32 [rope_rows, head_dim / 2]; the rotation of pair (i, i +
  * head_dim/2) at position p is (a c - b s, b c + a s) with c, s from row p: for
  * keys in float64, rounded once to fp32; for queries in fp32 (one rounded
@@ -372,7 +372,8 @@ int bp_kv_append(const bp_kv_cache *cache, int layer, int dtype, int tokens, con
  * 22 bits, codes are exact), sums, softmax statistics and scores are fp32.  The
  * order of the sums follows from the lengths of the whole batch: the same call
  * gives the same bits, another batch may round differently.  Entries at or past
- * max_length are left out (0: capacity); it bounds the workspace.  out may be q.
+ * max_length are left out (0: capacity); it bounds the workspace.  out may be a
+ * contiguous q, and lie on no input in any other way.
  * workspace: at least bp_paged_attention_workspace_size() bytes, 256-byte
  * aligned; NULL takes it stream-ordered from the device's memory pool. */
 int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype, int heads, const void *q, int64_t q_stride,

@@ -37,6 +37,16 @@ struct KvView {
 // Argument checks common to the cache's entry points; fills `view` for `layer`.
 int kv_check(const bp_kv_cache *c, int layer, const char *what, KvView *view);
 
+// Whether contiguous results out [rows, width] lie on inputs in [rows, stride], other than row for row in their place:
+// on a row that may be read after they were written.
+inline bool crosses(const void *in, int64_t stride, const void *out, int64_t rows, int64_t width, int element) {
+  if (rows < 1 || (in == out && (stride == width || rows == 1))) return false;
+  const int64_t d = (int64_t)((intptr_t)out - (intptr_t)in), s = stride * element, w = width * element, n = rows * w;
+  if (d < 0) return d + n > 0;
+  const int64_t r = d / s;               // the row that starts at `out` or before it
+  return (r < rows && d - r * s < w) || (r + 1 < rows && (r + 1) * s < d + n);
+}
+
 // Launches a kernel that begins with, or comes to, griddepcontrol.wait before it
 // touches memory that earlier work of the stream writes: its start overlaps the
 // end of the kernel ahead.

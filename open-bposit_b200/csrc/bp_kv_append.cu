@@ -324,9 +324,12 @@ extern "C" int bp_kv_append(const bp_kv_cache *cache, int layer, int dtype, int 
   const int64_t kvw = (int64_t)cache->kv_heads * cache->head_dim, qw = (int64_t)heads * cache->head_dim;
   if (k_stride < kvw || v_stride < kvw || (q && q_stride < qw))
     return set_error(kEInval, "%s: a token stride is smaller than its rows", what);
-  if (!aligned16(k) || !aligned16(v) || !aligned16(q) || !aligned16(q_out) || !aligned16(cos) || !aligned16(sin) ||
-      k_stride % per || v_stride % per || (q && q_stride % per))
+  if (!aligned16(k) || !aligned16(v) || !aligned16(q) || !aligned16(q_out) || k_stride % per || v_stride % per ||
+      (q && q_stride % per))
     return set_error(kEAlign, "%s: pointers and strides must be multiples of 16 bytes", what);
+  if (q && crosses(q, q_stride, q_out, tokens, qw, es))
+    return set_error(kEInval, "%s: q_out lies on q, but not row for row", what);
+  if (!aligned16(cos) || !aligned16(sin)) return set_error(kEAlign, "%s: tables must be 16-byte aligned", what);
   rc = check_device();
   if (rc != kOk) return rc;
   p.tokens = tokens; p.heads = heads; p.rope_rows = rope_rows;

@@ -223,6 +223,8 @@ extern "C" int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype
     return set_error(kEInval, "%s: the batch stride of q is smaller than its rows", what);
   if (!aligned16(q) || !aligned16(out) || q_stride % per)
     return set_error(kEAlign, "%s: pointers and strides must be multiples of 16 bytes", what);
+  if (crosses(q, q_stride, out, cache->batch, (int64_t)heads * cache->head_dim, 16 / per))
+    return set_error(kEInval, "%s: out lies on q, but not row for row", what);
   if (workspace && ((uintptr_t)workspace & 255u)) return set_error(kEAlign, "%s: workspace not 256-byte aligned", what);
   rc = check_device();
   const int grid = attend_grid();

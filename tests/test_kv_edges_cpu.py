@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import pytest
 
+from test_kv_cpu import append, attend, struct
+
 
 @pytest.mark.parametrize("budget", [1, 2, 3, 5, 8, 12, 67, 68, 69, 1000])
 def test_what_an_eviction_protects_fits_its_budget(budget):
@@ -20,3 +22,31 @@ def test_what_an_eviction_protects_fits_its_budget(budget):
     for bad in (0, -budget):
         with pytest.raises(ValueError):
             protected(bad)
+
+
+# ---- results that would lie on inputs still to be read: found by address, before any device work ----
+# (what the check lets through is refused behind it, by the address of a table or of the workspace)
+CALLS = [(append, "q_out", dict(cos=20)), (attend, "out", dict(ws=128, n=1 << 30))]
+
+
+@pytest.mark.parametrize("dtype,es", [(0, 4), (1, 2), (2, 2)])
+@pytest.mark.parametrize("call,where,behind", CALLS)
+def test_results_may_replace_queries_row_for_row_only(dtype, es, call, where, behind):
+    from bposit_b200 import _lib
+    L = _lib.lib()
+    row, at = 256 * es, 1 << 20                              # two rows of 4 heads of 64
+    for qs, out in ((256, 0), (256, 2 * row), (256, -2 * row), (1024, 5 * row), (1024, -2 * row),
+                    (1024, row), (1024, 2 * row)):
+        rc = call(L, struct(), dtype=dtype, q=at, qs=qs, **{where: at + out}, **behind)
+        assert rc == _lib.BP_EALIGN, (qs, out)
+    for qs, out in ((512, 0), (264, 0), (256, row), (256, -row), (256, 2 * row - 16), (256, 16 - 2 * row),
+                    (1024, row - 16), (1024, 2 * row + 16), (1024, 4 * row), (1024, 5 * row - 16)):
+        rc = call(L, struct(), dtype=dtype, q=at, qs=qs, **{where: at + out}, **behind)
+        assert rc == _lib.BP_EINVAL and b"row for row" in L.bp_last_error(), (qs, out)
+
+
+def test_one_row_of_queries_may_have_any_stride():
+    from bposit_b200 import _lib
+    L = _lib.lib()
+    assert attend(L, struct(batch=1), q=4096, qs=512, out=4096, ws=128, n=1 << 30) == _lib.BP_EALIGN
+    assert append(L, struct(batch=1), tokens=1, q=4096, qs=512, q_out=4096, cos=20) == _lib.BP_EALIGN
