@@ -380,7 +380,7 @@ int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype, int heads
                        void *out, float *lse, float scale, int max_length, int accumulate, void *workspace,
                        size_t workspace_bytes, void *stream);
 
-/* Workspace bytes bp_paged_attention needs. */
+/* Workspace bytes bp_paged_attention needs on the current device. */
 size_t bp_paged_attention_workspace_size(const bp_kv_cache *cache, int heads, int max_length, int accumulate);
 
 /* Cuts every (layer, sequence, kv head) with more than `budget` entries down to

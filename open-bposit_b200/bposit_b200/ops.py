@@ -529,7 +529,8 @@ def paged_attention(cache, q: torch.Tensor, layer: int = 0, scale: float | None 
     L = _lib.lib()
     need = cache._workspace.get((heads, max_length, accumulate))
     if need is None:
-        need = L.bp_paged_attention_workspace_size(cache._ref, heads, max_length, accumulate)
+        with torch.cuda.device(dev):         # (it follows the current device's SMs)
+            need = L.bp_paged_attention_workspace_size(cache._ref, heads, max_length, accumulate)
         if len(cache._workspace) < 64:
             cache._workspace[heads, max_length, accumulate] = need
     ws = q.new_empty(need >> 1 if dt != torch.float32 else need >> 2)      # (need is a multiple of 256)

@@ -50,3 +50,52 @@ def test_one_row_of_queries_may_have_any_stride():
     L = _lib.lib()
     assert attend(L, struct(batch=1), q=4096, qs=512, out=4096, ws=128, n=1 << 30) == _lib.BP_EALIGN
     assert append(L, struct(batch=1), tokens=1, q=4096, qs=512, q_out=4096, cos=20) == _lib.BP_EALIGN
+
+
+# ---- which device a call asks ----
+def test_the_workspace_is_sized_on_the_cache_s_device(monkeypatch):
+    """A cache on another device than the current one: the library asks the current device for its SMs, so both calls
+    are made with the cache's device current."""
+    import types
+
+    import torch
+
+    from bposit_b200 import _lib, ops
+    current, asked = [0], []
+
+    class Device:
+        index = 1
+
+        def __eq__(self, other):
+            return True
+
+        __hash__ = None
+
+    class Guard:
+        def __init__(self, device):
+            self.to = getattr(device, "index", device)
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.to
+
+        def __exit__(self, *a):
+            current[0] = self.was
+
+    def size(*a):
+        asked.append(("size", current[0]))
+        return 256
+
+    def attend(*a):
+        asked.append(("call", current[0]))
+        return 0
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    monkeypatch.setattr(_lib, "lib", lambda: types.SimpleNamespace(bp_paged_attention=attend,
+                                                                   bp_paged_attention_workspace_size=size))
+    cache = types.SimpleNamespace(device=Device(), head_dim=64, batch=2, capacity=64, layers=1, _workspace={}, _ref=None)
+    q = torch.zeros(2, 4, 64)
+    for _ in range(2):
+        ops.paged_attention(cache, q)
+    assert asked == [("size", 1), ("call", 1), ("call", 1)] and current == [0]
