@@ -155,6 +155,13 @@ class QwenShaped(torch.nn.Module):
         return PagedKVCache(batch, c["kv_heads"], c["head_dim"], max_tokens, layers=c["layers"], fmt=fmt,
                             page_size=page_size, track=track, device=self.embed.weight.device)
 
+    def _check_cache(self, cache):
+        """Refuses a cache that the layers cannot use, before its lengths move."""
+        c = self.c
+        if (cache.kv_heads, cache.head_dim) != (c["kv_heads"], c["head_dim"]) or cache.layers < c["layers"]:
+            raise ValueError(f"the cache has {cache.layers} layers of {cache.kv_heads} heads of {cache.head_dim}, the "
+                             f"model {c['layers']} of {c['kv_heads']} of {c['head_dim']}")
+
     @torch.no_grad()
     def prefill(self, ids, cache, lengths=None):
         """The forward of prompts ids [B, S] (padded on the right to S when
@@ -162,6 +169,7 @@ class QwenShaped(torch.nn.Module):
         enter the empty `cache`.  Returns forward(ids)."""
         B, S = ids.shape
         dev = ids.device
+        self._check_cache(cache)
         if B != cache.batch or not cache.is_empty():
             raise ValueError("prefill needs an empty cache of the batch's size")
         n = [S] * B if lengths is None else [int(x) for x in lengths]
@@ -188,6 +196,11 @@ class QwenShaped(torch.nn.Module):
         [B, hidden], its keys and values appended to `cache`.  tables:
         rope_tables of at least the tokens that the sequences will have seen.
         May be captured into a graph: each replay is one step further."""
+        self._check_cache(cache)
+        if ids.shape != (cache.batch,):
+            raise ValueError(f"ids must be one token for each of the cache's {cache.batch} sequences, got {list(ids.shape)}")
+        if cache.seen is None:
+            raise ValueError("a cache over the caller's tensors does not count the tokens seen, which are the positions")
         cache.advance()
         positions = cache.seen - 1
         x = self.embed(ids)

@@ -87,7 +87,9 @@ class PagedKVCache:
         max_pages] and lengths [batch] int32; positions int32 and scores float32
         [layers, batch, kv_heads, max_pages * page_size].  Nothing is copied.
         ``longest``, the host's bound of the lengths, starts at the capacity; set
-        it to what the lengths really are, or ``advance`` has to look."""
+        it to what the lengths really are, or ``advance`` has to look.  Such a
+        cache does not count the tokens seen (``seen`` is None): whoever appends to
+        it gives the positions."""
         c = cls.__new__(cls)
         if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
             raise ValueError("lengths must be a [batch] int32 tensor")

@@ -228,3 +228,26 @@ def test_a_budget_below_what_it_must_keep_is_refused():
             m.generate(ids, 4, budget=24, **kw)
     assert m.generate(ids, 2, budget=24, recent=20, sinks=4).shape == (1, 2)
     assert m.generate(ids, 2, budget=24, recent=24, sinks=0).shape == (1, 2)
+
+
+# ---- calls that a model refuses before it moves a length ----
+def test_steps_that_cannot_be_taken_leave_the_cache_alone():
+    from bposit_b200.kv import PagedKVCache
+    m = small(2)
+    ids = torch.zeros(2, 8, dtype=torch.int64, device="cuda")
+    token, tables = ids[:, 0], m.rope_tables(64)
+    cache = m.new_cache(2, 32, page_size=16)
+    m.prefill(ids, cache)
+    for bad in (ids[:1, 0], torch.zeros(3, dtype=torch.int64, device="cuda"), ids):
+        with pytest.raises(ValueError, match="ids"):
+            m.step(bad, cache, tables)
+    assert cache.lengths.tolist() == [8, 8] and cache.seen.tolist() == [8, 8] and cache.longest == 8
+    over = make(2, 2, 64, [8, 3], "bp8", 16, layers=2)  # over tensors: it has no count of the tokens seen
+    with pytest.raises(ValueError, match="seen"):
+        m.step(token, over, tables)
+    assert over.lengths.tolist() == [8, 3]
+    for other in (PagedKVCache(2, 1, 64, 32, layers=2), PagedKVCache(2, 2, 32, 32, layers=2), PagedKVCache(2, 2, 64, 32)):
+        for call in (lambda: m.step(token, other, tables), lambda: m.prefill(ids, other)):
+            with pytest.raises(ValueError, match="cache"):
+                call()
+        assert not other.lengths.any() and other.longest == 0
