@@ -251,3 +251,78 @@ def test_steps_that_cannot_be_taken_leave_the_cache_alone():
             with pytest.raises(ValueError, match="cache"):
                 call()
         assert not other.lengths.any() and other.longest == 0
+
+
+# ---- the value of every code ----
+def blocks(fmt, dim, n):
+    """Pools of one layer whose row (sequence b, kv head h, entry i) holds `dim` codes that follow one another, turned
+    by i, so that all rows together hold every code at every entry: (codes [batch, 8, n, dim], cache)."""
+    from bposit_b200.kv import PagedKVCache
+    codes, heads = (256, 2) if fmt == "bp8" else (65536, 8)
+    batch = codes // (heads * dim)
+    first = (torch.arange(batch * heads, device="cuda") * dim).view(batch, heads, 1, 1)
+    turn = torch.arange(n, device="cuda")[:, None] + torch.arange(dim, device="cuda")
+    c = first + turn % dim
+    dt = torch.uint8 if fmt == "bp8" else torch.int16
+    pool = torch.zeros(batch, heads, 64, dim, dtype=dt, device="cuda")
+    pool[:, :, :n] = (c if fmt == "bp8" else (c + 32768) % 65536 - 32768).to(dt)
+    pool = pool[None] if fmt == "bp8" else pool[None].view(torch.uint16)
+    exps = {}
+    if fmt == "bp8":
+        exps = {k: torch.zeros(1, batch, heads, 64, dtype=torch.int8, device="cuda") for k in ("k_exp", "v_exp")}
+    table = torch.arange(batch, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    other = torch.zeros_like(pool.view(dt)).view(pool.dtype)
+    return c, pool, other, lambda k, v: PagedKVCache.over(k, v, table, lengths, **exps)
+
+
+CODES = [("bp8", 32), ("bp8", 64), ("bp8", 128), ("bp16", 32), ("bp16", 64), ("bp16", 96), ("bp16", 128)]
+
+
+@pytest.mark.parametrize("fmt,dim", [c for c in CODES if c[1] != 96])
+@pytest.mark.parametrize("n", [1, 64])
+def test_the_value_of_every_code(orc, fmt, dim, n):
+    """One entry has the weight 1 and the others 0, both exactly, so the output is the values of its codes: one entry
+    in a unit by itself, or one of a whole tile of codes of its block."""
+    from bposit_b200 import ops
+    c, values, keys, over = blocks(fmt, dim, n)
+    batch, heads = c.shape[:2]
+    # key element 0 is 1.0 in the chosen entry and 0 in the others: 300 apart in the exponent of 2, e^-300 is 0 in fp32
+    chosen = (torch.arange(batch * heads, device="cuda") * 7 % n).view(batch, heads)
+    plain = keys if fmt == "bp8" else keys.view(torch.int16)
+    plain[0, torch.arange(batch, device="cuda")[:, None], torch.arange(heads, device="cuda"), chosen, 0] = \
+        0x40 if fmt == "bp8" else 0x4000
+    q = torch.zeros(batch, heads, dim, device="cuda")
+    q[..., 0] = 300.0
+    out = ops.paged_attention(over(keys, values), q, scale=1.0)
+    tab = ref.code_values(orc, fmt).float().cuda()
+    want = tab[torch.gather(c, 2, chosen[:, :, None, None].expand(-1, -1, 1, dim))[:, :, 0]]
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("fmt,dim", [c for c in CODES if c[1] != 96])
+@pytest.mark.parametrize("n", [1, 64])
+def test_the_score_of_every_code(orc, fmt, dim, n):
+    """A query head for each column of the keys, with 1 over the power of two of the code there and 0 elsewhere: the
+    score is the code's value between 1 and 2, and the logarithm of the denominator shows it, with one entry or with
+    a tile of equal ones."""
+    from bposit_b200 import ops
+    c, keys, values, over = blocks(fmt, dim, n)
+    batch, heads = c.shape[:2]
+    if n > 1:
+        # every entry of a row holds the same codes
+        plain = keys if fmt == "bp8" else keys.view(torch.int16)
+        plain.copy_(plain[:, :, :, :1].expand(plain.shape).clone())
+    tab = ref.code_values(orc, fmt)
+    v = tab[c[:, :, 0].cpu()]                                    # [batch, heads, dim]
+    size = torch.where(v == 0, 0.0, torch.exp2(1.0 - torch.frexp(v)[1].double()))
+    q = torch.zeros(batch, heads * dim, dim, dtype=torch.float64)
+    at = torch.arange(dim).repeat(heads)
+    q[:, torch.arange(heads * dim), at] = size.reshape(batch, -1)
+    _, lse = ops.paged_attention(over(keys, values), q.float().cuda(), scale=1.0, return_lse=True)
+    score = (v * size).reshape(batch, -1)                        # 0, or from 1 to 2 in magnitude
+    want = score + math.log(n)
+    # half steps: of log2(e) and ln 2 as fp32 numbers, the products with them, the sum with log2(n), at most 9 in base
+    # 2: codes are told apart by 2^-11
+    tol = 2.0 ** -24 * (4 * want.abs() + 9)
+    assert ((lse.double().cpu() - want).abs() <= tol).all()
