@@ -282,15 +282,16 @@ struct Deal {
 };
 // CTAs that take part: at least kMinUnits units each, so that short batches are
 // not cut into parts that cost more to join than to read (8 sequences of 1 to
-// 1500 entries, 14 and 2 heads of 64, bp8: 10.1 us with 8 units, 12.0 with 16,
-// 14.5 with 32).  What fits kOneCta units stays in one CTA and needs no second
+// 1500 entries, 14 and 2 heads of 64, bp8: 8.5 us with 4 units, 8.7 with 8, 9.5
+// with 16, 10.8 with 32; longer batches use every CTA with any of them).  What fits kOneCta units stays in one CTA and needs no second
 // kernel (one sequence of 17 entries: 5.3 us, against 5.9 in two).
 constexpr int kMinUnits = 8, kOneCta = 16;
 // Units that a row counts for besides its own, in front of them, when work is
 // dealt: its end and the next one's start leave the pipeline of fetches empty
-// (64 sequences of up to 16384 entries: 52.7 us with 0, 51.5 with 1, 51.3 with 2
-// to 6, 51.7 with 8; 16 sequences of up to 4096 entries of 8 x 128 in bp16: 50.1,
-// 48.4, 48.7 with 2 and 3, 49.5 with 6; 16 x 4096 with scores: 16.7, 16.0, 15.6 from 3 on).
+// (64 sequences of up to 16384 entries: 52.5 us with 0, 51.4 with 1, 50.6 to 50.9
+// with 2 to 6, 51.0 with 8; 16 sequences of up to 4096 entries of 8 x 128 in bp16:
+// 49.8 with 0, 47.4 with 1, 47.7 with 2 and 3, 48.3 with 6; 16 x 4096 with scores:
+// 16.5 with 0, 15.8 with 1, 15.4 from 3 to 6).
 constexpr int kRowUnits = 3;
 __device__ __forceinline__ int active_ctas(int units, int grid) {
   return units <= kOneCta ? min(units, 1) : min((units + kMinUnits - 1) / kMinUnits, grid);

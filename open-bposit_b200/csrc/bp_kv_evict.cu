@@ -443,9 +443,11 @@ extern "C" int bp_kv_evict(const bp_kv_cache *cache, const float *weights, int b
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)rows);
   // The smallest block that holds a row's weights in its registers; longer rows stream them.  us for 384 rows (one row)
-  // of 64-wide bp8 heads cut by half, at each limit and in the next larger form:
+  // of 64-wide bp8 heads cut by half, at each limit and in the next larger form, where few entries move:
   //   1024: 4.1 (2.8) and 7.4 (3.5)     2048: 7.8 (3.7) and 15.5 (6.6)     8192: 19.3 (7.1) and 34.9 (11.0)
   //   16384: 36.8 (11.4) and 89.8 (28.2); streamed, 32768: 202 (52)
+  // A quarter of the entries moved as well, in the form that is taken:
+  //   1024: 14.5 (6.3)     2048: 26.9 (8.0)     8192: 79 (19.5)     16384: 156 (32)     32768: 563 (120)
   static const char *const name = "k_kv_evict";
   if (p.c.cap <= 256 * 4) return launch_early(k_kv_evict_row<256, 4>, grid, 256, 0, s, name, p);
   if (p.c.cap <= 512 * 4) return launch_early(k_kv_evict_row<512, 4>, grid, 512, 0, s, name, p);
