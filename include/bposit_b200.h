@@ -362,18 +362,19 @@ int bp_kv_append(const bp_kv_cache *cache, int layer, int dtype, int tokens, con
  * multiple of 16 bytes); out: [batch, heads, head_dim] of the same dtype,
  * contiguous; lse (optional): fp32 [batch, heads], the natural logarithm of the
  * softmax's denominator.  An empty sequence gives zeros (lse -inf); one with a
- * page number outside the pool gives NaN, as does a query that is not finite.
- * Scores that overflow to -inf weigh nothing; where all of a head's are -inf
- * its out is NaN and its lse -inf.
+ * page number outside the pool gives NaN, as does a query that is not finite or
+ * a score above fp32's range.  Scores below it (-inf) weigh nothing; where all
+ * of a head's are -inf its out is NaN and its lse -inf.  (fmt 8: q . codes, the
+ * score before the key's exponent and the scale, has to keep that range too.)
  * accumulate = 1 also adds the softmax weight of each entry, summed over the
  * heads that share its kv head, to cache->scores (a kv head with a softmax that
  * is NaN -- a page number outside the pool, a query that is not finite, no score
- * above -inf -- keeps its scores).  Products keep fp32 accuracy (queries and weights are split into
- * 22 bits, codes are exact), sums, softmax statistics and scores are fp32.  The
- * order of the sums follows from the lengths of the whole batch: the same call
- * gives the same bits, another batch may round differently.  Entries at or past
- * max_length are left out (0: capacity); it bounds the workspace.  out may be a
- * contiguous q, and lie on no input in any other way.
+ * above -inf -- keeps its scores).  Products keep fp32 accuracy (queries and
+ * weights are split into 22 bits, codes are exact), sums, softmax statistics and
+ * scores are fp32.  The order of the sums follows from the lengths of the whole
+ * batch: the same call gives the same bits, another batch may round differently.
+ * Entries at or past max_length are left out (0: capacity); it bounds the
+ * workspace.  out may be a contiguous q, and lie on no input in any other way.
  * workspace: at least bp_paged_attention_workspace_size() bytes, 256-byte
  * aligned; NULL takes it stream-ordered from the device's memory pool. */
 int bp_paged_attention(const bp_kv_cache *cache, int layer, int dtype, int heads, const void *q, int64_t q_stride,

@@ -198,9 +198,10 @@ class QwenShaped(torch.nn.Module):
         May be captured into a graph: each replay is one step further."""
         self._check_cache(cache)
         if ids.shape != (cache.batch,):
-            raise ValueError(f"ids must be one token for each of the cache's {cache.batch} sequences, got {list(ids.shape)}")
+            raise ValueError(f"ids must be one token for each of the cache's {cache.batch} sequences, got "
+                             f"{list(ids.shape)}")
         if cache.seen is None:
-            raise ValueError("a cache over the caller's tensors does not count the tokens seen, which are the positions")
+            raise ValueError("a cache over the caller's tensors does not count the tokens seen, the positions")
         cache.advance()
         positions = cache.seen - 1
         x = self.embed(ids)

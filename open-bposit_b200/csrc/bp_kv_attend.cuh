@@ -200,7 +200,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// What scores and parts are weighed against: where there is nothing but -inf so far, any number gives them the weight 0.
+// What scores and parts are weighed against: where there is nothing but -inf so
+// far, any number gives them the weight 0.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ __forceinline__ uint32_t to_tf32(float x) {
   uint32_t y;
@@ -283,7 +284,8 @@ struct Deal {
 // CTAs that take part: at least kMinUnits units each, so that short batches are
 // not cut into parts that cost more to join than to read (8 sequences of 1 to
 // 1500 entries, 14 and 2 heads of 64, bp8: 8.5 us with 4 units, 8.7 with 8, 9.5
-// with 16, 10.8 with 32; longer batches use every CTA with any of them).  What fits kOneCta units stays in one CTA and needs no second
+// with 16, 10.8 with 32; longer batches use every CTA with any of them).  What
+// fits kOneCta units stays in one CTA and needs no second
 // kernel (one sequence of 17 entries: 5.3 us, against 5.9 in two).
 constexpr int kMinUnits = 8, kOneCta = 16;
 // Units that a row counts for besides its own, in front of them, when work is
