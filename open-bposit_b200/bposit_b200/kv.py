@@ -166,8 +166,11 @@ class PagedKVCache:
         if more < 0:
             raise ValueError("counts of new entries are not negative")
         longest = self.longest + more
-        if (longest > self.capacity or self._replayed) and not torch.cuda.is_current_stream_capturing() and \
-                (more <= self.capacity or not isinstance(n, int)):
+        never = more > self.capacity and isinstance(n, int)
+        if torch.cuda.is_current_stream_capturing():
+            if self._replayed and not never:     # an earlier capture was counted, though it moved nothing
+                longest = min(longest, self.capacity)
+        elif (longest > self.capacity or self._replayed) and not never:
             longest = self._longest_held(n)
         if longest > self.capacity:
             raise ValueError(f"{longest} entries do not fit a capacity of {self.capacity}")

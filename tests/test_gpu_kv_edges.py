@@ -190,6 +190,24 @@ def test_the_host_looks_at_the_lengths_once_they_were_captured():
     assert cache.lengths.tolist() == [20, 20] and cache.longest == 20
 
 
+def test_captures_do_not_use_up_the_room():
+    """A captured call moves no length until it is replayed: more of them than entries fit are still captured."""
+    from bposit_b200.kv import PagedKVCache
+    cache = PagedKVCache(1, 1, 64, 16, page_size=16)
+    cache.advance(14)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(4)]
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            cache.advance()
+    assert cache.lengths.tolist() == [14] and cache.longest == 16
+    cache.advance()
+    assert cache.lengths.tolist() == [15] and cache.longest == 15
+    graphs[3].replay()
+    assert cache.lengths.tolist() == [16]
+    with pytest.raises(ValueError, match="capacity"):
+        cache.advance()
+
+
 def test_an_empty_cache_has_a_bound():
     from bposit_b200 import ops
     from bposit_b200.kv import PagedKVCache
